@@ -1150,7 +1150,7 @@ __global__ __launch_bounds__(kKdThreads, 2) void kdlite_head_kernel(HeadArgs h) 
 }
 
 
-// ---- the same head, second form: class-innermost LDS image, packed arithmetic, one exponential per logit ----
+// ---- the same head, second form: class-innermost LDS image, paired arithmetic, one exponential per logit ----
 //
 // What the form above spends per logit is vector arithmetic, not bytes: four 4-byte LDS reads and an address
 // addition per class plane, the interpolation and the softmax statistics one value at a time, a running maximum
@@ -1158,13 +1158,13 @@ __global__ __launch_bounds__(kKdThreads, 2) void kdlite_head_kernel(HeadArgs h) 
 //  * the staged source rows lie [row][column][class] with the class axis padded to CPAD floats (CPAD / 4 odd, so
 //    the sixteen lanes one ds_read_b128 serves together hit sixteen different 16-byte slots): a pixel's four
 //    corners of FOUR classes are four 16-byte reads at immediate offsets, no address arithmetic in the class loop;
-//  * the interpolation and the statistics run on class pairs (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32), with the
+//  * the interpolation and the statistics run on class pairs (two independent fp32 operations each), with the
 //    fused multiply-adds placed as in upsample_bilinear_kernel: the interpolated logits are the same bits;
 //  * the softmax shift of a pixel is not its running maximum but M = the largest logit of its four source pixels
 //    (a table filled once per tile): an interpolated logit is a convex combination of the corners', so s - M <= 0
 //    up to rounding, and the sums never need rescaling.  Should M lie so far above the pixel's own maximum that
 //    sum exp(s - M) leaves the normal range (or a logit is not finite), the pixel is redone with its exact maximum;
-//  * for the integer temperatures (T = 1..4) exp(s - M) = exp((s - M) / T)^T: one exponential and two packed
+//  * for the integer temperatures (T = 1..4) exp(s - M) = exp((s - M) / T)^T: one exponential and two paired
 //    multiplications per logit pair instead of two exponentials per logit;
 //  * the label's logit is interpolated once per pixel behind the class loop instead of selected per class.
 // The teacher comes as prepared probabilities (kd_teacher_prepare_kernel).  LOSS = false: arg-max histogram only.
