@@ -529,6 +529,134 @@ int spice_conv3x3_bn_act_f16(const void *x, const void *weight9, void *y, int64_
                              const float *var, const float *bn_weight, const float *bn_bias, float eps,
                              int32_t relu, void *stream);
 
+/* ------------------------------------------------------------------------- *
+ * (9) Losses over the log-probabilities of given labels, with their gradients:
+ * label log-probabilities, the preference loss (paired log ratios against a
+ * frozen reference policy) and the clipped policy loss with a KL term.  They
+ * stand beside the KD-Lite loss of (2): fine-tuning a pruned network towards
+ * the better of two label maps (or answers), or towards a score of sampled
+ * ones, held near the frozen teacher.  No counterpart in the reference.
+ *
+ * n sequences (pictures) of l positions carry c logits each, at element strides
+ * n_stride / l_stride / c_stride from `data`: [N,C,H,W] is (C*H*W, 1, H*W), token
+ * logits [N,L,V] are (L*V, V, 1), and views of either are taken as they are.
+ * With m = max_c x_c, s = sum_c exp((x_c - m) / T):
+ *   logp = (x_label - m) / T - log s          (0 where the label is ignore_index)
+ * A label that is neither ignore_index nor in [0, c) gives NaN: logp, the loss and
+ * that position's gradient.  Positions with ignore_index are never read; their
+ * gradient is zero.  ignore_index must not be a class.
+ * ------------------------------------------------------------------------- */
+typedef struct spice_logits {
+    const void *data;
+    int32_t dtype; /* 0 = fp32, 1 = fp16, 2 = bf16 */
+    int32_t pad_;
+    int64_t n, l, c;
+    int64_t n_stride, l_stride, c_stride;
+} spice_logits;
+
+typedef struct spice_labels {
+    const int64_t *data;
+    int64_t n_stride, l_stride;
+    int64_t ignore_index;
+} spice_labels;
+
+/* Bytes of workspace of the two losses; nothing in it has to be cleared. */
+size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l);
+
+/* logp [n,l] fp32; stats [n,l,2] fp32 = {m, s} for spice_token_logprobs_grad, or NULL. */
+int spice_token_logprobs(const spice_logits *logits, const spice_labels *labels, float temperature, float *logp,
+                         float *stats, void *stream);
+
+/* grad = scale * d(sum_nl weight[n,l] * logp[n,l]) / d(logits), dense in the order [n][l][c] (class_last) or [n][c][l],
+ * in the logits' type; weight[n*w_n_stride + l*w_l_stride] (a stride may be 0).  device_scale: a further factor in device
+ * memory, or NULL; with unless_one nothing is read or written where that factor is 1 (a gradient taken with the loss
+ * already stands in `grad`, and an upstream factor other than 1 asks for it anew, rounded once). */
+int spice_token_logprobs_grad(const spice_logits *logits, const spice_labels *labels, float temperature, const float *stats,
+                              const float *weight, int64_t w_n_stride, int64_t w_l_stride, float scale,
+                              const float *device_scale, int32_t unless_one, int32_t class_last, void *grad, void *stream);
+
+#define SPICE_PREFERENCE_SIGMOID 0 /* -(1-e) log sigmoid(beta h) - e log sigmoid(-beta h), e = smoothing */
+#define SPICE_PREFERENCE_IPO 1     /* (h - 1/(2 beta))^2; smoothing must be 0 */
+typedef struct spice_preference_params {
+    float temperature;
+    float beta;       /* > 0 */
+    float smoothing;  /* in [0, 0.5) */
+    int32_t loss_type;
+    int32_t average;  /* non-zero: a sequence's log ratio is the mean over its counted positions, else their sum */
+} spice_preference_params;
+
+/* Sequences i < n/2 are preferred to sequences n/2 + i (n even, >= 2).  R_n = sum (or mean) over the counted positions of
+ * logp - ref_logp, h_i = R_i - R_{n/2+i}, total = mean over pairs of the loss of h_i; rewards[n] = beta * R_n.
+ * weight[n] = d total / d logp of every counted position of sequence n: spice_token_logprobs_grad(weight, 1, 0) on the
+ * stats written here is the gradient.  ref_logp [n,l] fp32 (0 or anything finite where ignored: it is not read there).
+ * Sums in fp64, in a fixed order. */
+int spice_preference_loss(const spice_logits *logits, const spice_labels *labels, const float *ref_logp,
+                          const spice_preference_params *params, float *total, float *rewards, float *weight, float *logp,
+                          float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
+#define SPICE_POLICY_TOKEN 0    /* mean over all counted positions */
+#define SPICE_POLICY_SEQUENCE 1 /* mean over the n sequences of the mean over each one's counted positions (none: 0) */
+typedef struct spice_policy_params {
+    float temperature;
+    float clip_low;   /* in [0, 1] */
+    float clip_high;  /* >= 0 */
+    float kl_weight;  /* >= 0; > 0 needs ref_logp */
+    float grad_scale; /* factor of the gradient (a loss scale) */
+    int32_t reduction;
+} spice_policy_params;
+
+/* r = exp(logp - old_logp), A = advantages[n*adv_n_stride + l*adv_l_stride]:
+ *   surrogate = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A),  kl = exp(ref_logp - logp) - (ref_logp - logp) - 1,
+ * both averaged as `reduction` says (kl = 0 without ref_logp).  out4 = {surrogate + kl_weight * kl, surrogate, kl,
+ * share of the counted positions where the clipped branch is the smaller one}.  logp [n,l] is written.  grad (or NULL):
+ * grad_scale * d out4[0] / d logits in the same pass over the logits, laid out as above; with it stats [n,l,2] and weight
+ * [n,l] (d out4[0] / d logp) are written where they are not NULL, for spice_token_logprobs_grad. */
+int spice_policy_loss(const spice_logits *logits, const spice_labels *labels, const float *old_logp,
+                      const float *advantages, int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp,
+                      const spice_policy_params *params, float *out4, float *logp, float *stats, float *weight,
+                      int32_t class_last, void *grad, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------- *
+ * (10) The update end of a fine-tuning step over many tensors: global gradient
+ * norm, clipping, Adam.  Stands behind the optimiser step of the fine-tune loop
+ * (pruning/trainer.py:160-228, which steps without clipping).
+ *
+ * `grads`, `params`, ... are HOST arrays of `count` device pointers (aligned to
+ * their element), numel a host array of element counts; they are read before the
+ * call returns.  dtype 0 = fp32, 1 = fp16, 2 = bf16, one for all tensors of a call.
+ * record: 4 device floats, {norm, clip factor, and two of the Adam step's}.
+ * ------------------------------------------------------------------------- */
+#define SPICE_NORM_L2 0
+#define SPICE_NORM_INF 1
+
+/* Bytes of workspace of spice_grad_norm and of spice_adam_step with clipping; nothing in it has to be cleared. */
+size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t count);
+
+/* record[0] = norm over all tensors (squares summed in fp64, fixed order), record[1] = min(1, max_norm / (norm + 1e-6)).
+ * A NaN or infinite gradient makes the norm NaN or infinite and the factor NaN or 0. */
+int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
+                    float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
+
+/* out = record[1] * grads, rounded once to out_dtype (the gradients' own, or fp32).  out may be grads (then nothing is
+ * moved where the factor is 1); other overlaps are not allowed. */
+int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
+                    int32_t count, const float *record, void *stream);
+
+typedef struct spice_adam_params {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;      /* this step's number, from 1; ignored with a device step count */
+    float max_norm;    /* clip as the gradients are read; negative: no clipping */
+    int32_t decoupled; /* non-zero: p *= 1 - lr * weight_decay; else the decay joins the gradient */
+} spice_adam_params;
+
+/* One Adam step of every tensor in place: exp_avg and exp_avg_sq fp32, params and grads of `dtype` (16-bit params: the
+ * update is computed in fp32 and rounded once).  The clipped gradient is used, never written.  norm: a norm taken before
+ * (device float; over more tensors than these, say), or NULL to take these tensors' here.  step: a device step count that
+ * the call raises by one and uses (a captured launch counts on), or NULL for params->step. */
+int spice_adam_step(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
+                    const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_params *p, const float *norm,
+                    int64_t *step, float *record, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch  # noqa: F401  (must precede the CDLL below)
 
@@ -64,6 +64,30 @@ class GatherItem(Structure):
                 ("idx_in_off", c_int64), ("row0", c_int32), ("n_rows", c_int32),
                 ("dst_cols", c_int32), ("src_cols", c_int32), ("inner", c_int32),
                 ("lanes", c_int32), ("flags", c_int32), ("pad_", c_int32)]
+
+
+class Logits(Structure):
+    _fields_ = [("data", c_void_p), ("dtype", c_int32), ("pad_", c_int32), ("n", c_int64), ("l", c_int64), ("c", c_int64),
+                ("n_stride", c_int64), ("l_stride", c_int64), ("c_stride", c_int64)]
+
+
+class Labels(Structure):
+    _fields_ = [("data", c_void_p), ("n_stride", c_int64), ("l_stride", c_int64), ("ignore_index", c_int64)]
+
+
+class PreferenceParams(Structure):
+    _fields_ = [("temperature", c_float), ("beta", c_float), ("smoothing", c_float), ("loss_type", c_int32),
+                ("average", c_int32)]
+
+
+class PolicyParams(Structure):
+    _fields_ = [("temperature", c_float), ("clip_low", c_float), ("clip_high", c_float), ("kl_weight", c_float),
+                ("grad_scale", c_float), ("reduction", c_int32)]
+
+
+class AdamParams(Structure):
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+                ("step", c_int64), ("max_norm", c_float), ("decoupled", c_int32)]
 
 
 # name -> (restype, argtypes); every symbol include/spice_amd.h declares
@@ -138,6 +162,23 @@ SIGNATURES = {
                                           c_int32, c_int32, c_int32, c_float, c_float, c_void_p]),
     "spice_upsample_bilinear_into": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int32,
                                           c_int32, c_int32, c_int32, c_float, c_float, c_int64, c_int64, c_void_p]),
+    "spice_token_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "spice_token_logprobs": (c_int32, [POINTER(Logits), POINTER(Labels), c_float, c_void_p, c_void_p, c_void_p]),
+    "spice_token_logprobs_grad": (c_int32, [POINTER(Logits), POINTER(Labels), c_float, c_void_p, c_void_p, c_int64, c_int64,
+                                            c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
+    "spice_preference_loss": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, POINTER(PreferenceParams), c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "spice_policy_loss": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                    POINTER(PolicyParams), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
+                                    c_void_p, c_size_t, c_void_p]),
+    "spice_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int32]),
+    "spice_grad_norm": (c_int32, [POINTER(c_void_p), POINTER(c_int64), c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
+                                  c_size_t, c_void_p]),
+    "spice_grad_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_void_p,
+                                  c_void_p]),
+    "spice_adam_step": (c_int32, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64),
+                                  c_int32, c_int32, POINTER(AdamParams), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                  c_void_p]),
 }
 
 _lib = None

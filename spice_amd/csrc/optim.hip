@@ -1,0 +1,414 @@
+// The update end of a fine-tuning step over many tensors: global gradient norm, clipping, Adam.
+//
+//   norm = (sum over all tensors of g^2)^1/2 (or max |g|),   c = min(1, max_norm / (norm + 1e-6)),
+//   clip:  out = c g
+//   Adam:  g' = c g (+ decay p),  m += (1 - b1)(g' - m),  v += (1 - b2)(g'^2 - v),
+//          p -= lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)     (decoupled decay: p *= 1 - lr decay first)
+//
+// The tensors of a call travel as kernel arguments: pointers, sizes and the first work item of each, as many as fit into
+// 4 KB, so nothing is uploaded, nothing outlives the call and a captured launch holds all it needs.  A workgroup finds its
+// tensor by bisection of the first-item table.  Squares are summed in fp64: a gradient of 1e20 or 1e-30 neither overflows
+// nor vanishes, and the partial sums are folded in a fixed order by one workgroup, so the norm repeats bit for bit.
+#include "common.h"
+
+#include <math.h>
+
+namespace spice {
+namespace {
+
+constexpr int kOptThreads = 256;
+constexpr int kOptFold = 1024;
+constexpr int64_t kOptItemLeast = 8192;            // elements of a work item at least
+constexpr int64_t kOptItems = 8192;                // work items of a call, about, at most
+constexpr int64_t kOptEntryMost = (int64_t)1 << 30; // elements of one table entry: longer tensors take several
+
+// A call's work items: `each` elements of one tensor.  Up to N table entries a launch.
+template <int PTRS, int N>
+struct Table {
+    void *p[PTRS][N];
+    uint32_t numel[N];
+    uint32_t first[N];   // first work item of the entry, from the launch's first
+    int32_t count;
+    uint32_t each;
+};
+
+template <int PTRS>
+constexpr int table_entries() { return PTRS == 1 ? 240 : PTRS == 2 ? 160 : 96; }
+template <int PTRS>
+using TableOf = Table<PTRS, table_entries<PTRS>()>;
+static_assert(sizeof(TableOf<1>) <= 3900 && sizeof(TableOf<2>) <= 3900 && sizeof(TableOf<4>) <= 3900, "kernel arguments");
+
+template <typename TB>
+__device__ __forceinline__ int entry_of(const TB &t, uint32_t item) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.first[mid] <= item) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float opt_f32(float v) { return v; }
+__device__ __forceinline__ float opt_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float opt_f32(__bf16 v) { return (float)v; }
+
+__device__ __forceinline__ bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int K>
+struct __attribute__((aligned(sizeof(T) * K))) Vec { T v[K]; };
+
+// NaN-keeping maximum
+__device__ __forceinline__ double max_keep(double a, double b) { return (a > b || a != a) ? a : b; }
+
+template <bool INF>
+__device__ __forceinline__ double norm_join(double a, double b) { return INF ? max_keep(a, b) : a + b; }
+
+template <bool INF>
+__device__ __forceinline__ double norm_fold(double v, double *lds, int threads) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = norm_join<INF>(v, __shfl_xor(v, o, kWave));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = lds[0];
+    for (int w = 1; w < threads / kWave; ++w) v = norm_join<INF>(v, lds[w]);
+    return v;
+}
+
+template <typename T, bool INF>
+__device__ __forceinline__ double norm_take(double acc, T g) {
+    const double d = (double)opt_f32(g);
+    return INF ? max_keep(fabs(d), acc) : __builtin_fma(d, d, acc);
+}
+
+template <typename T, bool INF>
+__global__ __launch_bounds__(kOptThreads) void grad_norm_kernel(TableOf<1> t, double *part) {
+    __shared__ double lds[kOptThreads / kWave];
+    const int e = entry_of(t, blockIdx.x);
+    const uint32_t at = (blockIdx.x - t.first[e]) * t.each;
+    const T *g = (const T *)t.p[0][e] + at;
+    const uint32_t n = min(t.each, t.numel[e] - at);
+    double acc = 0.0;
+    uint32_t done = 0;
+    if (on16(g)) {
+        constexpr int K = 16 / sizeof(T);
+        const Vec<T, K> *gv = (const Vec<T, K> *)g;
+        const uint32_t nv = n / K;
+        for (uint32_t i = threadIdx.x; i < nv; i += kOptThreads) {
+            const Vec<T, K> x = gv[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) acc = norm_take<T, INF>(acc, x.v[k]);
+        }
+        done = nv * K;
+    }
+    for (uint32_t i = done + threadIdx.x; i < n; i += kOptThreads) acc = norm_take<T, INF>(acc, g[i]);
+    acc = norm_fold<INF>(acc, lds, kOptThreads);
+    if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// The call's record: {norm, clip factor, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)}.
+struct RecordArgs {
+    const double *part;
+    int64_t parts;
+    const float *norm_in;   // a norm taken before, or NULL
+    int inf, clip, adam;
+    double max_norm;
+    double lr, beta1, beta2;
+    int64_t host_step;
+    int64_t *step;          // device step count, raised here; NULL: host_step
+    float *record;
+};
+
+__global__ __launch_bounds__(kOptFold) void grad_record_kernel(RecordArgs a) {
+    __shared__ double lds[kOptFold / kWave];
+    double norm = 0.0;
+    if (a.norm_in) {
+        norm = (double)*a.norm_in;
+    } else if (a.inf) {
+        for (int64_t i = threadIdx.x; i < a.parts; i += kOptFold) norm = norm_join<true>(norm, a.part[i]);
+        norm = norm_fold<true>(norm, lds, kOptFold);
+    } else {
+        for (int64_t i = threadIdx.x; i < a.parts; i += kOptFold) norm += a.part[i];
+        norm = sqrt(norm_fold<false>(norm, lds, kOptFold));
+    }
+    if (threadIdx.x != 0) return;
+    double c = 1.0;
+    if (a.clip) {
+        c = a.max_norm / (norm + 1e-6);
+        if (c > 1.0) c = 1.0;
+    }
+    a.record[0] = (float)norm;
+    a.record[1] = (float)c;
+    if (a.adam) {
+        int64_t t = a.host_step;
+        if (a.step) {
+            t = *a.step + 1;
+            *a.step = t;
+        }
+        a.record[2] = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
+        a.record[3] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+    }
+}
+
+template <typename T, typename O>
+__global__ __launch_bounds__(kOptThreads) void grad_clip_kernel(TableOf<2> t, const float *record) {
+    const float c = record[1];
+    const int e = entry_of(t, blockIdx.x);
+    const uint32_t at = (blockIdx.x - t.first[e]) * t.each;
+    const T *g = (const T *)t.p[0][e] + at;
+    O *out = (O *)t.p[1][e] + at;
+    if (c == 1.f && (const void *)g == (const void *)out) return;
+    const uint32_t n = min(t.each, t.numel[e] - at);
+    uint32_t done = 0;
+    if (on16(g) && on16(out)) {
+        constexpr int K = 16 / (sizeof(T) < sizeof(O) ? sizeof(O) : sizeof(T));
+        const uint32_t nv = n / K;
+        for (uint32_t i = threadIdx.x; i < nv; i += kOptThreads) {
+            const Vec<T, K> x = ((const Vec<T, K> *)g)[i];
+            Vec<O, K> y;
+#pragma unroll
+            for (int k = 0; k < K; ++k) y.v[k] = (O)(opt_f32(x.v[k]) * c);
+            ((Vec<O, K> *)out)[i] = y;
+        }
+        done = nv * K;
+    }
+    for (uint32_t i = done + threadIdx.x; i < n; i += kOptThreads) out[i] = (O)(opt_f32(g[i]) * c);
+}
+
+struct AdamArgs {
+    float a1, a2, eps, decay, keep;   // a = 1 - beta, taken in fp64 (1 - 0.999f is 1e-5 of itself off); keep = 1 - lr * decay with decoupled decay, else 1; decay = 0 then
+};
+
+template <typename T>
+__device__ __forceinline__ void adam_take(T &p, T g, float &m, float &v, const AdamArgs &a, float c, float rate, float root) {
+    float w = opt_f32(p), d = opt_f32(g) * c;
+    w *= a.keep;
+    d = __builtin_fmaf(a.decay, w, d);
+    m = __builtin_fmaf(a.a1, d - m, m);
+    v = __builtin_fmaf(a.a2, d * d - v, v);
+    w -= rate * (m / __builtin_fmaf(sqrtf(v), root, a.eps));
+    p = (T)w;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kOptThreads) void adam_kernel(TableOf<4> t, AdamArgs a, const float *record) {
+    const float c = record[1], rate = record[2], root = record[3];
+    const int e = entry_of(t, blockIdx.x);
+    const uint32_t at = (blockIdx.x - t.first[e]) * t.each;
+    T *p = (T *)t.p[0][e] + at;
+    const T *g = (const T *)t.p[1][e] + at;
+    float *m = (float *)t.p[2][e] + at, *v = (float *)t.p[3][e] + at;
+    const uint32_t n = min(t.each, t.numel[e] - at);
+    uint32_t done = 0;
+    if (on16(p) && on16(g) && on16(m) && on16(v)) {
+        const uint32_t nv = n / 4;
+        for (uint32_t i = threadIdx.x; i < nv; i += kOptThreads) {
+            Vec<T, 4> pv = ((const Vec<T, 4> *)p)[i];
+            const Vec<T, 4> gv = ((const Vec<T, 4> *)g)[i];
+            Vec<float, 4> mv = ((const Vec<float, 4> *)m)[i], vv = ((const Vec<float, 4> *)v)[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) adam_take<T>(pv.v[k], gv.v[k], mv.v[k], vv.v[k], a, c, rate, root);
+            ((Vec<T, 4> *)p)[i] = pv;
+            ((Vec<float, 4> *)m)[i] = mv;
+            ((Vec<float, 4> *)v)[i] = vv;
+        }
+        done = nv * 4;
+    }
+    for (uint32_t i = done + threadIdx.x; i < n; i += kOptThreads) adam_take<T>(p[i], g[i], m[i], v[i], a, c, rate, root);
+}
+
+// Elements of a work item: few items for large calls (their partial sums are folded by one workgroup), short ones for
+// small calls (a workgroup's share of the chip).  A multiple of 1024 keeps every item's start on 16 bytes.
+uint32_t item_elements(const int64_t *numel, int32_t count) {
+    int64_t total = 0;
+    for (int32_t i = 0; i < count; ++i) total += numel[i];
+    const int64_t each = ceil_div(ceil_div(total, kOptItems), 1024) * 1024;
+    return (uint32_t)(each < kOptItemLeast ? kOptItemLeast : each > ((int64_t)1 << 28) ? ((int64_t)1 << 28) : each);
+}
+
+bool counts_ok(const int64_t *numel, int32_t count) {
+    if (count < 0 || (count && !numel)) return false;
+    int64_t total = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        if (numel[i] < 0 || numel[i] > ((int64_t)1 << 40)) return false;
+        total += numel[i];
+        if (total > ((int64_t)1 << 42)) return false;
+    }
+    return true;
+}
+
+int64_t item_count(const int64_t *numel, int32_t count, uint32_t each) {
+    int64_t items = 0;
+    const int64_t most = kOptEntryMost / each * each;
+    for (int32_t i = 0; i < count; ++i)
+        for (int64_t at = 0; at < numel[i]; at += most) items += ceil_div(numel[i] - at < most ? numel[i] - at : most, each);
+    return items;
+}
+
+// Calls launch(table, first item, items) for as many tables as the tensors need.  ptrs: PTRS host arrays of device
+// pointers; bytes: element size of each.
+template <int PTRS, typename F>
+int for_tables(void *const *const (&ptrs)[PTRS], const int64_t (&bytes)[PTRS], const int64_t *numel, int32_t count, uint32_t each, F launch) {
+    TableOf<PTRS> t;
+    t.count = 0;
+    t.each = each;
+    int64_t items = 0, before = 0;
+    const int64_t most = kOptEntryMost / each * each;
+    for (int32_t i = 0; i < count; ++i) {
+        for (int64_t at = 0; at < numel[i]; at += most) {
+            const int64_t n = numel[i] - at < most ? numel[i] - at : most;
+            for (int k = 0; k < PTRS; ++k) t.p[k][t.count] = (char *)ptrs[k][i] + at * bytes[k];
+            t.numel[t.count] = (uint32_t)n;
+            t.first[t.count] = (uint32_t)items;
+            items += ceil_div(n, each);
+            if (++t.count == table_entries<PTRS>()) {
+                const int rc = launch(t, before, items);
+                if (rc) return rc;
+                before += items;
+                items = 0;
+                t.count = 0;
+            }
+        }
+    }
+    return t.count ? launch(t, before, items) : SPICE_OK;
+}
+
+bool pointers_ok(void *const *p, const int64_t *numel, int32_t count, int64_t bytes) {
+    if (count && !p) return false;
+    for (int32_t i = 0; i < count; ++i)
+        if (numel[i] && (!p[i] || (reinterpret_cast<uintptr_t>(p[i]) & (uintptr_t)(bytes - 1)))) return false;
+    return true;
+}
+
+int64_t type_bytes(int32_t dtype) { return dtype == 0 ? 4 : 2; }
+
+template <typename T>
+int launch_norm(void *const *grads, const int64_t *numel, int32_t count, int64_t bytes, int inf, double *part, hipStream_t s) {
+    void *const *const p[1] = {grads};
+    const int64_t b[1] = {bytes};
+    return for_tables<1>(p, b, numel, count, item_elements(numel, count), [&](const TableOf<1> &t, int64_t before, int64_t items) {
+        if (inf)
+            grad_norm_kernel<T, true><<<(unsigned)items, kOptThreads, 0, s>>>(t, part + before);
+        else
+            grad_norm_kernel<T, false><<<(unsigned)items, kOptThreads, 0, s>>>(t, part + before);
+        SPICE_LAUNCH_CHECK();
+        return (int)SPICE_OK;
+    });
+}
+
+template <typename T, typename O>
+int launch_clip(void *const *grads, void *const *out, const int64_t *numel, int32_t count, const float *record, hipStream_t s) {
+    void *const *const p[2] = {grads, out};
+    const int64_t b[2] = {(int64_t)sizeof(T), (int64_t)sizeof(O)};
+    return for_tables<2>(p, b, numel, count, item_elements(numel, count), [&](const TableOf<2> &t, int64_t, int64_t items) {
+        grad_clip_kernel<T, O><<<(unsigned)items, kOptThreads, 0, s>>>(t, record);
+        SPICE_LAUNCH_CHECK();
+        return (int)SPICE_OK;
+    });
+}
+
+template <typename T>
+int launch_adam(void *const *params, void *const *grads, void *const *m, void *const *v, const int64_t *numel, int32_t count,
+                const AdamArgs &a, const float *record, hipStream_t s) {
+    void *const *const p[4] = {params, grads, m, v};
+    const int64_t b[4] = {(int64_t)sizeof(T), (int64_t)sizeof(T), 4, 4};
+    return for_tables<4>(p, b, numel, count, item_elements(numel, count), [&](const TableOf<4> &t, int64_t, int64_t items) {
+        adam_kernel<T><<<(unsigned)items, kOptThreads, 0, s>>>(t, a, record);
+        SPICE_LAUNCH_CHECK();
+        return (int)SPICE_OK;
+    });
+}
+
+}  // namespace
+}  // namespace spice
+
+using namespace spice;
+
+extern "C" size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t count) {
+    if (!counts_ok(numel, count)) return 0;
+    return (size_t)(item_count(numel, count, item_elements(numel, count)) * (int64_t)sizeof(double) + 64);
+}
+
+extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
+                               float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream) {
+    if (dtype < 0 || dtype > 2 || !counts_ok(numel, count) || !pointers_ok(grads, numel, count, type_bytes(dtype)) || !record ||
+        !workspace || !aligned8(workspace) || norm_type < 0 || norm_type > 1 || !(max_norm >= 0.f))
+        return SPICE_ERR_ARG;
+    if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    double *part = (double *)workspace;
+    int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, norm_type, part, s)
+             : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, norm_type, part, s)
+                          : launch_norm<__bf16>(grads, numel, count, 2, norm_type, part, s);
+    if (rc) return rc;
+    RecordArgs a = {};
+    a.part = part;
+    a.parts = item_count(numel, count, item_elements(numel, count));
+    a.inf = norm_type == SPICE_NORM_INF;
+    a.clip = 1;
+    a.max_norm = (double)max_norm;
+    a.record = record;
+    grad_record_kernel<<<1, kOptFold, 0, s>>>(a);
+    SPICE_LAUNCH_CHECK();
+    return SPICE_OK;
+}
+
+extern "C" int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
+                               int32_t count, const float *record, void *stream) {
+    if (dtype < 0 || dtype > 2 || !(out_dtype == dtype || out_dtype == 0) || !counts_ok(numel, count) ||
+        !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(out, numel, count, type_bytes(out_dtype)) || !record)
+        return SPICE_ERR_ARG;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == 0) return launch_clip<float, float>(grads, out, numel, count, record, s);
+    if (dtype == 1)
+        return out_dtype == 0 ? launch_clip<_Float16, float>(grads, out, numel, count, record, s)
+                              : launch_clip<_Float16, _Float16>(grads, out, numel, count, record, s);
+    return out_dtype == 0 ? launch_clip<__bf16, float>(grads, out, numel, count, record, s)
+                          : launch_clip<__bf16, __bf16>(grads, out, numel, count, record, s);
+}
+
+extern "C" int spice_adam_step(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
+                               const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_params *p,
+                               const float *norm, int64_t *step, float *record, void *workspace, size_t workspace_bytes,
+                               void *stream) {
+    if (dtype < 0 || dtype > 2 || !p || !counts_ok(numel, count) || !pointers_ok(params, numel, count, type_bytes(dtype)) ||
+        !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(exp_avg, numel, count, 4) ||
+        !pointers_ok(exp_avg_sq, numel, count, 4) || !record || !(p->lr >= 0.0 && p->lr <= 1e30) ||
+        !(p->beta1 >= 0.0 && p->beta1 < 1.0) || !(p->beta2 >= 0.0 && p->beta2 < 1.0) || !(p->eps >= 0.0) ||
+        !(p->weight_decay >= 0.0) || (!step && p->step < 1) || p->max_norm != p->max_norm)
+        return SPICE_ERR_ARG;
+    const bool clip = p->max_norm >= 0.f, take = clip && !norm;
+    if (take && (!workspace || !aligned8(workspace))) return SPICE_ERR_ARG;
+    if (take && workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    RecordArgs r = {};
+    int rc = SPICE_OK;
+    if (take) {
+        r.part = (const double *)workspace;
+        r.parts = item_count(numel, count, item_elements(numel, count));
+        rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, 0, (double *)workspace, s)
+             : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, 0, (double *)workspace, s)
+                          : launch_norm<__bf16>(grads, numel, count, 2, 0, (double *)workspace, s);
+        if (rc) return rc;
+    }
+    r.norm_in = clip ? norm : nullptr;
+    r.clip = clip;
+    r.adam = 1;
+    r.max_norm = (double)p->max_norm;
+    r.lr = p->lr;
+    r.beta1 = p->beta1;
+    r.beta2 = p->beta2;
+    r.host_step = p->step;
+    r.step = step;
+    r.record = record;
+    grad_record_kernel<<<1, kOptFold, 0, s>>>(r);
+    SPICE_LAUNCH_CHECK();
+    AdamArgs a;
+    a.a1 = (float)(1.0 - p->beta1);
+    a.a2 = (float)(1.0 - p->beta2);
+    a.eps = (float)p->eps;
+    a.decay = p->decoupled ? 0.f : (float)p->weight_decay;
+    a.keep = p->decoupled ? (float)(1.0 - p->lr * p->weight_decay) : 1.f;
+    return dtype == 0   ? launch_adam<float>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
+           : dtype == 1 ? launch_adam<_Float16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
+                        : launch_adam<__bf16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s);
+}

@@ -22,9 +22,11 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <iterator>
 #include <mutex>
 #include <limits>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/spice_amd.h"
@@ -876,6 +878,361 @@ Tensor conv3x3_bn_act(const Tensor &x, const Tensor &weight9, const Tensor &mean
     return out;
 }
 
+// ---- (9) losses over label log-probabilities --------------------------------------------------
+
+// The consecutive dimensions [from, to) of t as one axis of `size` elements, `stride` apart; false when they are not one.
+bool one_axis(const Tensor &t, int64_t from, int64_t to, int64_t &size, int64_t &stride) {
+    size = 1;
+    stride = 1;
+    bool any = false;
+    for (int64_t d = to - 1; d >= from; --d) {
+        if (t.size(d) == 1) continue;
+        if (any && t.stride(d) != stride * size) return false;
+        if (!any) stride = t.stride(d);
+        any = true;
+        size *= t.size(d);
+    }
+    return true;
+}
+
+struct TokenView {
+    spice_logits x;
+    spice_labels y;
+    bool last;      // the class axis is the last one
+};
+
+TokenView token_view(const Tensor &logits, const Tensor &labels, int64_t class_dim, double temperature, int64_t ignore_index,
+                     const char *what) {
+    TORCH_CHECK_VALUE(temperature > 0.0 && temperature <= 1e30 && temperature >= 1e-30, what,
+                      ": temperature must be positive, got ", temperature);
+    TokenView v;
+    v.x.dtype = logits_code(logits, "logits");
+    v.x.pad_ = 0;
+    TORCH_CHECK(logits.is_cuda(), "logits is on ", logits.device(),
+                "; the MI355X path has no CPU implementation (move the tensor to a HIP device)");
+    TORCH_CHECK_TYPE(labels.scalar_type() == at::kLong, "labels must be ", at::kLong, ", got ", labels.scalar_type());
+    check_same_device(logits, labels, "labels");
+    const int64_t d = logits.dim();
+    TORCH_CHECK_VALUE(d >= 2, what, ": logits must have a sequence axis and a class axis, got ", logits.sizes());
+    if (class_dim < 0) class_dim += d;
+    TORCH_CHECK_VALUE(class_dim == 1 || class_dim == d - 1, what, ": class_dim must be 1 or the last axis");
+    v.last = class_dim == d - 1;
+    v.x.c = logits.size(class_dim);
+    TORCH_CHECK_VALUE(v.x.c >= 1, what, ": no classes");
+    TORCH_CHECK_VALUE(ignore_index < 0 || ignore_index >= v.x.c, what, ": ignore_index ", ignore_index, " is one of the ", v.x.c,
+                      " classes");
+    bool same = labels.dim() == d - 1 && labels.size(0) == logits.size(0);
+    for (int64_t k = 1; same && k < d - 1; ++k) same = labels.size(k) == logits.size(v.last ? k : k + 1);
+    TORCH_CHECK_VALUE(same, what, ": labels must have the logits' shape without the class axis, got ", labels.sizes(), " for ",
+                      logits.sizes());
+    v.x.n = logits.size(0);
+    v.x.n_stride = logits.stride(0);
+    v.x.c_stride = logits.stride(class_dim);
+    int64_t ll = 0;
+    TORCH_CHECK_VALUE(one_axis(logits, v.last ? 1 : 2, v.last ? d - 1 : d, v.x.l, v.x.l_stride) &&
+                          one_axis(labels, 1, d - 1, ll, v.y.l_stride),
+                      what, ": the positions of logits and labels must lie at one stride (make the tensor contiguous)");
+    v.x.data = logits.data_ptr();
+    v.y.data = labels.data_ptr<int64_t>();
+    v.y.n_stride = labels.stride(0);
+    v.y.ignore_index = ignore_index;
+    return v;
+}
+
+void check_positions(const Tensor &t, const char *name, const Tensor &labels) {
+    check_dev(t, name, at::kFloat);
+    check_same_device(labels, t, name);
+    TORCH_CHECK_VALUE(t.sizes() == labels.sizes(), name, " must have the labels' shape ", labels.sizes(), ", got ", t.sizes());
+}
+
+Tensor stats_for(const Tensor &labels, const at::TensorOptions &f32) {
+    std::vector<int64_t> shape = labels.sizes().vec();
+    shape.push_back(2);
+    return at::empty(shape, f32);
+}
+
+Tensor loss_workspace(const TokenView &v, const at::TensorOptions &f32) {
+    return at::empty({(int64_t)spice_token_loss_workspace_bytes(v.x.n, v.x.l)}, f32.dtype(at::kByte));
+}
+
+const float *one_float(const c10::optional<Tensor> &t, const char *name, const Tensor &like) {
+    if (!t.has_value()) return nullptr;
+    check_dev(*t, name, at::kFloat);
+    check_same_device(like, *t, name);
+    TORCH_CHECK_VALUE(t->numel() == 1, name, " must hold one value");
+    return t->data_ptr<float>();
+}
+
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &labels, int64_t class_dim, double temperature,
+                                          int64_t ignore_index) {
+    const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "token_logprobs");
+    c10::DeviceGuard guard(logits.device());
+    const auto f32 = logits.options().dtype(at::kFloat);
+    Tensor logp = at::empty(labels.sizes(), f32), stats = stats_for(labels, f32);
+    check_rc(spice_token_logprobs(&v.x, &v.y, (float)temperature, logp.data_ptr<float>(), stats.data_ptr<float>(),
+                                  current_stream(logits)),
+             "spice_token_logprobs");
+    return std::make_tuple(logp, stats);
+}
+
+Tensor token_logprobs_grad(const Tensor &logits, const Tensor &labels, const Tensor &stats, const Tensor &weight,
+                           int64_t class_dim, double temperature, int64_t ignore_index, double scale,
+                           const c10::optional<Tensor> &device_scale, c10::optional<Tensor> out) {
+    const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "token_logprobs_grad");
+    check_dev(stats, "stats", at::kFloat);
+    check_same_device(logits, stats, "stats");
+    check_dev(weight, "weight", at::kFloat);
+    check_same_device(logits, weight, "weight");
+    TORCH_CHECK_VALUE(stats.numel() == 2 * labels.numel(), "stats must be the second output of token_logprobs for these labels");
+    const bool per_sequence = weight.dim() == 1 && weight.size(0) == v.x.n;
+    TORCH_CHECK_VALUE(per_sequence || weight.sizes() == labels.sizes(), "weight must have the labels' shape ", labels.sizes(),
+                      " or one value a sequence, got ", weight.sizes());
+    c10::DeviceGuard guard(logits.device());
+    if (out.has_value()) {
+        check_dev(*out, "out", logits.scalar_type());
+        check_same_device(logits, *out, "out");
+        TORCH_CHECK_VALUE(out->sizes() == logits.sizes(), "out must have the logits' shape");
+        TORCH_CHECK_VALUE(device_scale.has_value(), "out holds the gradient for a device_scale of 1: give the device_scale");
+    }
+    Tensor grad = out.has_value() ? *out : at::empty(logits.sizes(), logits.options());
+    check_rc(spice_token_logprobs_grad(&v.x, &v.y, (float)temperature, stats.data_ptr<float>(), weight.data_ptr<float>(),
+                                       per_sequence ? 1 : v.x.l, per_sequence ? 0 : 1, (float)scale,
+                                       one_float(device_scale, "device_scale", logits), out.has_value() ? 1 : 0,
+                                       v.last ? 1 : 0, grad.data_ptr(), current_stream(logits)),
+             "spice_token_logprobs_grad");
+    return grad;
+}
+
+// (total [], rewards [N], weight [N], stats): the gradient is token_logprobs_grad on the last two.
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor &logits, const Tensor &labels, const Tensor &ref_logprobs,
+                                                           int64_t class_dim, double temperature, int64_t ignore_index,
+                                                           double beta, double smoothing, int64_t loss_type, bool average) {
+    const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "preference_loss");
+    check_positions(ref_logprobs, "ref_logprobs", labels);
+    TORCH_CHECK_VALUE(v.x.n >= 2 && v.x.n % 2 == 0, "preference_loss: the first axis must hold the preferred half and the other "
+                                                     "half, got ", v.x.n, " sequences");
+    TORCH_CHECK_VALUE(beta > 0.0 && beta <= 1e30, "preference_loss: beta must be positive, got ", beta);
+    TORCH_CHECK_VALUE(smoothing >= 0.0 && smoothing < 0.5, "preference_loss: label_smoothing must lie in [0, 0.5), got ", smoothing);
+    TORCH_CHECK_VALUE(loss_type != SPICE_PREFERENCE_IPO || smoothing == 0.0, "preference_loss: ipo takes no label_smoothing");
+    c10::DeviceGuard guard(logits.device());
+    const auto f32 = logits.options().dtype(at::kFloat);
+    Tensor total = at::empty({}, f32), rewards = at::empty({v.x.n}, f32), weight = at::empty({v.x.n}, f32);
+    Tensor logp = at::empty(labels.sizes(), f32), stats = stats_for(labels, f32), ws = loss_workspace(v, f32);
+    spice_preference_params p;
+    p.temperature = (float)temperature;
+    p.beta = (float)beta;
+    p.smoothing = (float)smoothing;
+    p.loss_type = (int32_t)loss_type;
+    p.average = average ? 1 : 0;
+    check_rc(spice_preference_loss(&v.x, &v.y, ref_logprobs.data_ptr<float>(), &p, total.data_ptr<float>(),
+                                   rewards.data_ptr<float>(), weight.data_ptr<float>(), logp.data_ptr<float>(),
+                                   stats.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(logits)),
+             "spice_preference_loss");
+    return std::make_tuple(total, rewards, weight, stats);
+}
+
+// (out4, logp, grad, stats, weight): the last three without elements where they are not wanted
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor &logits, const Tensor &labels, const Tensor &old_logprobs,
+                                               const Tensor &advantages, const c10::optional<Tensor> &ref_logprobs,
+                                               int64_t class_dim, double temperature, int64_t ignore_index, double clip_low,
+                                               double clip_high, double kl_weight, int64_t reduction, bool want_grad,
+                                               double grad_scale, bool want_weight) {
+    const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "policy_loss");
+    check_positions(old_logprobs, "old_logprobs", labels);
+    check_dev(advantages, "advantages", at::kFloat);
+    check_same_device(logits, advantages, "advantages");
+    const bool per_sequence = advantages.dim() == 1 && advantages.size(0) == v.x.n;
+    TORCH_CHECK_VALUE(per_sequence || advantages.sizes() == labels.sizes(), "advantages must have the labels' shape ",
+                      labels.sizes(), " or one value a sequence, got ", advantages.sizes());
+    if (ref_logprobs.has_value()) check_positions(*ref_logprobs, "ref_logprobs", labels);
+    TORCH_CHECK_VALUE(clip_low >= 0.0 && clip_low <= 1.0 && clip_high >= 0.0 && kl_weight >= 0.0,
+                      "policy_loss: clip_low must lie in [0, 1], clip_high and kl_weight must not be negative");
+    TORCH_CHECK_VALUE(kl_weight == 0.0 || ref_logprobs.has_value(), "policy_loss: a KL weight needs ref_logprobs");
+    c10::DeviceGuard guard(logits.device());
+    const auto f32 = logits.options().dtype(at::kFloat);
+    Tensor out4 = at::empty({4}, f32), logp = at::empty(labels.sizes(), f32), ws = loss_workspace(v, f32);
+    Tensor none = at::empty({0}, f32), grad = want_grad ? at::empty(logits.sizes(), logits.options()) : none;
+    want_weight = want_weight && want_grad;
+    Tensor stats = want_weight ? stats_for(labels, f32) : none, weight = want_weight ? at::empty(labels.sizes(), f32) : none;
+    spice_policy_params p;
+    p.temperature = (float)temperature;
+    p.clip_low = (float)clip_low;
+    p.clip_high = (float)clip_high;
+    p.kl_weight = (float)kl_weight;
+    p.grad_scale = (float)grad_scale;
+    p.reduction = (int32_t)reduction;
+    check_rc(spice_policy_loss(&v.x, &v.y, old_logprobs.data_ptr<float>(), advantages.data_ptr<float>(),
+                               per_sequence ? 1 : v.x.l, per_sequence ? 0 : 1,
+                               ref_logprobs.has_value() ? ref_logprobs->data_ptr<float>() : nullptr, &p, out4.data_ptr<float>(),
+                               logp.data_ptr<float>(), want_weight ? stats.data_ptr<float>() : nullptr,
+                               want_weight ? weight.data_ptr<float>() : nullptr, v.last ? 1 : 0,
+                               want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), current_stream(logits)),
+             "spice_policy_loss");
+    return std::make_tuple(out4, logp, grad, stats, weight);
+}
+
+// ---- (10) gradient norm, clipping, Adam ---------------------------------------------------------
+
+struct TensorTable {
+    std::vector<void *> p;
+    int32_t code;
+};
+
+// Device pointers of tensors that are walked in memory order: any strides without gaps.
+TensorTable table_of(const std::vector<Tensor> &ts, const char *name, const Tensor &like, at::ScalarType type) {
+    TensorTable t;
+    t.code = type == at::kFloat ? 0 : type == at::kHalf ? 1 : 2;
+    t.p.reserve(ts.size());
+    for (const Tensor &x : ts) {
+        TORCH_CHECK(x.is_cuda(), name, " is on ", x.device(),
+                    "; the MI355X path has no CPU implementation (move the tensor to a HIP device)");
+        TORCH_CHECK_TYPE(x.scalar_type() == type, name, " must be ", type, ", got ", x.scalar_type());
+        check_same_device(like, x, name);
+        TORCH_CHECK_VALUE(x.is_non_overlapping_and_dense(), name, " must be dense (contiguous in some order of its axes)");
+        t.p.push_back(x.data_ptr());
+    }
+    return t;
+}
+
+at::ScalarType float_type(const Tensor &t, const char *name) {
+    logits_code(t, name);
+    return t.scalar_type();
+}
+
+// Tensor for tensor the same shape and the same order in memory.
+void check_alike(const std::vector<Tensor> &a, const std::vector<Tensor> &b, const char *name) {
+    TORCH_CHECK_VALUE(a.size() == b.size(), name, ": ", b.size(), " tensors, expected ", a.size());
+    for (size_t i = 0; i < a.size(); ++i)
+        TORCH_CHECK_VALUE(a[i].sizes() == b[i].sizes() && (a[i].strides() == b[i].strides() || a[i].numel() <= 1), name, "[", i,
+                          "] must have the shape and strides of its counterpart");
+}
+
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
+
+void add_range(const Tensor &t, Ranges &ranges) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel()) ranges.emplace_back(p, p + (uintptr_t)t.numel() * t.element_size());
+}
+
+// Tensors that a launch writes may not share memory with each other nor with what it reads: every workgroup writes its
+// own part, in no order.  `writes` is sorted here.
+void check_apart(Ranges &writes, const Ranges &reads, const char *what) {
+    std::sort(writes.begin(), writes.end());
+    for (size_t i = 1; i < writes.size(); ++i)
+        TORCH_CHECK_VALUE(writes[i].first >= writes[i - 1].second, what, ": two of the written tensors share memory");
+    for (const auto &r : reads) {
+        auto w = std::lower_bound(writes.begin(), writes.end(), std::make_pair(r.second, (uintptr_t)0));   // the first behind r
+        TORCH_CHECK_VALUE(w == writes.begin() || std::prev(w)->second <= r.first, what,
+                          ": a written tensor and one that is read share memory");
+    }
+}
+
+std::vector<int64_t> counts_of(const std::vector<Tensor> &ts) {
+    std::vector<int64_t> n;
+    n.reserve(ts.size());
+    for (const Tensor &t : ts) n.push_back(t.numel());
+    return n;
+}
+
+// Written behind autograd's back: the tensors' versions say so.
+void written(const std::vector<Tensor> &ts) {
+    for (const Tensor &t : ts)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor norm_workspace(const std::vector<int64_t> &n, const Tensor &like) {
+    return at::empty({(int64_t)spice_grad_norm_workspace_bytes(n.data(), (int32_t)n.size())}, like.options().dtype(at::kByte));
+}
+
+Tensor grad_norm(std::vector<Tensor> grads, double max_norm, bool inf) {
+    TORCH_CHECK_VALUE(!grads.empty(), "grad_norm: no tensors");
+    const at::ScalarType type = float_type(grads[0], "grads");
+    TensorTable g = table_of(grads, "grads", grads[0], type);
+    TORCH_CHECK_VALUE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
+    const std::vector<int64_t> n = counts_of(grads);
+    c10::DeviceGuard guard(grads[0].device());
+    Tensor record = at::empty({4}, grads[0].options().dtype(at::kFloat)), ws = norm_workspace(n, grads[0]);
+    check_rc(spice_grad_norm(g.p.data(), n.data(), (int32_t)n.size(), g.code, inf ? SPICE_NORM_INF : SPICE_NORM_L2,
+                             (float)max_norm, record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(),
+                             current_stream(grads[0])),
+             "spice_grad_norm");
+    return record;
+}
+
+void grad_clip(std::vector<Tensor> grads, std::vector<Tensor> out, const Tensor &record) {
+    TORCH_CHECK_VALUE(!grads.empty(), "grad_clip: no tensors");
+    TORCH_CHECK_VALUE(out.size() == grads.size(), "out: ", out.size(), " tensors, expected ", grads.size());
+    const at::ScalarType type = float_type(grads[0], "grads"), out_type = float_type(out[0], "out");
+    TORCH_CHECK_TYPE(out_type == type || out_type == at::kFloat, "out must be of the gradients' type or fp32, got ", out_type);
+    TensorTable g = table_of(grads, "grads", grads[0], type), o = table_of(out, "out", grads[0], out_type);
+    check_alike(grads, out, "out");
+    check_dev(record, "record", at::kFloat);
+    check_same_device(grads[0], record, "record");
+    TORCH_CHECK_VALUE(record.numel() == 4, "record must be grad_norm's");
+    Ranges writes, reads;
+    for (size_t i = 0; i < grads.size(); ++i) {   // a gradient may be its own output and nothing else's
+        add_range(out[i], writes);
+        if (grads[i].data_ptr() != out[i].data_ptr() || type != out_type) add_range(grads[i], reads);
+    }
+    check_apart(writes, reads, "grad_clip");
+    const std::vector<int64_t> n = counts_of(grads);
+    c10::DeviceGuard guard(grads[0].device());
+    check_rc(spice_grad_clip(g.p.data(), g.code, o.p.data(), o.code, n.data(), (int32_t)n.size(), record.data_ptr<float>(),
+                             current_stream(grads[0])),
+             "spice_grad_clip");
+    written(out);
+}
+
+Tensor adam_step(std::vector<Tensor> params, std::vector<Tensor> grads, std::vector<Tensor> exp_avg, std::vector<Tensor> exp_avg_sq,
+                 c10::optional<Tensor> step, int64_t host_step, double lr, double beta1, double beta2, double eps,
+                 double weight_decay, bool decoupled, double max_norm, const c10::optional<Tensor> &norm) {
+    TORCH_CHECK_VALUE(!params.empty(), "adam_step: no tensors");
+    const at::ScalarType type = float_type(params[0], "params");
+    const Tensor &like = params[0];
+    TensorTable p = table_of(params, "params", like, type), g = table_of(grads, "grads", like, type),
+                m = table_of(exp_avg, "exp_avg", like, at::kFloat), v = table_of(exp_avg_sq, "exp_avg_sq", like, at::kFloat);
+    check_alike(params, grads, "grads");
+    check_alike(params, exp_avg, "exp_avg");
+    check_alike(params, exp_avg_sq, "exp_avg_sq");
+    Ranges writes, reads;
+    for (size_t i = 0; i < params.size(); ++i) {
+        for (const Tensor *t : {&params[i], &exp_avg[i], &exp_avg_sq[i]}) add_range(*t, writes);
+        add_range(grads[i], reads);
+    }
+    check_apart(writes, reads, "adam_step");
+    int64_t *device_step = nullptr;
+    if (step.has_value()) {
+        check_dev(*step, "step", at::kLong);
+        check_same_device(like, *step, "step");
+        TORCH_CHECK_VALUE(step->numel() == 1, "step must hold one count");
+        device_step = step->data_ptr<int64_t>();
+    }
+    const std::vector<int64_t> n = counts_of(params);
+    TORCH_CHECK_VALUE(lr >= 0.0 && beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 &&
+                          weight_decay >= 0.0 && (step.has_value() || host_step >= 1),
+                      "adam_step: lr, eps and weight_decay must not be negative, the betas lie in [0, 1), steps count from 1");
+    c10::DeviceGuard guard(like.device());
+    Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws = norm_workspace(n, like);
+    spice_adam_params a;
+    a.lr = lr;
+    a.beta1 = beta1;
+    a.beta2 = beta2;
+    a.eps = eps;
+    a.weight_decay = weight_decay;
+    a.step = host_step;
+    a.max_norm = (float)max_norm;
+    a.decoupled = decoupled ? 1 : 0;
+    check_rc(spice_adam_step(p.p.data(), g.p.data(), m.p.data(), v.p.data(), n.data(), (int32_t)n.size(), p.code, &a,
+                             one_float(norm, "norm", like), device_step, record.data_ptr<float>(), ws.data_ptr(),
+                             (size_t)ws.numel(), current_stream(like)),
+             "spice_adam_step");
+    written(params);
+    written(exp_avg);
+    written(exp_avg_sq);
+    if (step.has_value()) written({*step});
+    return record;
+}
+
 int64_t abi_version() { return spice_abi_version(); }
 
 }  // namespace
@@ -928,4 +1285,18 @@ TORCH_LIBRARY(spice, m) {
           "Tensor? residual, Tensor? r_mean, Tensor? r_var, Tensor? r_weight, Tensor? r_bias, float r_eps, bool relu, "
           "int route, Tensor(a!)? out, Tensor? p_mean, Tensor? p_var, Tensor? p_weight, Tensor? p_bias, float p_eps, "
           "bool p_relu, int act=0) -> Tensor(a!)", &conv1x1_bn_act);
+    m.def("token_logprobs(Tensor logits, Tensor labels, int class_dim, float temperature, int ignore_index) -> (Tensor, Tensor)",
+          &token_logprobs);
+    m.def("token_logprobs_grad(Tensor logits, Tensor labels, Tensor stats, Tensor weight, int class_dim, float temperature, "
+          "int ignore_index, float scale, Tensor? device_scale, Tensor(a!)? out) -> Tensor(a!)", &token_logprobs_grad);
+    m.def("preference_loss(Tensor logits, Tensor labels, Tensor ref_logprobs, int class_dim, float temperature, int ignore_index, "
+          "float beta, float smoothing, int loss_type, bool average) -> (Tensor, Tensor, Tensor, Tensor)", &preference_loss);
+    m.def("policy_loss(Tensor logits, Tensor labels, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, int class_dim, "
+          "float temperature, int ignore_index, float clip_low, float clip_high, float kl_weight, int reduction, bool want_grad, "
+          "float grad_scale, bool want_weight) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", &policy_loss);
+    m.def("grad_norm(Tensor[] grads, float max_norm, bool inf) -> Tensor", &grad_norm);
+    m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, Tensor record) -> ()", &grad_clip);
+    m.def("adam_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)? step, "
+          "int host_step, float lr, float beta1, float beta2, float eps, float weight_decay, bool decoupled, float max_norm, "
+          "Tensor? norm) -> Tensor", &adam_step);
 }

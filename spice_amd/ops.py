@@ -875,3 +875,128 @@ def conv3x3_bn_act(x: torch.Tensor, weight9: torch.Tensor, bn: "torch.nn.BatchNo
     if _conv_probe is not None:
         return _probed("matrix_core_3x3", _conv3x3_fn, args, x, weight9.shape[0], weight9.shape[1])
     return _conv3x3_fn(*args)
+
+
+# --------------------------------------------------------------------------------------
+# losses over label log-probabilities
+
+_PREFERENCE_TYPES = {"sigmoid": 0, "ipo": 1}
+_POLICY_REDUCTIONS = {"token": 0, "sequence": 1}
+
+
+def _choice(table: Dict[str, int], value: str, what: str) -> int:
+    try:
+        return table[value]
+    except KeyError:
+        raise ValueError(f"{what} must be one of {sorted(table)}, got {value!r}") from None
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, class_dim: int = 1, temperature: float = 1.0,
+                   ignore_index: int = 255) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(log softmax(logits / temperature) at the labels, statistics): fp32, the first of the labels' shape, 0 where the
+    label is ignore_index; the second for token_logprobs_grad.
+
+    logits fp32 / fp16 / bf16: the class axis is axis 1 ([N,C,H,W], [N,C,L]) or, with class_dim=-1, the last one
+    ([N,L,V]); views are taken as they are as long as the positions of a sequence lie at one stride (a next-token shift,
+    a vocabulary padded in memory).  labels int64.  A label that is neither ignore_index nor a class gives NaN (loud,
+    without a host synchronisation); ignore_index must not be a class (255 is one of a large vocabulary: pass -100).
+    Not differentiable by itself: pruning.losses.token_logprobs is."""
+    return spice_ops().token_logprobs(logits, labels, class_dim, temperature, ignore_index)
+
+
+def token_logprobs_grad(logits: torch.Tensor, labels: torch.Tensor, stats: torch.Tensor, weight: torch.Tensor, *,
+                        class_dim: int = 1, temperature: float = 1.0, ignore_index: int = 255, scale: float = 1.0,
+                        device_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """scale * d(sum(weight * logp)) / d(logits) in the logits' type (rounded once), dense; `weight` fp32 of the labels'
+    shape, or one value a sequence ([N]).  `device_scale`: one more factor, in device memory.  `out`: a contiguous tensor
+    that holds the gradient for a device_scale of 1 already; it is written anew where that factor is another one, and
+    left as it is, without being read, where it is 1."""
+    return spice_ops().token_logprobs_grad(logits, labels, stats, weight, class_dim, temperature, ignore_index, scale,
+                                           device_scale, out)
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor, *, beta: float = 0.1,
+                    label_smoothing: float = 0.0, loss_type: str = "sigmoid", average: bool = False, class_dim: int = 1,
+                    temperature: float = 1.0, ignore_index: int = 255, want_grad: bool = False, grad_scale: float = 1.0
+                    ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(total, rewards [N], grad or None).  The first N/2 sequences (label maps, answers) are preferred to the other half,
+    pair by pair.  R_n = sum over the counted positions of logp - ref_logprobs (their mean with `average`),
+    h = R_better - R_worse: total = mean of -log sigmoid(beta h) (label_smoothing e: (1-e) of it and e of the swapped
+    pair's), or of (h - 1/(2 beta))^2 with loss_type="ipo"; rewards = beta R.  ref_logprobs: the frozen reference's
+    token_logprobs for the same labels.  grad = grad_scale * d total / d logits.  logits and labels as token_logprobs."""
+    f = spice_ops()
+    total, rewards, weight, stats = f.preference_loss(logits, labels, ref_logprobs, class_dim, temperature, ignore_index, beta,
+                                                      label_smoothing, _choice(_PREFERENCE_TYPES, loss_type, "loss_type"), average)
+    if not want_grad:
+        return total, rewards, None
+    return total, rewards, f.token_logprobs_grad(logits, labels, stats, weight, class_dim, temperature, ignore_index,
+                                                 grad_scale, None, None)
+
+
+def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
+                ref_logprobs: Optional[torch.Tensor] = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_weight: float = 0.0, reduction: str = "token", class_dim: int = 1, temperature: float = 1.0,
+                ignore_index: int = 255, want_grad: bool = False, grad_scale: float = 1.0
+                ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(out4 = [total, surrogate, kl, clipped share], logp, grad or None) of sampled labels.  r = exp(logp -
+    old_logprobs): surrogate = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(ref - logp) - (ref - logp) - 1
+    (0 without ref_logprobs), total = surrogate + kl_weight * kl, averaged over all counted positions ("token") or as the
+    mean over sequences of each one's mean ("sequence"; a sequence without counted positions adds 0).  advantages fp32, one
+    a sequence or one a position.  grad = grad_scale * d total / d logits, taken in the same pass over the logits.  logits and labels as token_logprobs."""
+    out4, logp, grad, _, _ = spice_ops().policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs, class_dim,
+                                                     temperature, ignore_index, clip_low, clip_high, kl_weight,
+                                                     _choice(_POLICY_REDUCTIONS, reduction, "reduction"), want_grad,
+                                                     grad_scale, False)
+    return out4, logp, grad if want_grad else None
+
+
+# --------------------------------------------------------------------------------------
+# gradient norm, clipping, Adam
+
+
+def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """Norm over all elements of all tensors (2, or float("inf"): the largest magnitude), a device scalar; no host
+    synchronisation.  The tensors: one device, one type (fp32 / fp16 / bf16), dense in any order of their axes.  Squares
+    are summed in fp64 in a fixed order."""
+    return spice_ops().grad_norm(grads, 0.0, _norm_inf(norm_type))[0]
+
+
+def _norm_inf(norm_type: float) -> bool:
+    if norm_type not in (2.0, float("inf")):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
+    return norm_type != 2.0
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                   out: Optional[Sequence[torch.Tensor]] = None, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """grads *= min(1, max_norm / (norm + 1e-6)), the norm taken over all of them; returns that norm, a device scalar.
+    `out`: where the clipped gradients go instead (tensors of the same shapes, of the gradients' type or fp32: half
+    precision gradients clipped into fp32 ones round nowhere).  Nothing is moved where the factor is 1 and the gradients
+    stay in place.  A NaN norm makes the gradients NaN; with error_if_nonfinite it raises first (a host synchronisation).
+    Tensors as grad_norm; no two of the written ones may share memory."""
+    f = spice_ops()
+    record = f.grad_norm(grads, float(max_norm), _norm_inf(norm_type))
+    if error_if_nonfinite and not bool(torch.isfinite(record[0])):
+        raise RuntimeError(f"the gradient norm of order {norm_type} is not finite: the gradients are left as they are")
+    f.grad_clip(grads, grads if out is None else out, record)
+    return record[0]
+
+
+def adam_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
+              exp_avg_sq: Sequence[torch.Tensor], step, *, lr: float, betas: Tuple[float, float] = (0.9, 0.999),
+              eps: float = 1e-8, weight_decay: float = 0.0, decoupled: bool = False, max_norm: Optional[float] = None,
+              norm: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """One Adam step of every tensor, in place; params and grads of one type (fp32 / fp16 / bf16), the moments fp32, each
+    dense and in its parameter's order of axes.  weight_decay joins the gradient, or shrinks the parameter
+    (`decoupled`).  max_norm: the gradients count as clipped to that norm over all of them (they are read, not written);
+    `norm` a norm taken before (grad_norm over more tensors than these, say).  step: this step's number, from 1, or an
+    int64 device tensor with one count, which the call raises by one first (so a captured launch counts on).
+    Returns the norm, a device scalar, with max_norm; else None."""
+    if max_norm is not None and not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if norm is not None and max_norm is None:
+        raise ValueError("a norm without a max_norm clips nothing")
+    tensor = isinstance(step, torch.Tensor)
+    record = spice_ops().adam_step(params, grads, exp_avg, exp_avg_sq, step if tensor else None, 1 if tensor else int(step), lr,
+                                   betas[0], betas[1], eps, weight_decay, decoupled, -1.0 if max_norm is None else max_norm, norm)
+    return None if max_norm is None else record[0]

@@ -22,6 +22,7 @@ _FLAGS = [
     ("--fine-tune-epochs", "fine_tune_epochs", dict(type=int, help="Epochs for intermediate fine-tuning")),
     ("--final-fine-tune-epochs", "final_fine_tune_epochs", dict(type=int, help="Epochs for final fine-tuning")),
     ("--lr", "fine_tune_lr", dict(type=float, help="Learning rate for fine-tuning")),
+    ("--max-grad-norm", "max_grad_norm", dict(type=float, help="Clip the global gradient norm of each fine-tuning step")),
     ("--batch-size", "batch_size", dict(type=int, help="Batch size for fine-tuning")),
     ("--early-stop-patience", "early_stop_patience", dict(type=int, help="Early stopping patience")),
     ("--data-root", "data_root", dict(type=str, help="Root directory for dataset")),
@@ -69,6 +70,9 @@ def validate_args(args: argparse.Namespace) -> None:
         raise ValueError("Pruning ratio must be between 0 and 1")
     if args.steps and args.steps <= 0:
         raise ValueError("Number of steps must be positive")
+    limit = getattr(args, "max_grad_norm", None)
+    if limit is not None and not limit > 0:
+        raise ValueError("Gradient norm limit must be positive")
     if args.data_root and not Path(args.data_root).exists():
         logging.getLogger(__name__).warning(f"Data root directory does not exist: {args.data_root}")
 

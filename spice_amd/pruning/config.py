@@ -29,6 +29,7 @@ class PruningConfig:
     final_fine_tune_epochs: int = 30
     fine_tune_lr: float = 1e-4
     weight_decay: float = 1e-4
+    max_grad_norm: Optional[float] = None  # clip the global gradient norm of each fine-tuning step
     use_cosine_annealing: bool = True
     lr_warmup_epochs: int = 2
     lr_min_factor: float = 0.01

@@ -1,12 +1,16 @@
 """KD-Lite losses with the reference's module interface (pruning/losses.py:15-162), computed by
 the fused HIP kernel: one pass over the logits yields ce, kd and total (and, when the student
-needs a gradient, d(total)/d(student) in the same pass)."""
+needs a gradient, d(total)/d(student) in the same pass).
+
+Beside them: label log-probabilities, the preference loss and the clipped policy loss, for fine-tuning a pruned student
+from pairs of label maps (or answers) or from scores of sampled ones, held near the frozen teacher."""
 from __future__ import annotations
 
-from typing import Dict, Optional
+from typing import Dict, Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -162,3 +166,141 @@ class SegmentationLoss(nn.Module):
         # alpha = 1: total == ce, and its gradient is the one the fused pass already wrote
         total, _, _ = _apply(p, p.detach(), targets.long().contiguous(), opts)
         return total
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, how):
+        logp, stats = ops.token_logprobs(logits.detach(), labels, **how)
+        ctx.how = how
+        ctx.save_for_backward(logits, labels, stats)
+        return logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, labels, stats = ctx.saved_tensors
+        return ops.token_logprobs_grad(logits.detach(), labels, stats, g.contiguous(), **ctx.how), None, None
+
+
+class _Preference(torch.autograd.Function):
+    """The pair's factor depends on all positions of both sequences, so the gradient is a second pass over the logits; it
+    runs in backward, where the upstream factor (a loss scale) is known, and rounds once."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, ref, how, opts):
+        total, rewards, weight, stats = ops.spice_ops().preference_loss(
+            logits.detach(), labels, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts)
+        ctx.how = how
+        ctx.save_for_backward(logits, labels, stats, weight)
+        ctx.mark_non_differentiable(rewards)
+        return total, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_total, _g_rewards):
+        logits, labels, stats, weight = ctx.saved_tensors
+        return ops.token_logprobs_grad(logits.detach(), labels, stats, weight, device_scale=g_total.float().contiguous(),
+                                       **ctx.how), None, None, None, None
+
+
+class _Policy(torch.autograd.Function):
+    """The gradient for an upstream factor of 1 is written by the forward pass over the logits; backward takes it anew
+    from the logits where the factor is another one (decided on the device), so that it is rounded once either way."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, old, advantages, ref, how, opts, want):
+        out4, logp, grad, stats, weight = ops.spice_ops().policy_loss(
+            logits.detach(), labels, old, advantages, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts,
+            want, 1.0, want)
+        ctx.how = how
+        ctx.grad = grad if want else None
+        ctx.save_for_backward(logits, labels, stats, weight)
+        parts = out4.unbind()
+        total, rest = parts[0].clone(), [p.clone() for p in parts[1:]]
+        ctx.mark_non_differentiable(logp, *rest)
+        return (total, *rest, logp)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_total, *_):
+        logits, labels, stats, weight = ctx.saved_tensors
+        out, ctx.grad = ctx.grad, None   # (handed on: a second backward through the same graph takes a new one)
+        return (ops.token_logprobs_grad(logits.detach(), labels, stats, weight, device_scale=g_total.float().contiguous(),
+                                        out=out, **ctx.how), *([None] * 7))
+
+
+def _one_stride(t: torch.Tensor, first: int, last: int) -> bool:
+    """Whether the axes first .. last - 1 of t lie at one stride in memory."""
+    size = step = None
+    for d in range(last - 1, first - 1, -1):
+        if t.shape[d] == 1:
+            continue
+        if size is not None and t.stride(d) != size * step:
+            return False
+        if size is None:
+            size, step = 1, t.stride(d)
+        size *= t.shape[d]
+    return True
+
+
+def _positions(logits: torch.Tensor, labels: torch.Tensor, class_dim: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    last = class_dim in (-1, logits.dim() - 1)
+    if not _one_stride(logits, 1 if last else 2, logits.dim() - 1 if last else logits.dim()):
+        logits = logits.contiguous()
+    labels = labels.long()
+    return logits, labels if _one_stride(labels, 1, labels.dim()) else labels.contiguous()
+
+
+def _constant(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.detach().float().contiguous()
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, class_dim: int = 1, temperature: float = 1.0,
+                   ignore_index: int = 255) -> torch.Tensor:
+    """log softmax(logits / temperature) at the labels (fp32, the labels' shape, 0 where ignored), differentiable by the
+    logits.  Under torch.no_grad() it gives a reference's or an older policy's values for the two losses below.
+    Arguments as ops.token_logprobs."""
+    how = dict(class_dim=class_dim, temperature=temperature, ignore_index=ignore_index)
+    return _TokenLogprobs.apply(*_positions(logits, labels, class_dim), how)
+
+
+class PreferenceLoss(nn.Module):
+    """Paired log ratios against a frozen reference: the first half of the batch is preferred to the second half, pair by
+    pair (ops.preference_loss has the formulas).  forward(logits, labels, ref_logprobs) gives {"total", "rewards"};
+    ref_logprobs = token_logprobs(reference(x), labels) under no_grad."""
+
+    def __init__(self, beta: float = 0.1, label_smoothing: float = 0.0, loss_type: str = "sigmoid", average: bool = False,
+                 class_dim: int = 1, temperature: float = 1.0, ignore_index: int = 255):
+        super().__init__()
+        self.beta, self.label_smoothing, self.average = beta, label_smoothing, average
+        self.loss_type = loss_type
+        self.how = dict(class_dim=class_dim, temperature=temperature, ignore_index=ignore_index)
+
+    def forward(self, logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor) -> Dict[str, torch.Tensor]:
+        opts = (self.beta, self.label_smoothing, ops._choice(ops._PREFERENCE_TYPES, self.loss_type, "loss_type"), self.average)
+        logits, labels = _positions(logits, labels, self.how["class_dim"])
+        total, rewards = _Preference.apply(logits, labels, _constant(ref_logprobs), self.how, opts)
+        return {"total": total, "rewards": rewards}
+
+
+class ClippedPolicyLoss(nn.Module):
+    """Clipped importance-ratio surrogate of sampled labels with a KL term that holds the policy near a reference
+    (ops.policy_loss has the formulas).  forward(logits, labels, old_logprobs, advantages, ref_logprobs) gives
+    {"total", "surrogate", "kl", "clipped", "logprobs"}; only "total" is differentiable."""
+
+    def __init__(self, clip_low: float = 0.2, clip_high: float = 0.2, kl_weight: float = 0.0, reduction: str = "token",
+                 class_dim: int = 1, temperature: float = 1.0, ignore_index: int = 255):
+        super().__init__()
+        self.clip_low, self.clip_high, self.kl_weight, self.reduction = clip_low, clip_high, kl_weight, reduction
+        self.how = dict(class_dim=class_dim, temperature=temperature, ignore_index=ignore_index)
+
+    def forward(self, logits: torch.Tensor, labels: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                ref_logprobs: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
+        opts = (self.clip_low, self.clip_high, self.kl_weight,
+                ops._choice(ops._POLICY_REDUCTIONS, self.reduction, "reduction"))
+        logits, labels = _positions(logits, labels, self.how["class_dim"])
+        want = torch.is_grad_enabled() and logits.requires_grad
+        out = _Policy.apply(logits, labels, _constant(old_logprobs), _constant(advantages), _constant(ref_logprobs), self.how,
+                            opts, want)
+        return dict(zip(("total", "surrogate", "kl", "clipped", "logprobs"), out))

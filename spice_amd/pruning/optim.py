@@ -1,0 +1,81 @@
+"""Adam that clips the global gradient norm as it reads the gradients: the norm's launch, then one launch that updates
+every tensor; the clipped gradients are never written and the host never waits for the norm.  The reference's fine-tune
+loop steps torch's Adam without clipping (pruning/trainer.py:160-228); the trainer takes this optimiser where
+`max_grad_norm` is set."""
+from __future__ import annotations
+
+from typing import Dict, List, Optional, Tuple
+
+import torch
+
+from .. import ops
+
+
+class ClippedAdam(torch.optim.Optimizer):
+    """Parameters and gradients fp32 / fp16 / bf16 on one HIP device, moments fp32.  `decoupled`: weight decay as
+    p *= 1 - lr * weight_decay, else added to the gradient (torch.optim.Adam's way).  max_grad_norm: the gradients of
+    all groups together count as clipped to that norm; `last_grad_norm` is that norm of the last step, a device scalar."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.0, decoupled: bool = False, max_grad_norm: Optional[float] = None):
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError("lr, eps and weight_decay must not be negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.last_grad_norm: Optional[torch.Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled))
+
+    def _state_of(self, p: torch.Tensor) -> dict:
+        state = self.state[p]
+        if not state:
+            state["step"] = 0
+            for key in ("exp_avg", "exp_avg_sq"):
+                state[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        return state
+
+    @staticmethod
+    def _grad_of(p: torch.Tensor) -> torch.Tensor:
+        if p.grad.is_sparse:
+            raise RuntimeError("ClippedAdam takes no sparse gradients")
+        # the update walks a parameter and its gradient in memory order
+        return p.grad if p.grad.stride() == p.stride() or p.numel() <= 1 else torch.empty_like(p).copy_(p.grad)
+
+    def _norm(self, grads: List[torch.Tensor]) -> torch.Tensor:
+        kinds: Dict[torch.dtype, list] = {}
+        for g in grads:
+            kinds.setdefault(g.dtype, []).append(g)
+        norms = [ops.grad_norm(k) for k in kinds.values()]
+        return norms[0] if len(norms) == 1 else torch.linalg.vector_norm(torch.stack(norms))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ClippedAdam counts its steps on the host: capture ops.adam_step with a device step count")
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        # parameters of a group that have taken as many steps and are of one type go in one launch
+        sets: Dict[tuple, list] = {}
+        for i, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                if p.grad is not None:
+                    sets.setdefault((i, self._state_of(p)["step"], p.dtype), []).append((p, self._grad_of(p)))
+        if not sets:
+            return loss
+        norm = None
+        if self.max_grad_norm is not None and len(sets) > 1:
+            norm = self._norm([g for s in sets.values() for _, g in s])
+        for (i, steps, _), members in sets.items():
+            group, states = self.param_groups[i], [self.state[p] for p, _ in members]
+            got = ops.adam_step([p for p, _ in members], [g for _, g in members], [s["exp_avg"] for s in states],
+                                [s["exp_avg_sq"] for s in states], steps + 1, lr=float(group["lr"]), betas=group["betas"],
+                                eps=group["eps"], weight_decay=group["weight_decay"], decoupled=group["decoupled"],
+                                max_norm=self.max_grad_norm, norm=norm)
+            for s in states:
+                s["step"] = steps + 1
+            self.last_grad_norm = got if norm is None else norm
+        return loss

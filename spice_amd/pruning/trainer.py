@@ -29,6 +29,7 @@ from .dataset import PruningDataHandler
 from .kd_lite import KnowledgeDistiller
 from .losses import SegmentationLoss
 from .lr_scheduler import create_scheduler
+from .optim import ClippedAdam
 from .utils import generate_config_hash, set_random_seeds
 
 logger = logging.getLogger(__name__)
@@ -93,6 +94,9 @@ class PruningTrainer:
         return SegmentationLoss(self.config.num_classes).to(self.config.device)
 
     def _setup_optimizer(self, model: nn.Module) -> optim.Optimizer:
+        if getattr(self.config, "max_grad_norm", None) is not None:
+            return ClippedAdam([p for p in model.parameters() if p.requires_grad], lr=self.config.fine_tune_lr,
+                               weight_decay=self.config.weight_decay, max_grad_norm=self.config.max_grad_norm)
         return optim.Adam([p for p in model.parameters() if p.requires_grad], lr=self.config.fine_tune_lr,
                           weight_decay=self.config.weight_decay)
 

@@ -1,0 +1,293 @@
+"""Gradient norm, clipping and Adam on the GPU against the 64-bit oracle.  u = 2^-24.
+
+Tolerances: the norm's squares are summed in fp64 (n 2^-53, below everything here), its square root rounds to fp32 once: u.
+The factor: its rounding and the norm's are not joined (both come from the fp64 norm): u; a clipped value: the product's
+and the factor's u, plus half a step of the output's type."""
+import copy
+import math
+
+import pytest
+import torch
+
+from oracle import tokenloss as ot
+from spice_amd import ops
+from spice_amd.pruning.optim import ClippedAdam
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+LEAST = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -126}
+SIZES = {"one": [1], "small": [5, 1, 0, 64, 7, 2304, 3], "odd": [8191, 8192, 8193, 100003, 17], "many": [3 + 5 * i for i in range(700)],
+         "large": [3000001, 64, 1 << 20]}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+def _tensors(sizes, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(scale * torch.randn(s, generator=g)).to(dtype) for s in sizes]
+
+
+def _dev(ts, dev):
+    return [t.to(dev) for t in ts]
+
+
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("limit", [0.5, 1e6])
+def test_clip(dev, sizes, dtype, limit):
+    host = _tensors(sizes, dtype, 1)
+    norm = ot.grad_norm(host)
+    factor = ot.clip_factor(norm, limit)
+    for out_type in {dtype, torch.float32}:
+        grads = _dev(host, dev)
+        out = [torch.full(g.shape, math.nan, dtype=out_type, device=dev) for g in grads]
+        got = ops.clip_grad_norm(grads, limit, out=out)
+        assert got.dtype == torch.float32 and got.dim() == 0
+        assert abs(got.item() - norm.item()) <= 2 * U * norm.item()
+        for g, o, h in zip(grads, out, host):
+            assert torch.equal(g.cpu(), h)
+            want = h.double() * factor
+            assert ((o.cpu().double() - want).abs() <= (3 * U + HALF_STEP[out_type]) * want.abs() + LEAST[out_type] / 2).all()
+    place = _dev(host, dev)
+    versions = [t._version for t in place]
+    got = ops.clip_grad_norm(place, limit)
+    same = ops.clip_grad_norm(_dev(host, dev), limit, out=[torch.empty_like(t) for t in place])
+    assert torch.equal(got, same)
+    want = [torch.empty_like(t) for t in place]
+    ops.clip_grad_norm(_dev(host, dev), limit, out=want)
+    assert all(torch.equal(a, b) for a, b in zip(place, want))
+    assert all(t._version > v for t, v in zip(place, versions))
+    assert torch.equal(ops.grad_norm(_dev(host, dev)), got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_largest_magnitude(dev, dtype):
+    host = _tensors(SIZES["odd"], dtype, 2)
+    got = ops.grad_norm(_dev(host, dev), float("inf"))
+    assert got.item() == max(t.double().abs().max().item() for t in host)
+    place = _dev(host, dev)
+    ops.clip_grad_norm(place, 1.0, float("inf"))
+    want = host[3].double() / (got.item() + 1e-6)
+    assert ((place[3].cpu().double() - want).abs() <= (3 * U + HALF_STEP[dtype]) * want.abs() + LEAST[dtype] / 2).all()
+    host[1][5] = math.nan
+    assert math.isnan(ops.grad_norm(_dev(host, dev), float("inf")).item())
+    host[1][5] = -math.inf
+    assert ops.grad_norm(_dev(host, dev), float("inf")).item() == math.inf
+
+
+def test_extreme_and_nonfinite_gradients(dev):
+    for scale in (1e20, 1e-25, 1e-38):
+        host = _tensors([5000, 3], torch.float32, 3, scale)
+        got, want = ops.grad_norm(_dev(host, dev)), ot.grad_norm(host)
+        assert abs(got.item() - want.item()) <= 2 * U * want.item()
+    for bad in (math.nan, math.inf):
+        host = _tensors([50, 9], torch.float32, 4)
+        host[1][4] = bad
+        grads = _dev(host, dev)
+        with pytest.raises(RuntimeError, match="not finite"):
+            ops.clip_grad_norm(grads, 1.0, error_if_nonfinite=True)
+        assert torch.equal(grads[0].cpu(), host[0])
+        norm = ops.clip_grad_norm(grads, 1.0)
+        if math.isnan(bad):
+            assert math.isnan(norm.item()) and torch.isnan(grads[0]).all()
+        else:    # a factor of 0: the infinite value alone becomes NaN
+            assert norm.item() == math.inf and (grads[0] == 0).all() and torch.isnan(grads[1][4]) and (grads[1][:4] == 0).all()
+    zero = [torch.zeros(77, device=dev)]
+    assert ops.clip_grad_norm(zero, 0.0).item() == 0 and (zero[0] == 0).all()
+
+
+def test_strides_alignment_and_orders(dev):
+    """Tensors off 16 bytes, in channels-last order, transposed: walked in memory order; gaps are refused."""
+    base = torch.randn(40000, generator=torch.Generator().manual_seed(5)).to(dev)
+    grads = [base[1:10001], base[10003:10004], base[20000:20000 + 4 * 9 * 7 * 5].view(4, 9, 7, 5).contiguous(memory_format=torch.channels_last),
+             base[30000:30600].view(20, 30).t()]
+    want = ot.grad_norm([g.cpu() for g in grads])
+    assert abs(ops.grad_norm(grads).item() - want.item()) <= 2 * U * want.item()
+    out = [torch.empty_like(g) for g in grads]
+    assert out[2].is_contiguous(memory_format=torch.channels_last) and out[3].stride() == grads[3].stride()
+    ops.clip_grad_norm(grads, 1.0, out=out)
+    f = ot.clip_factor(want, 1.0)
+    for g, o in zip(grads, out):
+        assert ((o.cpu().double() - g.cpu().double() * f).abs() <= 4 * U * g.cpu().double().abs()).all()
+    with pytest.raises(ValueError, match="dense"):
+        ops.grad_norm([base[:100:2]])
+    with pytest.raises(ValueError, match="dense"):
+        ops.grad_norm([base[:1].expand(5)])
+    with pytest.raises(ValueError, match="strides"):
+        ops.clip_grad_norm([grads[3]], 1.0, out=[torch.empty(30, 20, device=dev)])
+
+
+def test_shared_memory_and_mixed_types_are_refused(dev):
+    a, b = torch.ones(100, device=dev), torch.ones(50, device=dev)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.clip_grad_norm([a, a], 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.clip_grad_norm([a[:50], a[49:99]], 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.clip_grad_norm([a[:50], b], 1.0, out=[b, a[50:]])
+    with pytest.raises(TypeError):
+        ops.grad_norm([a, b.half()])
+    with pytest.raises(TypeError):
+        ops.grad_norm([a.double()])
+    with pytest.raises(TypeError, match="out"):
+        ops.clip_grad_norm([a], 1.0, out=[a.half()])
+    with pytest.raises(RuntimeError, match="grads is on"):
+        ops.grad_norm([a, b.cpu()])
+    with pytest.raises(ValueError, match="max_norm"):
+        ops.clip_grad_norm([a], -1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.adam_step([a], [a], [torch.zeros(100, device=dev)], [torch.zeros(100, device=dev)], 1, lr=1e-3)
+    with pytest.raises(ValueError, match="grads"):
+        ops.adam_step([a], [b], [torch.zeros(100, device=dev)], [torch.zeros(100, device=dev)], 1, lr=1e-3)
+    with pytest.raises(TypeError, match="exp_avg"):
+        ops.adam_step([a], [torch.ones(100, device=dev)], [torch.zeros(100, device=dev).half()], [torch.zeros(100, device=dev)], 1, lr=1e-3)
+    with pytest.raises(ValueError, match="steps count"):
+        ops.adam_step([a], [torch.ones(100, device=dev)], [torch.zeros(100, device=dev)], [torch.zeros(100, device=dev)], 0, lr=1e-3)
+    assert (a == 1).all()
+    # the same gradient read twice is fine: nothing writes it
+    out = [torch.empty_like(a), torch.empty_like(a)]
+    assert abs(ops.clip_grad_norm([a, a], 1.0, out=out).item() - math.sqrt(200)) <= 2 * U * 15 and torch.equal(out[0], out[1])
+
+
+def _adam_tol(p, g, m, v, new, t, factor, lr, betas, eps, decay, dtype):
+    """Bounds of p, m, v after a step.  g' rounds twice (3 with decay in it): 3 u (|g f| + |decay p|).  m: that times 1 - b1,
+    plus 3 u (|m| + |g'|) for the two operations and the constant; v alike with squares, 2 |g'| times the error of g'.
+    The update r m / (sqrt(v) q + eps): the relative errors of m, half of v's, and 6 u for r, q, root, product, quotient."""
+    gp = (g * factor).abs() + decay * p.abs()
+    eg = 3 * U * gp
+    em = (1 - betas[0]) * eg + 3 * U * (m.abs() + gp)
+    ev = (1 - betas[1]) * (2 * gp * eg + 2 * U * gp * gp) + 3 * U * (v + gp * gp)
+    up = (new[0] - p).abs()
+    root = (new[2] / (1 - betas[1] ** t)).sqrt() + eps
+    eu = lr / (1 - betas[0] ** t) * em / root + up * (ev / new[2].clamp(min=1e-300) + 8 * U)
+    ep = eu + 3 * U * p.abs()
+    return ep + HALF_STEP[dtype] * (new[0].abs() + ep) + LEAST[dtype] / 2, em + U * new[1].abs(), ev + U * new[2]
+
+
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("decoupled, decay, limit", [(False, 0.0, None), (False, 0.1, 0.5), (True, 0.1, 1e6)])
+def test_adam_step(dev, sizes, dtype, decoupled, decay, limit):
+    p, g = _tensors(sizes, dtype, 6), _tensors(sizes, dtype, 7, 0.1)
+    m, v = _tensors(sizes, torch.float32, 8, 0.01), [t.square() for t in _tensors(sizes, torch.float32, 9, 0.1)]
+    opts = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8)
+    norm = ot.grad_norm(g)
+    factor = ot.clip_factor(norm, limit).item() if limit is not None else 1.0
+    pd, gd, md, vd = (_dev(x, dev) for x in (p, g, m, v))
+    step = torch.tensor([4], device=dev)
+    got = ops.adam_step(pd, gd, md, vd, step, weight_decay=decay, decoupled=decoupled, max_norm=limit, **opts)
+    assert step.item() == 5 and (got is None) == (limit is None)
+    if got is not None:
+        assert abs(got.item() - norm.item()) <= 2 * U * norm.item()
+    # the host's count gives the same bits, and so does a norm taken before
+    ph, mh, vh = (_dev(x, dev) for x in (p, m, v))
+    ops.adam_step(ph, gd, mh, vh, 5, weight_decay=decay, decoupled=decoupled, max_norm=limit, **opts)
+    for a, b in ((pd, ph), (md, mh), (vd, vh)):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for i in range(len(sizes)):
+        assert torch.equal(gd[i].cpu(), g[i])
+        new = ot.adam(p[i], g[i], m[i], v[i], 5, factor, weight_decay=decay, decoupled=decoupled, **opts)
+        tol = _adam_tol(p[i].double(), g[i].double(), m[i].double(), v[i].double(), new, 5, factor, opts["lr"], opts["betas"],
+                        opts["eps"], 0.0 if decoupled else decay, dtype)
+        for name, a, w, t in zip("pmv", (pd, md, vd), new, tol):
+            off = (a[i].cpu().double() - w).abs()
+            assert (off <= t).all(), (name, i, float((off / t).max()))
+
+
+def test_adam_first_steps_and_zero_gradients(dev):
+    """From empty moments the first step moves every parameter by lr times its gradient's sign; a zero gradient moves
+    nothing; steps accumulate as torch.optim.Adam's do in 64 bits."""
+    p, g = [torch.zeros(10, device=dev)], [torch.tensor([1.0, -1e-3, 1e-12, 0.0, 5e4, -2.0, 3.0, 0.0, 1e-6, -1e10], device=dev)]
+    m, v = [torch.zeros(10, device=dev)], [torch.zeros(10, device=dev)]
+    ops.adam_step(p, g, m, v, 1, lr=0.1, eps=0.0)
+    want = torch.where(g[0] == 0, torch.full((), math.nan, device=dev), -0.1 * torch.sign(g[0]))
+    seen = ~torch.isnan(want) & (g[0].abs() > 1e-10)     # (squares of 1e-12 times 1e-3 are below fp32's normal range)
+    assert ((p[0] - want).abs()[seen] <= 0.1 * 16 * U).all()
+    host = torch.randn(2000, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    ref = torch.nn.Parameter(host.clone())
+    mine = torch.nn.Parameter(host.float().to(dev))
+    a, b = torch.optim.Adam([ref], lr=1e-2, weight_decay=1e-2), ClippedAdam([mine], lr=1e-2, weight_decay=1e-2)
+    for k in range(5):
+        gr = torch.randn(2000, generator=torch.Generator().manual_seed(10 + k), dtype=torch.float64)
+        ref.grad, mine.grad = gr, gr.float().to(dev)
+        a.step()
+        b.step()
+    # a step's relative error is at most 20 u of its 1e-2, the parameter's own rounding u of about 4, five times
+    assert (mine.detach().cpu().double() - ref.detach()).abs().max() <= 5 * (20 * U * 1e-1 + 8 * U)
+
+
+def test_clipped_adam_is_clip_then_adam(dev):
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 3), torch.nn.ReLU(), torch.nn.Conv2d(8, 5, 1)).to(dev)
+    net[0].weight.data = net[0].weight.data.contiguous(memory_format=torch.channels_last)
+    twin = copy.deepcopy(net)
+    groups = [dict(params=net[0].parameters(), lr=1e-2), dict(params=net[2].parameters())]
+    fused, one = ClippedAdam(groups, lr=1e-3, max_grad_norm=0.05), ClippedAdam(
+        [dict(params=twin[0].parameters(), lr=1e-2), dict(params=twin[2].parameters())], lr=1e-3)
+    x = torch.randn(2, 3, 9, 9, device=dev)
+    for k in range(3):
+        for n, opt in ((net, fused), (twin, one)):
+            opt.zero_grad()
+            n(x).square().mean().backward()
+            if k == 1:
+                n[2].bias.grad = None            # a parameter left out keeps its own count
+        norm = ops.clip_grad_norm([p.grad for p in twin.parameters() if p.grad is not None], 0.05)
+        fused.step()
+        one.step()
+        assert abs(fused.last_grad_norm.item() - norm.item()) <= 1e-5 * norm.item()
+    assert fused.state[net[2].bias]["step"] == 2 and fused.state[net[0].weight]["step"] == 3
+    # clipped gradients are rounded once more in the twin's buffers, and its networks' gradients follow its parameters: a
+    # few u of the update a step
+    for p, q in zip(net.parameters(), twin.parameters()):
+        assert (p - q).abs().max() <= 3 * 1e-2 * 2.0 ** -12
+    state = copy.deepcopy(fused.state_dict())
+    again = ClippedAdam([dict(params=net[0].parameters(), lr=1e-2), dict(params=net[2].parameters())], lr=1e-3, max_grad_norm=0.05)
+    again.load_state_dict(state)
+    assert again.state[net[2].bias]["step"] == 2 and torch.equal(again.state[net[0].weight]["exp_avg"], fused.state[net[0].weight]["exp_avg"])
+    loss = again.step(lambda: net(x).square().mean())
+    assert loss.requires_grad
+
+
+def test_captured_step_counts_on(dev):
+    """adam_step with a device step count in a graph: three replays, eager work between, give what three eager steps give."""
+    def fresh():
+        return [_dev(_tensors([5000, 7, 300000], torch.float32, s, 0.1), dev) for s in (1, 2, 3)] + [
+            [t.square() for t in _dev(_tensors([5000, 7, 300000], torch.float32, 4, 0.1), dev)], torch.zeros(1, dtype=torch.int64, device=dev)]
+
+    opts = dict(lr=1e-2, weight_decay=1e-2, max_norm=0.3)
+    p, g, m, v, step = fresh()
+    q, h, n, w, count = fresh()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        norm = ops.adam_step(q, h, n, w, count, **opts)
+    opt = ClippedAdam([torch.nn.Parameter(q[0])])
+    for k in range(3):
+        for a, b in zip(g, h):
+            a.mul_(1.5)
+            b.mul_(1.5)
+        want = ops.adam_step(p, g, m, v, step, **opts)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(want, norm) and step.item() == count.item() == k + 1
+        for x, y in ((p, q), (m, n), (v, w)):
+            assert all(torch.equal(a, b) for a, b in zip(x, y))
+    del opt
+
+
+def test_another_stream(dev):
+    host = _tensors(SIZES["many"], torch.float32, 1)
+    want = ops.grad_norm(_dev(host, dev))
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    sets = [_dev(host, dev) for _ in sides]
+    torch.cuda.synchronize()
+    norms = []
+    for s, grads in zip(sides, sets):
+        with torch.cuda.stream(s):
+            norms.append(ops.clip_grad_norm(grads, 1.0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(n, want) for n in norms) and all(torch.equal(a, b) for a, b in zip(*sets))

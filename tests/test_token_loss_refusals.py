@@ -1,0 +1,186 @@
+"""What the loss and update entry points refuse, and what runs without a device."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import tokenloss as ot
+from spice_amd import _native as nat
+from spice_amd import ops
+from spice_amd.pruning.cli_helpers import build_config_from_args, create_parser, validate_args
+from spice_amd.pruning.losses import ClippedPolicyLoss, PreferenceLoss, token_logprobs
+from spice_amd.pruning.optim import ClippedAdam
+
+X, Y, F = torch.zeros(2, 5, 3), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.token_logprobs(X, Y),
+    lambda: ops.token_logprobs_grad(X, Y, torch.zeros(2, 3, 2), F),
+    lambda: ops.preference_loss(X, Y, F),
+    lambda: ops.policy_loss(X, Y, F, torch.zeros(2)),
+    lambda: token_logprobs(X, Y),
+    lambda: PreferenceLoss()(X, Y, F),
+    lambda: ClippedPolicyLoss()(X, Y, F, torch.zeros(2)),
+    lambda: ops.grad_norm([F]),
+    lambda: ops.clip_grad_norm([F], 1.0),
+    lambda: ops.adam_step([F], [F], [F], [F], 1, lr=1e-3),
+])
+def test_host_tensors_are_refused(call):
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        call()
+
+
+def test_choices_and_empty_lists_are_refused():
+    with pytest.raises(ValueError, match="loss_type"):
+        ops.preference_loss(X, Y, F, loss_type="hinge")
+    with pytest.raises(ValueError, match="reduction"):
+        ops.policy_loss(X, Y, F, F, reduction="sum")
+    with pytest.raises(ValueError, match="norm_type"):
+        ops.grad_norm([F], norm_type=1.0)
+    for call in (lambda: ops.grad_norm([]), lambda: ops.clip_grad_norm([], 1.0),
+                 lambda: ops.adam_step([], [], [], [], 1, lr=1e-3)):
+        with pytest.raises(ValueError, match="no tensors"):
+            call()
+    with pytest.raises(ValueError, match="max_norm"):
+        ops.adam_step([F], [F], [F], [F], 1, lr=1e-3, max_norm=-1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        ops.adam_step([F], [F], [F], [F], 1, lr=1e-3, norm=torch.zeros(()))
+
+
+def _logits(**over):
+    f = dict(data=16, dtype=0, pad_=0, n=2, l=3, c=5, n_stride=15, l_stride=5, c_stride=1)
+    f.update(over)
+    return nat.Logits(*[f[k] for k, _ in nat.Logits._fields_])
+
+
+def _labels(**over):
+    f = dict(data=16, n_stride=3, l_stride=1, ignore_index=255)
+    f.update(over)
+    return nat.Labels(*[f[k] for k, _ in nat.Labels._fields_])
+
+
+@pytest.mark.parametrize("x, y, t", [
+    (_logits(data=None), _labels(), 1.0), (_logits(dtype=3), _labels(), 1.0), (_logits(c=0), _labels(), 1.0),
+    (_logits(n=-1), _labels(), 1.0), (_logits(n=1 << 30, l=1 << 30), _labels(), 1.0), (_logits(), _labels(data=None), 1.0),
+    (_logits(), _labels(ignore_index=4), 1.0), (_logits(), _labels(), 0.0), (_logits(), _labels(), -1.0),
+    (_logits(), _labels(), float("nan")), (_logits(), _labels(), float("inf"))])
+def test_c_abi_checks_the_logits_before_anything_is_queued(x, y, t):
+    assert nat.lib().spice_token_logprobs(x, y, t, 16, 16, None) == nat.ERR_ARG
+    assert nat.lib().spice_token_logprobs_grad(x, y, t, 16, 16, 3, 1, 1.0, None, 0, 1, 16, None) == nat.ERR_ARG
+    p = nat.PreferenceParams(t, 0.1, 0.0, 0, 0)
+    assert nat.lib().spice_preference_loss(x, y, 16, p, 16, 16, 16, 16, 16, 16, 1 << 20, None) == nat.ERR_ARG
+    q = nat.PolicyParams(t, 0.2, 0.2, 0.0, 1.0, 0)
+    assert nat.lib().spice_policy_loss(x, y, 16, 16, 1, 0, None, q, 16, 16, None, None, 1, None, 16, 1 << 20, None) == nat.ERR_ARG
+
+
+def test_c_abi_checks_the_losses_options():
+    L = nat.lib()
+    need = L.spice_token_loss_workspace_bytes(2, 3)
+    good = nat.PreferenceParams(1.0, 0.1, 0.0, 0, 0)
+
+    def pref(p=good, x=None, ref=16, total=16, ws=16, size=need):
+        return L.spice_preference_loss(x or _logits(), _labels(), ref, p, total, 16, 16, 16, 16, ws, size, None)
+
+    assert pref(x=_logits(n=3)) == nat.ERR_ARG and pref(x=_logits(n=0)) == nat.ERR_ARG
+    assert pref(ref=None) == nat.ERR_ARG and pref(total=None) == nat.ERR_ARG and pref(ws=None) == nat.ERR_ARG
+    assert pref(ws=20) == nat.ERR_ARG and pref(size=need - 1) == nat.ERR_WORKSPACE
+    for bad in ((1.0, 0.0, 0.0, 0, 0), (1.0, 0.1, 0.5, 0, 0), (1.0, 0.1, -0.1, 0, 0), (1.0, 0.1, 0.0, 2, 0), (1.0, 0.1, 0.1, 1, 0),
+                (1.0, float("nan"), 0.0, 0, 0)):
+        assert pref(nat.PreferenceParams(*bad)) == nat.ERR_ARG
+
+    def pol(*p, ref=None, size=need):
+        return L.spice_policy_loss(_logits(), _labels(), 16, 16, 1, 0, ref, nat.PolicyParams(*p), 16, 16, None, None, 1, None, 16,
+                                   size, None)
+
+    for bad in ((1.0, -0.1, 0.2, 0.0, 1.0, 0), (1.0, 1.1, 0.2, 0.0, 1.0, 0), (1.0, 0.2, -0.2, 0.0, 1.0, 0),
+                (1.0, 0.2, 0.2, 0.1, 1.0, 0), (1.0, 0.2, 0.2, 0.0, 1.0, 2), (1.0, 0.2, 0.2, -1.0, 1.0, 0)):
+        assert pol(*bad) == nat.ERR_ARG
+    assert pol(1.0, 0.2, 0.2, 0.0, 1.0, 0, size=need - 1) == nat.ERR_WORKSPACE
+
+
+def _table(*p):
+    return (ctypes.c_void_p * len(p))(*p)
+
+
+def _counts(*n):
+    return (ctypes.c_int64 * len(n))(*n)
+
+
+def test_c_abi_checks_the_tensor_tables():
+    L = nat.lib()
+    n = _counts(8, 8)
+    need = L.spice_grad_norm_workspace_bytes(n, 2)
+    assert L.spice_grad_norm_workspace_bytes(_counts(8, -1), 2) == 0
+
+    def norm(p=(16, 64), n=n, dtype=0, kind=0, limit=1.0, record=16, ws=16, size=need):
+        return L.spice_grad_norm(_table(*p), n, 2, dtype, kind, limit, record, ws, size, None)
+
+    for bad in (dict(p=(16, None)), dict(p=(16, 18)), dict(n=_counts(8, -8)), dict(dtype=3), dict(kind=2), dict(limit=-1.0),
+                dict(limit=float("nan")), dict(record=None), dict(ws=None), dict(ws=12)):
+        assert norm(**bad) == nat.ERR_ARG, bad
+    assert norm(size=need - 1) == nat.ERR_WORKSPACE
+    assert L.spice_grad_clip(_table(16, 64), 0, _table(16, 64), 1, n, 2, 16, None) == nat.ERR_ARG
+    assert L.spice_grad_clip(_table(16, 64), 0, _table(16, None), 0, n, 2, 16, None) == nat.ERR_ARG
+
+    def adam(lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.0, step=1, limit=1.0, p=(16, 64), size=need):
+        t = _table(16, 64)
+        return L.spice_adam_step(_table(*p), t, t, t, n, 2, 0, nat.AdamParams(lr, b1, b2, eps, wd, step, limit, 0), None, None, 16,
+                                 16, size, None)
+
+    for bad in (dict(lr=-1.0), dict(b1=1.0), dict(b2=1.0), dict(b1=-0.1), dict(eps=-1.0), dict(wd=-1.0), dict(step=0),
+                dict(limit=float("nan")), dict(p=(16, None)), dict(lr=float("nan"))):
+        assert adam(**bad) == nat.ERR_ARG, bad
+    assert adam(size=need - 1) == nat.ERR_WORKSPACE
+
+
+def test_struct_sizes_match_the_header():
+    assert ctypes.sizeof(nat.Logits) == 64 and ctypes.sizeof(nat.Labels) == 32
+    assert ctypes.sizeof(nat.PreferenceParams) == 20 and ctypes.sizeof(nat.PolicyParams) == 24
+    assert ctypes.sizeof(nat.AdamParams) == 56
+
+
+def test_optimizer_checks_its_options():
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(max_grad_norm=0.0)):
+        with pytest.raises(ValueError):
+            ClippedAdam(p, **bad)
+
+
+def test_max_grad_norm_flag(tmp_path):
+    base = ["--model", "DeepLabV3Plus_resnet", "--strategy", "magnitude", "--ratio", "0.5", "--output-dir", str(tmp_path)]
+    args = create_parser().parse_args(base + ["--max-grad-norm", "0.5"])
+    validate_args(args)
+    assert build_config_from_args(args).max_grad_norm == 0.5
+    assert build_config_from_args(create_parser().parse_args(base)).max_grad_norm is None
+    with pytest.raises(ValueError, match="norm limit"):
+        validate_args(create_parser().parse_args(base + ["--max-grad-norm", "0"]))
+
+
+def _differences(f, x, eps=1e-6):
+    got = torch.zeros_like(x)
+    for i in range(x.numel()):
+        d = torch.zeros_like(x)
+        d.view(-1)[i] = eps
+        got.view(-1)[i] = (f(x + d) - f(x - d)) / (2 * eps)
+    return got
+
+
+@pytest.mark.parametrize("loss", ["sigmoid", "ipo", "policy"])
+def test_oracle_gradients_against_differences(loss):
+    """Central differences in 64 bits: their error is eps^2/6 of a third derivative (order 1 here) plus 2^-53 / eps."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 3, 4, dtype=torch.float64, generator=g)
+    y = torch.tensor([[0, 2, 1, 255], [1, 255, 0, 2]])
+    aux = torch.randn(2, 4, generator=g).double() - 1.0
+    adv = torch.randn(2, 4, generator=g)
+
+    def f(v):
+        if loss == "policy":
+            old = ot.token_logprobs(x, y)[0] - 0.1
+            return ot.policy(v, y, old, adv, ref=aux, kl_weight=0.3, reduction="sequence")[0]
+        return ot.preference(v, y, aux, beta=0.5, loss_type=loss)[0]
+
+    v = x.clone().requires_grad_(True)
+    got, = torch.autograd.grad(f(v), v)
+    assert (got - _differences(f, x)).abs().max() <= 1e-8
