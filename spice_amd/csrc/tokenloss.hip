@@ -41,6 +41,7 @@ static Temper temper(float t) {
     const double k = 1.4426950408889634074 / (double)t;
     Temper r;
     r.k = (float)k;
+    if ((double)r.k >= k) r.k = nextafterf(r.k, 0.f);   // k_lo > 0: an excluded class's d = -inf stays -inf in both products
     r.k_lo = (float)(k - (double)r.k);
     r.inv = (float)(1.0 / (double)t);
     return r;
@@ -144,11 +145,28 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy &p, float logp, i
     return r;
 }
 
+template <int K>
+__device__ __forceinline__ void block_sums(double (&v)[K], double *lds, int threads) {
+    const int waves = threads / kWave;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) lds[(threadIdx.x / kWave) * K + k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = 0.0;
+    for (int w = 0; w < waves; ++w)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += lds[w * K + k];
+    __syncthreads();
+}
+
 // ---- one position a workgroup, any strides ----
 
-// LOGP: logp and (max, sum) of each position.  GRAD: weight * d logp / d x from them.  POLICY: logp, and the policy loss's
-// gradient behind it.
-enum { kModeLogp = 0, kModeGrad = 1, kModePolicy = 2, kModePolicyGrad = 3 };
+// Logp: logp and (max, sum) of each position.  Grad: weight * d logp / d x from them.  Preference, Policy: logp, and what the
+// loss sums over positions.  PolicyGrad: the policy loss's gradient behind that.
+enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kModePolicyGrad = 4 };
 
 struct TokArgs {
     Logits x;
@@ -166,7 +184,9 @@ struct TokArgs {
     void *grad;
     int64_t g_sn, g_sl, g_sc;
     Policy policy;
+    const float *ref;       // kModePreference
     const float *share;     // [n] what a position of sequence n counts in the mean
+    double *part;           // sums of each workgroup's item
 };
 
 template <typename T, int MODE>
@@ -225,24 +245,463 @@ __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
     }
 }
 
-// ---- passes over positions ----
+// ---- classes next to each other in memory: LANES lanes hold a row in registers ----
 
-template <int K>
-__device__ __forceinline__ void block_sums(double (&v)[K], double *lds, int threads) {
-    const int waves = threads / kWave;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Vec16 { u32x4 v; };   // 16 bytes at any element's address
+
+template <typename T> constexpr int vec_elements() { return 16 / (int)sizeof(T); }
+
+__device__ __forceinline__ void unpack(u32x4 r, float (&v)[4], float) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const f4 f = __builtin_bit_cast(f4, r);
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-        for (int k = 0; k < K; ++k) lds[(threadIdx.x / kWave) * K + k] = v[k];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = 0.0;
-    for (int w = 0; w < waves; ++w)
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += lds[w * K + k];
-    __syncthreads();
+    for (int k = 0; k < 4; ++k) v[k] = f[k];
 }
+__device__ __forceinline__ void unpack(u32x4 r, float (&v)[8], _Float16) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 h = __builtin_bit_cast(h8, r);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (float)h[k];
+}
+__device__ __forceinline__ void unpack(u32x4 r, float (&v)[8], __bf16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned low = r[k] << 16, high = r[k] & 0xffff0000u;   // (bfloat16 is fp32's upper half)
+        v[2 * k] = __builtin_bit_cast(float, low);
+        v[2 * k + 1] = __builtin_bit_cast(float, high);
+    }
+}
+
+template <typename T, int K>
+__device__ __forceinline__ u32x4 pack(const float (&v)[K]) {
+    typedef T tk __attribute__((ext_vector_type(K)));
+    tk t;
+#pragma unroll
+    for (int k = 0; k < K; ++k) t[k] = (T)v[k];
+    return __builtin_bit_cast(u32x4, t);
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_vec(const T *p, int32_t left) {
+    constexpr int K = vec_elements<T>();
+    if (left >= K) return reinterpret_cast<const Vec16 *>(p)->v;
+    float v[K];     // the row's last few classes, -inf behind them: they add nothing
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = k < left ? to_f32(p[k]) : -INFINITY;
+    return pack<T, K>(v);
+}
+
+template <typename T, int K>
+__device__ __forceinline__ void store_vec(T *p, int32_t left, const float (&v)[K]) {
+    if (left >= K) {
+        reinterpret_cast<Vec16 *>(p)->v = pack<T, K>(v);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k < left) p[k] = (T)v[k];
+}
+
+// The gradient of K classes from c0 on.
+template <int K>
+__device__ __forceinline__ void grad_of(float (&v)[K], float m, float each, float w, int32_t y, int32_t c0, Temper t) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = each * exp_of(v[k] - m, t);
+    if ((uint32_t)(y - c0) < (uint32_t)K) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += y - c0 == k ? w : 0.f;
+    }
+}
+
+// (m, s) of LANES neighbouring lanes; LANES > 64: of the workgroup.
+template <int LANES>
+__device__ __forceinline__ void fold_row(float &m, float &s, Temper t, float *lds) {
+    if (LANES <= kWave) {
+        float all = m;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
+        s *= rescale(m, all, t);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
+        m = all;
+    } else {
+        fold_max_sum<LANES>(m, s, t, lds);
+    }
+}
+
+template <typename T, int LANES, int NV, int MODE>
+__global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES) void tok_row_kernel(TokArgs a) {
+    constexpr int K = vec_elements<T>();
+    constexpr int kBlock = LANES < kTokThreads ? kTokThreads : LANES;
+    constexpr bool kGrad = MODE == kModePolicyGrad;
+    __shared__ float lds[2 * kBlock / kWave];
+    const int64_t total = a.x.n * a.x.l;
+    const int32_t lane = threadIdx.x % LANES, classes = (int32_t)a.x.c;
+    for (int64_t at = (int64_t)blockIdx.x * (kBlock / LANES) + __builtin_amdgcn_readfirstlane(threadIdx.x / LANES); at < total;
+         at += (int64_t)gridDim.x * (kBlock / LANES)) {
+        const int64_t n = at / a.x.l, l = at - n * a.x.l;
+        const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
+        const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
+        const int kind = label_kind(y, a.y.ignore, a.x.c);
+        float m = -INFINITY, s = 0.f, logp = kind == kBad ? NAN : 0.f;
+        u32x4 raw[NV];
+        if (kind == kCounted) {
+            const float xl = to_f32(x[y]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int32_t c0 = (i * LANES + lane) * K;
+                if (c0 < classes) raw[i] = load_vec<T>(x + c0, classes - c0);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if ((i * LANES + lane) * K < classes) {
+                    float v[K];
+                    unpack(raw[i], v, T());
+#pragma unroll
+                    for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]);
+                }
+            const float shift = shift_of(m);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if ((i * LANES + lane) * K < classes) {
+                    float v[K];
+                    unpack(raw[i], v, T());
+#pragma unroll
+                    for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+                }
+            fold_row<LANES>(m, s, a.t, lds);
+            logp = (xl - shift_of(m)) * a.t.inv - log_of(s);
+        }
+        if (lane == 0) {
+            a.logp[at] = logp;
+            if (a.stats) a.stats[at] = make_float2(m, s);
+        }
+        if (kGrad) {
+            T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
+            float w = kind == kBad ? NAN : 0.f;
+            if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+            if (a.weight_out && lane == 0) a.weight_out[at] = w;
+            const float shift = shift_of(m);
+            w *= a.t.inv * a.host_scale;
+            const float each = kind == kCounted ? -w / s : w;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int32_t c0 = (i * LANES + lane) * K;
+                if (c0 < classes) {
+                    float v[K];
+                    if (kind == kCounted) {
+                        unpack(raw[i], v, T());
+                        grad_of<K>(v, shift, each, w, (int32_t)y, c0, a.t);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < K; ++k) v[k] = each;
+                    }
+                    store_vec<T, K>(g + c0, classes - c0, v);
+                }
+            }
+        }
+    }
+}
+
+// Rows longer than the registers of a workgroup: read twice, the maximum and sum running along.
+template <typename T, int MODE>
+__global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
+    constexpr int K = vec_elements<T>(), kBlock = 1024, kStep = 4;
+    constexpr bool kGrad = MODE == kModePolicyGrad;
+    __shared__ float lds[2 * kBlock / kWave];
+    const int64_t total = a.x.n * a.x.l;
+    const int32_t classes = (int32_t)a.x.c;
+    for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
+        const int64_t n = at / a.x.l, l = at - n * a.x.l;
+        const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
+        const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
+        const int kind = label_kind(y, a.y.ignore, a.x.c);
+        float m = -INFINITY, s = 0.f, logp = kind == kBad ? NAN : 0.f;
+        if (kind == kCounted) {
+            for (int64_t base = 0; base < classes; base += (int64_t)kStep * kBlock * K) {
+                u32x4 raw[kStep];
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < kStep; ++i) {
+                    const int64_t c0 = base + (i * kBlock + (int)threadIdx.x) * K;
+                    if (c0 < classes) raw[i] = load_vec<T>(x + c0, (int32_t)(classes - c0));
+                }
+#pragma unroll
+                for (int i = 0; i < kStep; ++i)
+                    if (base + (i * kBlock + (int)threadIdx.x) * K < classes) {
+                        float v[K];
+                        unpack(raw[i], v, T());
+#pragma unroll
+                        for (int k = 0; k < K; ++k) top = fmaxf(top, v[k]);
+                    }
+                s *= rescale(m, top, a.t);
+                m = top;
+                const float shift = shift_of(m);
+#pragma unroll
+                for (int i = 0; i < kStep; ++i)
+                    if (base + (i * kBlock + (int)threadIdx.x) * K < classes) {
+                        float v[K];
+                        unpack(raw[i], v, T());
+#pragma unroll
+                        for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+                    }
+            }
+            fold_row<kBlock>(m, s, a.t, lds);
+            logp = (to_f32(x[y]) - shift_of(m)) * a.t.inv - log_of(s);
+        }
+        if (threadIdx.x == 0) {
+            a.logp[at] = logp;
+            if (a.stats) a.stats[at] = make_float2(m, s);
+        }
+        if (kGrad) {
+            T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
+            float w = kind == kBad ? NAN : 0.f;
+            if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+            if (a.weight_out && threadIdx.x == 0) a.weight_out[at] = w;
+            const float shift = shift_of(m);
+            w *= a.t.inv * a.host_scale;
+            const float each = kind == kCounted ? -w / s : w;
+            for (int64_t c0 = threadIdx.x * K; c0 < classes; c0 += kBlock * K) {
+                float v[K];
+                if (kind == kCounted) {
+                    unpack(load_vec<T>(x + c0, (int32_t)(classes - c0)), v, T());
+                    grad_of<K>(v, shift, each, w, (int32_t)y, (int32_t)c0, a.t);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) v[k] = each;
+                }
+                store_vec<T, K>(g + c0, (int32_t)(classes - c0), v);
+            }
+        }
+    }
+}
+
+// weight * d logp / d x of rows whose maximum and sum are known: a workgroup takes kGradVecs vectors a lane of one row.
+constexpr int kGradVecs = 4;
+
+template <typename T>
+__global__ __launch_bounds__(kTokThreads) void tok_row_grad_kernel(TokArgs a, int64_t pieces) {
+    constexpr int K = vec_elements<T>();
+    if (a.unless_one && *a.scale == 1.f) return;
+    const int32_t classes = (int32_t)a.x.c;
+    const float out_scale = a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f);
+    for (int64_t item = blockIdx.x; item < a.x.n * a.x.l * pieces; item += gridDim.x) {
+        const int64_t at = item / pieces, n = at / a.x.l, l = at - n * a.x.l;
+        const int32_t c1 = (int32_t)((item - at * pieces) * (kGradVecs * kTokThreads * K)) + (int32_t)threadIdx.x * K;
+        const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
+        T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
+        const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
+        const int kind = label_kind(y, a.y.ignore, a.x.c);
+        if (kind == kCounted) {
+            u32x4 raw[kGradVecs];
+#pragma unroll
+            for (int i = 0; i < kGradVecs; ++i) {
+                const int32_t c0 = c1 + i * kTokThreads * K;
+                if (c0 < classes) raw[i] = load_vec<T>(x + c0, classes - c0);
+            }
+            const float2 st = a.stats_in[at];
+            const float w = a.weight[n * a.w_sn + l * a.w_sl] * out_scale, each = -w / st.y, shift = shift_of(st.x);
+#pragma unroll
+            for (int i = 0; i < kGradVecs; ++i) {
+                const int32_t c0 = c1 + i * kTokThreads * K;
+                if (c0 < classes) {
+                    float v[K];
+                    unpack(raw[i], v, T());
+                    grad_of<K>(v, shift, each, w, (int32_t)y, c0, a.t);
+                    store_vec<T, K>(g + c0, classes - c0, v);
+                }
+            }
+        } else {
+            float v[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] = kind == kBad ? NAN : 0.f;
+#pragma unroll
+            for (int i = 0; i < kGradVecs; ++i) {
+                const int32_t c0 = c1 + i * kTokThreads * K;
+                if (c0 < classes) store_vec<T, K>(g + c0, classes - c0, v);
+            }
+        }
+    }
+}
+
+// ---- positions next to each other in memory: a lane takes VEC of them, walking the class planes ----
+
+// Planes of one position group in registers: CREG classes at most, so the logits are read once for maximum, sum and
+// gradient; CREG = 0: any number, eight planes at a time, read again for the gradient.
+template <typename T, int VEC>
+struct __attribute__((aligned(sizeof(T) * VEC))) Group { T v[VEC]; };
+
+template <typename T, int VEC, int CREG, int MODE>
+__global__ __launch_bounds__(kTokThreads) void tok_planes_kernel(TokArgs a, int64_t tiles) {
+    constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
+    constexpr bool kStats = MODE == kModeGrad;          // (max, sum) given
+    constexpr int K = MODE == kModePreference ? 2 : 4;  // sums of a workgroup
+    constexpr bool kSums = MODE == kModePreference || MODE == kModePolicy || MODE == kModePolicyGrad;
+    constexpr int kStep = 8;
+    __shared__ double lds[kSums ? K * kTokThreads / kWave : 1];
+    if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
+    const int32_t classes = (int32_t)a.x.c;
+    const float out_scale = kGrad ? a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f) : 0.f;
+    for (int64_t item = blockIdx.x; item < a.x.n * tiles; item += gridDim.x) {
+        const int64_t n = item / tiles, l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
+        double sums[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) sums[k] = 0.0;
+        if (l0 < a.x.l) {
+            const T *x = (const T *)a.x.x + n * a.x.sn + l0 * a.x.sl;
+            T *g = kGrad ? (T *)a.grad + n * a.g_sn + l0 * a.g_sl : nullptr;
+            const int64_t at = n * a.x.l + l0;
+            int32_t y[VEC];         // the label, or -1
+            int kind[VEC];
+            bool any = false;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const int64_t label = a.y.y[n * a.y.sn + (l0 + k) * a.y.sl];
+                kind[k] = label_kind(label, a.y.ignore, a.x.c);
+                y[k] = kind[k] == kCounted ? (int32_t)label : -1;
+                any |= kind[k] == kCounted;
+            }
+            float m[VEC], s[VEC], xl[VEC], w[VEC];
+            Group<T, VEC> raw[CREG > 0 ? CREG : 1];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                m[k] = -INFINITY;
+                s[k] = xl[k] = w[k] = 0.f;
+            }
+            if (any && kStats) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    if (kind[k] == kCounted) {
+                        const float2 st = a.stats_in[at + k];
+                        m[k] = st.x;
+                        s[k] = st.y;
+                    }
+            }
+            if (any && CREG > 0) {
+#pragma unroll
+                for (int c = 0; c < CREG; ++c)
+                    if (c < classes) raw[c] = *(const Group<T, VEC> *)(x + c * a.x.sc);
+                if (!kStats) {
+#pragma unroll
+                    for (int c = 0; c < CREG; ++c)
+                        if (c < classes) {
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) {
+                                const float v = to_f32(raw[c].v[k]);
+                                m[k] = fmaxf(m[k], v);
+                                xl[k] = y[k] == c ? v : xl[k];
+                            }
+                        }
+#pragma unroll
+                    for (int c = 0; c < CREG; ++c)
+                        if (c < classes) {
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) s[k] += exp_of(to_f32(raw[c].v[k]) - shift_of(m[k]), a.t);
+                        }
+                }
+            } else if (any && !kStats) {
+                for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
+                    Group<T, VEC> part[kStep];
+                    float top[VEC];
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) top[k] = m[k];
+#pragma unroll
+                    for (int j = 0; j < kStep; ++j)
+                        if (c0 + j < classes) part[j] = *(const Group<T, VEC> *)(x + (int64_t)(c0 + j) * a.x.sc);
+#pragma unroll
+                    for (int j = 0; j < kStep; ++j)
+                        if (c0 + j < classes) {
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) {
+                                const float v = to_f32(part[j].v[k]);
+                                top[k] = fmaxf(top[k], v);
+                                xl[k] = y[k] == c0 + j ? v : xl[k];
+                            }
+                        }
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        s[k] *= rescale(m[k], top[k], a.t);
+                        m[k] = top[k];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kStep; ++j)
+                        if (c0 + j < classes) {
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) s[k] += exp_of(to_f32(part[j].v[k]) - shift_of(m[k]), a.t);
+                        }
+                }
+            }
+            float each[VEC];     // factor of a class's exponential in the gradient, and what else its value gets
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const int64_t l = l0 + k;
+                each[k] = 0.f;
+                if (!kStats) {
+                    const float logp = kind[k] == kCounted ? (xl[k] - shift_of(m[k])) * a.t.inv - log_of(s[k])
+                                       : kind[k] == kBad   ? NAN : 0.f;
+                    a.logp[at + k] = logp;
+                    if (a.stats) a.stats[at + k] = make_float2(m[k], s[k]);
+                    if (MODE == kModePreference && kind[k] != kIgnored) {
+                        sums[0] += (double)logp - (double)a.ref[at + k];
+                        sums[1] += 1.0;
+                    }
+                    if ((MODE == kModePolicy || MODE == kModePolicyGrad) && kind[k] != kIgnored) {
+                        const PolicyTerm t = policy_term(a.policy, logp, at + k, n, l);
+                        sums[0] += t.surrogate;
+                        sums[1] += t.far;
+                        sums[2 % K] += t.over ? 1.0 : 0.0;
+                        sums[3 % K] += 1.0;
+                        w[k] = kind[k] == kBad ? NAN : t.dlogp * (MODE == kModePolicyGrad ? a.share[n] : 0.f);
+                    }
+                    if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at + k] = w[k];
+                } else if (kind[k] == kCounted) {
+                    w[k] = a.weight[n * a.w_sn + l * a.w_sl];
+                } else {
+                    w[k] = kind[k] == kBad ? NAN : 0.f;
+                }
+                if (kGrad) {
+                    w[k] *= out_scale;
+                    each[k] = kind[k] == kCounted ? -w[k] / s[k] : w[k];
+                }
+            }
+            if (kGrad) {
+                const auto store = [&](const Group<T, VEC> &from, int32_t c) {
+                    Group<T, VEC> to;
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        const float e = each[k] * exp_of(to_f32(from.v[k]) - shift_of(m[k]), a.t);
+                        to.v[k] = (T)(kind[k] == kCounted ? (y[k] == c ? e + w[k] : e) : each[k]);
+                    }
+                    *(Group<T, VEC> *)(g + (int64_t)c * a.g_sc) = to;
+                };
+                if (CREG > 0) {
+#pragma unroll
+                    for (int c = 0; c < CREG; ++c)
+                        if (c < classes) store(raw[c], c);
+                } else {
+                    for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
+                        Group<T, VEC> part[kStep];
+#pragma unroll
+                        for (int j = 0; j < kStep; ++j)
+                            if (any && c0 + j < classes) part[j] = *(const Group<T, VEC> *)(x + (int64_t)(c0 + j) * a.x.sc);
+#pragma unroll
+                        for (int j = 0; j < kStep; ++j)
+                            if (c0 + j < classes) store(part[j], c0 + j);
+                    }
+                }
+            }
+        }
+        if (kSums) {
+            block_sums<K>(sums, lds, kTokThreads);
+            if (threadIdx.x == 0)
+#pragma unroll
+                for (int k = 0; k < K; ++k) a.part[item * K + k] = sums[k];
+        }
+    }
+}
+
+// ---- passes over positions ----
 
 struct SumArgs {
     const float *logp;
@@ -388,7 +847,7 @@ int64_t chunks_of(int64_t l) { return l > kTokChunk ? ceil_div(l, kTokChunk) : 1
 unsigned grid_of(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
 bool logits_ok(const spice_logits *x) {
-    return x && x->n >= 0 && x->l >= 0 && x->c >= 1 && x->dtype >= 0 && x->dtype <= 2 &&
+    return x && x->n >= 0 && x->l >= 0 && x->c >= 1 && x->c <= 0x7fffffff - 65536 && x->dtype >= 0 && x->dtype <= 2 &&
            (x->data || x->n == 0 || x->l == 0) &&
            (x->n == 0 || x->l <= ((int64_t)1 << 40) / x->n);
 }
@@ -416,19 +875,107 @@ void grad_layout(TokArgs &a, void *grad, int32_t class_last) {
     a.g_sc = class_last ? 1 : a.x.l;
 }
 
-template <int MODE>
-int launch_positions(const TokArgs &a, int32_t dtype, hipStream_t stream) {
-    const int64_t total = a.x.n * a.x.l;
-    if (total == 0) return SPICE_OK;
-    const unsigned grid = grid_of(total);
-    if (dtype == 0)
-        tok_any_kernel<float, MODE><<<grid, kTokThreads, 0, stream>>>(a);
-    else if (dtype == 1)
-        tok_any_kernel<_Float16, MODE><<<grid, kTokThreads, 0, stream>>>(a);
-    else
-        tok_any_kernel<__bf16, MODE><<<grid, kTokThreads, 0, stream>>>(a);
+template <typename T, int LANES, int NV, int MODE>
+int launch_row(const TokArgs &a, hipStream_t stream) {
+    constexpr int block = LANES < kTokThreads ? kTokThreads : LANES;
+    tok_row_kernel<T, LANES, NV, MODE><<<grid_of(ceil_div(a.x.n * a.x.l, block / LANES)), block, 0, stream>>>(a);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
+}
+
+// How many lanes hold a row, by its 16-byte vectors: as few as keep at most 8 vectors a lane, then 16 and 20 with a
+// whole workgroup of 1024.
+template <typename T, int MODE>
+int launch_rows(const TokArgs &a, hipStream_t stream) {
+    const int64_t vecs = ceil_div(a.x.c, vec_elements<T>());
+    if (vecs <= 64 * 2) return launch_row<T, 64, 2, MODE>(a, stream);
+    if (vecs <= 64 * 8) return launch_row<T, 64, 8, MODE>(a, stream);
+    if (vecs <= 256 * 4) return launch_row<T, 256, 4, MODE>(a, stream);
+    if (vecs <= 256 * 8) return launch_row<T, 256, 8, MODE>(a, stream);
+    if (vecs <= 512 * 8) return launch_row<T, 512, 8, MODE>(a, stream);
+    if (vecs <= 1024 * 8) return launch_row<T, 1024, 8, MODE>(a, stream);
+    if (vecs <= 1024 * 16) return launch_row<T, 1024, 16, MODE>(a, stream);
+    if (vecs <= 1024 * 20) return launch_row<T, 1024, 20, MODE>(a, stream);
+    tok_long_row_kernel<T, MODE><<<grid_of(a.x.n * a.x.l), 1024, 0, stream>>>(a);
+    SPICE_LAUNCH_CHECK();
+    return SPICE_OK;
+}
+
+// Positions of one workgroup of the planes kernel.
+constexpr int kPlanesVec = 4;
+
+// Whether VEC neighbouring positions of every plane can move as one aligned word.
+template <typename T>
+bool planes_vec(const TokArgs &a) {
+    const int64_t bytes = kPlanesVec * (int64_t)sizeof(T);
+    const auto whole = [&](int64_t stride) { return stride * (int64_t)sizeof(T) % bytes == 0; };
+    return a.x.sl == 1 && a.x.l % kPlanesVec == 0 && whole(a.x.sc) && (a.x.n == 1 || whole(a.x.sn)) &&
+           reinterpret_cast<uintptr_t>(a.x.x) % bytes == 0 &&
+           (!a.grad || (reinterpret_cast<uintptr_t>(a.grad) % bytes == 0 && a.g_sl == 1));
+}
+
+int64_t planes_tiles(int64_t l, bool vec) { return ceil_div(l, (int64_t)kTokThreads * (vec ? kPlanesVec : 1)); }
+
+template <typename T, int VEC, int MODE>
+int launch_planes(const TokArgs &a, hipStream_t stream) {
+    const int64_t tiles = planes_tiles(a.x.l, VEC > 1);
+    const unsigned grid = grid_of(a.x.n * tiles);
+    if (MODE == kModeGrad || a.x.c > 32)
+        tok_planes_kernel<T, VEC, 0, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
+    else if (a.x.c <= 8)
+        tok_planes_kernel<T, VEC, 8, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
+    else if (a.x.c <= 24)
+        tok_planes_kernel<T, VEC, 24, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
+    else
+        tok_planes_kernel<T, VEC, 32, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
+    SPICE_LAUNCH_CHECK();
+    return SPICE_OK;
+}
+
+// Which kernel takes a call: rows where the classes are neighbours in memory and many, planes where the positions are, or
+// the classes few (a lane then walks a position's own classes, whose lines stay in its L1), any strides else.
+enum { kByRows, kByPlanes, kByAny };
+int route_of(const TokArgs &a) {
+    if (a.x.sc == 1 && a.x.c > 64) return !a.grad || a.g_sc == 1 ? kByRows : kByAny;   // (channels last: its gradient is in planes)
+    if (a.x.sl == 1 || (a.x.sc == 1 && a.x.c <= 64)) return kByPlanes;
+    return kByAny;
+}
+
+template <typename T, int MODE>
+int launch_typed(const TokArgs &a, hipStream_t stream) {
+    const int64_t total = a.x.n * a.x.l;
+    const int route = route_of(a);
+    if (route == kByPlanes)
+        return planes_vec<T>(a) ? launch_planes<T, kPlanesVec, MODE>(a, stream) : launch_planes<T, 1, MODE>(a, stream);
+    // rows and any strides: the sums over positions are a pass of their own over logp
+    constexpr int mode = MODE == kModePreference || MODE == kModePolicy ? kModeLogp : MODE;
+    if (route == kByRows) {
+        if constexpr (mode == kModeGrad) {
+            const int64_t pieces = ceil_div(a.x.c, (int64_t)kGradVecs * kTokThreads * vec_elements<T>());
+            tok_row_grad_kernel<T><<<grid_of(total * pieces), kTokThreads, 0, stream>>>(a, pieces);
+        } else {
+            return launch_rows<T, mode>(a, stream);
+        }
+    } else {
+        tok_any_kernel<T, mode><<<grid_of(total), kTokThreads, 0, stream>>>(a);
+    }
+    SPICE_LAUNCH_CHECK();
+    return SPICE_OK;
+}
+
+template <int MODE>
+int launch_positions(const TokArgs &a, int32_t dtype, hipStream_t stream) {
+    if (a.x.n * a.x.l == 0) return SPICE_OK;
+    return dtype == 0 ? launch_typed<float, MODE>(a, stream)
+           : dtype == 1 ? launch_typed<_Float16, MODE>(a, stream)
+                        : launch_typed<__bf16, MODE>(a, stream);
+}
+
+// Items a sequence's partial sums come in: the planes kernel's tiles, or the chunks of the pass over logp.
+int64_t items_of(const TokArgs &a, int32_t dtype) {
+    if (route_of(a) != kByPlanes) return chunks_of(a.x.l);
+    const bool vec = dtype == 0 ? planes_vec<float>(a) : dtype == 1 ? planes_vec<_Float16>(a) : planes_vec<__bf16>(a);
+    return a.x.l ? planes_tiles(a.x.l, vec) : 1;
 }
 
 SumArgs sums_of(const TokArgs &a, double *part) {
@@ -459,7 +1006,8 @@ using namespace spice;
 
 extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
     if (n < 0 || l < 0) return 0;
-    return (size_t)(n * chunks_of(l) * 4 * (int64_t)sizeof(double) + ((n + 1) / 2) * 8 + 64);
+    const int64_t items = l > kTokThreads ? ceil_div(l, kTokThreads) : 1;   // the smallest items: a workgroup of single positions
+    return (size_t)(n * items * 4 * (int64_t)sizeof(double) + ((n + 1) / 2) * 8 + 64);
 }
 
 extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, float temperature, float *logp, float *stats,
@@ -504,13 +1052,18 @@ extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *
     TokArgs a = args_of(x, y, p->temperature);
     a.logp = logp;
     a.stats = (float2 *)stats;
-    int rc = launch_positions<kModeLogp>(a, x->dtype, s);
+    a.ref = ref_logp;
+    a.part = (double *)workspace;
+    int rc = launch_positions<kModePreference>(a, x->dtype, s);
     if (rc) return rc;
-    SumArgs sums = sums_of(a, (double *)workspace);
-    sums.ref = ref_logp;
-    rc = launch_sums<kSumPreference>(sums, s);
-    if (rc) return rc;
-    PreferenceEnd e = {sums.part, x->n, sums.chunks, p->beta, p->smoothing, p->loss_type == SPICE_PREFERENCE_IPO, p->average != 0,
+    const int64_t items = items_of(a, x->dtype);
+    if (route_of(a) != kByPlanes || x->l == 0) {
+        SumArgs sums = sums_of(a, a.part);
+        sums.ref = ref_logp;
+        rc = launch_sums<kSumPreference>(sums, s);
+        if (rc) return rc;
+    }
+    PreferenceEnd e = {a.part, x->n, items, p->beta, p->smoothing, p->loss_type == SPICE_PREFERENCE_IPO, p->average != 0,
                        total, rewards, weight};
     tok_preference_kernel<<<1, kTokFold, 0, s>>>(e);
     SPICE_LAUNCH_CHECK();
@@ -535,23 +1088,23 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     a.host_scale = p->grad_scale;
     a.policy = Policy{old_logp, advantages, ref_logp, adv_n_stride, adv_l_stride, 1.f - p->clip_low, 1.f + p->clip_high,
                       p->kl_weight};
-    SumArgs sums = sums_of(a, (double *)workspace);
-    float *share = (float *)((double *)workspace + x->n * sums.chunks * 4);
+    if (grad) grad_layout(a, grad, class_last);
+    a.part = (double *)workspace;
+    SumArgs sums = sums_of(a, a.part);
+    const int64_t items = items_of(a, x->dtype);
+    float *share = (float *)(a.part + x->n * (items > sums.chunks ? items : sums.chunks) * 4);
     a.share = share;
     int rc = launch_sums<kSumCount>(sums, s);
     if (rc) return rc;
     tok_share_kernel<<<1, kTokFold, 0, s>>>(sums.part, x->n, sums.chunks, p->reduction == SPICE_POLICY_SEQUENCE, share);
     SPICE_LAUNCH_CHECK();
-    if (grad) {
-        grad_layout(a, grad, class_last);
-        rc = launch_positions<kModePolicyGrad>(a, x->dtype, s);
-    } else {
-        rc = launch_positions<kModePolicy>(a, x->dtype, s);
+    rc = grad ? launch_positions<kModePolicyGrad>(a, x->dtype, s) : launch_positions<kModePolicy>(a, x->dtype, s);
+    if (rc) return rc;
+    if (route_of(a) != kByPlanes || x->l == 0) {
+        rc = launch_sums<kSumPolicy>(sums, s);
+        if (rc) return rc;
     }
-    if (rc) return rc;
-    rc = launch_sums<kSumPolicy>(sums, s);
-    if (rc) return rc;
-    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(sums.part, x->n, sums.chunks, share, p->kl_weight, out4);
+    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(a.part, x->n, items, share, p->kl_weight, out4);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
 }

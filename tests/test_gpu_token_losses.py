@@ -117,7 +117,8 @@ def test_token_logprobs_and_gradient(dev, shape, t):
 
 @pytest.mark.parametrize("layout, positions, c", [("last", (6,), 5000), ("last", (40,), 9), ("planes", (8, 12), 21), ("planes", (5, 7), 70)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
-def test_excluded_classes_and_rubbish_in_ignored_positions(dev, layout, positions, c, dtype):
+@pytest.mark.parametrize("t", [1.0, 0.7, 1.44269502, 3.0])
+def test_excluded_classes_and_rubbish_in_ignored_positions(dev, layout, positions, c, dtype, t):
     """-inf and the type's lowest value as masks of classes, a row with nothing left, +inf, NaN; an ignored position may
     hold anything and gives zeros."""
     x, y, d, ignore = _inputs(layout, 2, positions, c, dtype, seed=5)
@@ -134,12 +135,12 @@ def test_excluded_classes_and_rubbish_in_ignored_positions(dev, layout, position
     rows[6, 0] = -math.inf                     # the label itself is excluded
     rows[7, :] = torch.finfo(dtype).min       # a plain row at the lowest value
     x = rows.reshape(2, *positions, c).movedim(-1, d).contiguous()
-    how = dict(class_dim=d, ignore_index=ignore)
+    how = dict(class_dim=d, ignore_index=ignore, temperature=t)
     v = x.double().requires_grad_(True)
     want, keep = ot.token_logprobs(v, y, **how)
     weight = torch.rand(y.shape, generator=torch.Generator().manual_seed(2)) + 0.5
     logp, stats = ops.token_logprobs(x.to(dev), y.to(dev), **how)
-    tol = _bounds(x, d, 1.0)[1] + 2 * U * want.detach().abs().nan_to_num(0.0, 0.0, 0.0)
+    tol = _bounds(x, d, t)[1] + 2 * U * want.detach().abs().nan_to_num(0.0, 0.0, 0.0)
     got, ref = logp.cpu().double().reshape(-1), want.detach().reshape(-1)
     assert torch.isnan(got[2]) and torch.isnan(ref[2]) and torch.isnan(got[3]) and got[6] == -math.inf
     assert got[4] == 0 and got[5] == 0
@@ -152,15 +153,15 @@ def test_excluded_classes_and_rubbish_in_ignored_positions(dev, layout, position
     assert (g[0, c // 2:] == 0).all() and (g[1, 4:] == 0).all()
     g64, = torch.autograd.grad((want * weight.double()).sum(), v)
     g64 = torch.where(torch.isfinite(g64), g64, torch.zeros((), dtype=g64.dtype))
-    t = _last(_grad_tol(x, g64, weight.double(), d, 1.0), d).reshape(-1, c)
+    gt = _last(_grad_tol(x, g64, weight.double(), d, t), d).reshape(-1, c)
     rest[6] = True                             # p of the label is 0 there: w (1 - 0) at the label, -w p elsewhere
-    p6 = torch.softmax(rows[6].double(), -1)
+    p6 = torch.softmax(rows[6].double() / t, -1) / t
     expect = _last(g64, d).reshape(-1, c).clone()
     expect[6] = -weight.reshape(-1)[6].double() * p6
-    expect[6, 0] += weight.reshape(-1)[6].double()
+    expect[6, 0] += weight.reshape(-1)[6].double() / t
     rest[3] = rest[2] = False
-    t[6] = t[6] + HALF_STEP[dtype] * expect[6].abs()
-    _close(g[rest], expect[rest], t[rest])
+    gt[6] = gt[6] + HALF_STEP[dtype] * expect[6].abs()
+    _close(g[rest], expect[rest], gt[rest])
 
 
 @pytest.mark.parametrize("layout, c", [("last", 3000), ("last", 6), ("planes", 21), ("planes", 100)])
