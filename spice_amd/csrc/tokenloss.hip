@@ -286,7 +286,7 @@ template <typename T>
 __device__ __forceinline__ u32x4 load_vec(const T *p, int32_t left) {
     constexpr int K = vec_elements<T>();
     if (left >= K) return reinterpret_cast<const Vec16 *>(p)->v;
-    float v[K];     // the row's last few classes, -inf behind them: they add nothing
+    float v[K];     // the row's last classes, or none of them, and -inf behind: they add nothing
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = k < left ? to_f32(p[k]) : -INFINITY;
     return pack<T, K>(v);
@@ -330,76 +330,95 @@ __device__ __forceinline__ void fold_row(float &m, float &s, Temper t, float *ld
     }
 }
 
+// The packed row is all that is kept from one phase to the next: unpacked values that the compiler would carry along
+// take twice the registers for 16-bit logits.
+template <int NV>
+__device__ __forceinline__ void forget(u32x4 (&raw)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
+}
+
+// Vector i of lane j holds the classes from (i LANES + j) K on: the first `whole` are full in every lane (the same count in
+// all of them), the one behind is ragged, filled up with -inf.
 template <typename T, int LANES, int NV, int MODE>
-__global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES) void tok_row_kernel(TokArgs a) {
+__global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 ? 6 : 4) void tok_row_kernel(TokArgs a, int64_t first) {
     constexpr int K = vec_elements<T>();
     constexpr int kBlock = LANES < kTokThreads ? kTokThreads : LANES;
     constexpr bool kGrad = MODE == kModePolicyGrad;
     __shared__ float lds[2 * kBlock / kWave];
-    const int64_t total = a.x.n * a.x.l;
-    const int32_t lane = threadIdx.x % LANES, classes = (int32_t)a.x.c;
-    for (int64_t at = (int64_t)blockIdx.x * (kBlock / LANES) + __builtin_amdgcn_readfirstlane(threadIdx.x / LANES); at < total;
-         at += (int64_t)gridDim.x * (kBlock / LANES)) {
-        const int64_t n = at / a.x.l, l = at - n * a.x.l;
-        const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
-        const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
-        const int kind = label_kind(y, a.y.ignore, a.x.c);
-        float m = -INFINITY, s = 0.f, logp = kind == kBad ? NAN : 0.f;
-        u32x4 raw[NV];
+    const int64_t at = first + (int64_t)blockIdx.x * (kBlock / LANES) + __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    if (at >= a.x.n * a.x.l) return;
+    const int32_t lane = threadIdx.x % LANES, classes = (int32_t)a.x.c, whole = classes / (LANES * K);
+    const int32_t tail = (whole * LANES + lane) * K, left = classes - tail;
+    const int64_t n = at / a.x.l, l = at - n * a.x.l;
+    const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
+    const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
+    const int kind = label_kind(y, a.y.ignore, a.x.c);
+    float m = -INFINITY, s = 0.f, logp = kind == kBad ? NAN : 0.f;
+    u32x4 raw[NV], last;
+    if (kind == kCounted) {
+        const T *mine = x + lane * K;
+        const float xl = to_f32(x[y]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < whole) raw[i] = reinterpret_cast<const Vec16 *>(mine + i * LANES * K)->v;
+        last = load_vec<T>(x + tail, left);
+        float v[K];
+        unpack(last, v, T());
+#pragma unroll
+        for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < whole) {
+                unpack(raw[i], v, T());
+#pragma unroll
+                for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]);
+            }
+        const float shift = shift_of(m);
+        forget<NV>(raw);
+        unpack(last, v, T());
+#pragma unroll
+        for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < whole) {
+                unpack(raw[i], v, T());
+#pragma unroll
+                for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+            }
+        fold_row<LANES>(m, s, a.t, lds);
+        logp = (xl - shift_of(m)) * a.t.inv - log_of(s);
+    }
+    if (lane == 0) {
+        a.logp[at] = logp;
+        if (a.stats) a.stats[at] = make_float2(m, s);
+    }
+    if (kGrad) {
+        T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
+        float w = kind == kBad ? NAN : 0.f;
+        if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+        if (a.weight_out && lane == 0) a.weight_out[at] = w;
+        const float shift = shift_of(m);
+        w *= a.t.inv * a.host_scale;
+        const float each = kind == kCounted ? -w / s : w;
+        float v[K];
         if (kind == kCounted) {
-            const float xl = to_f32(x[y]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int32_t c0 = (i * LANES + lane) * K;
-                if (c0 < classes) raw[i] = load_vec<T>(x + c0, classes - c0);
-            }
+            T *mine = g + lane * K;
+            forget<NV>(raw);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if ((i * LANES + lane) * K < classes) {
-                    float v[K];
+                if (i < whole) {
                     unpack(raw[i], v, T());
-#pragma unroll
-                    for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]);
+                    grad_of<K>(v, shift, each, w, (int32_t)y, (i * LANES + lane) * K, a.t);
+                    reinterpret_cast<Vec16 *>(mine + i * LANES * K)->v = pack<T, K>(v);
                 }
-            const float shift = shift_of(m);
+            unpack(last, v, T());
+            grad_of<K>(v, shift, each, w, (int32_t)y, tail, a.t);
+            if (left > 0) store_vec<T, K>(g + tail, left, v);
+        } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if ((i * LANES + lane) * K < classes) {
-                    float v[K];
-                    unpack(raw[i], v, T());
-#pragma unroll
-                    for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
-                }
-            fold_row<LANES>(m, s, a.t, lds);
-            logp = (xl - shift_of(m)) * a.t.inv - log_of(s);
-        }
-        if (lane == 0) {
-            a.logp[at] = logp;
-            if (a.stats) a.stats[at] = make_float2(m, s);
-        }
-        if (kGrad) {
-            T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
-            float w = kind == kBad ? NAN : 0.f;
-            if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
-            if (a.weight_out && lane == 0) a.weight_out[at] = w;
-            const float shift = shift_of(m);
-            w *= a.t.inv * a.host_scale;
-            const float each = kind == kCounted ? -w / s : w;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int32_t c0 = (i * LANES + lane) * K;
-                if (c0 < classes) {
-                    float v[K];
-                    if (kind == kCounted) {
-                        unpack(raw[i], v, T());
-                        grad_of<K>(v, shift, each, w, (int32_t)y, c0, a.t);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < K; ++k) v[k] = each;
-                    }
-                    store_vec<T, K>(g + c0, classes - c0, v);
-                }
-            }
+            for (int k = 0; k < K; ++k) v[k] = each;
+            for (int32_t c0 = lane * K; c0 < classes; c0 += LANES * K) store_vec<T, K>(g + c0, classes - c0, v);
         }
     }
 }
@@ -877,17 +896,21 @@ void grad_layout(TokArgs &a, void *grad, int32_t class_last) {
 
 template <typename T, int LANES, int NV, int MODE>
 int launch_row(const TokArgs &a, hipStream_t stream) {
-    constexpr int block = LANES < kTokThreads ? kTokThreads : LANES;
-    tok_row_kernel<T, LANES, NV, MODE><<<grid_of(ceil_div(a.x.n * a.x.l, block / LANES)), block, 0, stream>>>(a);
-    SPICE_LAUNCH_CHECK();
+    constexpr int block = LANES < kTokThreads ? kTokThreads : LANES, rows = block / LANES;
+    constexpr int64_t most = (int64_t)1 << 30;
+    for (int64_t first = 0; first < a.x.n * a.x.l; first += most) {
+        const int64_t left = a.x.n * a.x.l - first;
+        tok_row_kernel<T, LANES, NV, MODE><<<(unsigned)ceil_div(left < most ? left : most, rows), block, 0, stream>>>(a, first);
+        SPICE_LAUNCH_CHECK();
+    }
     return SPICE_OK;
 }
 
-// How many lanes hold a row, by its 16-byte vectors: as few as keep at most 8 vectors a lane, then 16 and 20 with a
-// whole workgroup of 1024.
+// How many lanes hold a row, by its full 16-byte vectors: as few as keep at most 8 a lane, then 16 and 20 with a whole
+// workgroup of 1024.
 template <typename T, int MODE>
 int launch_rows(const TokArgs &a, hipStream_t stream) {
-    const int64_t vecs = ceil_div(a.x.c, vec_elements<T>());
+    const int64_t vecs = a.x.c / vec_elements<T>() + 1;    // (less than NV + 1 for all lanes together: the ragged one is extra)
     if (vecs <= 64 * 2) return launch_row<T, 64, 2, MODE>(a, stream);
     if (vecs <= 64 * 8) return launch_row<T, 64, 8, MODE>(a, stream);
     if (vecs <= 256 * 4) return launch_row<T, 256, 4, MODE>(a, stream);
