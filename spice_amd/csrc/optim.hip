@@ -91,13 +91,32 @@ __global__ __launch_bounds__(kOptThreads) void grad_norm_kernel(TableOf<1> t, do
     uint32_t done = 0;
     if (on16(g)) {
         constexpr int K = 16 / sizeof(T);
+        typedef Vec<T, K> VecTK;
         const Vec<T, K> *gv = (const Vec<T, K> *)g;
         const uint32_t nv = n / K;
-        for (uint32_t i = threadIdx.x; i < nv; i += kOptThreads) {
+        // eight loads in flight a lane; two chains of sums
+        double two = 0.0;
+        uint32_t i = threadIdx.x;
+        for (; i + 7 * kOptThreads < nv; i += 8 * kOptThreads) {
+            u32x4_t x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_nontemporal_load((const u32x4_t *)(gv + i + j * kOptThreads));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Vec<T, K> v = __builtin_bit_cast(VecTK, x[j]);
+#pragma unroll
+                for (int k = 0; k < K; k += 2) {
+                    acc = norm_take<T, INF>(acc, v.v[k]);
+                    two = norm_take<T, INF>(two, v.v[k + 1]);
+                }
+            }
+        }
+        for (; i < nv; i += kOptThreads) {
             const Vec<T, K> x = gv[i];
 #pragma unroll
             for (int k = 0; k < K; ++k) acc = norm_take<T, INF>(acc, x.v[k]);
         }
+        acc = norm_join<INF>(acc, two);
         done = nv * K;
     }
     for (uint32_t i = done + threadIdx.x; i < n; i += kOptThreads) acc = norm_take<T, INF>(acc, g[i]);

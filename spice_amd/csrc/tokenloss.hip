@@ -14,8 +14,9 @@ namespace spice {
 namespace {
 
 constexpr int kTokThreads = 256;
-constexpr int kTokChunk = 4096;      // positions of one workgroup of the passes over positions
+constexpr int kTokChunk = 2048;      // positions of one workgroup of the passes over positions
 constexpr int kTokFold = 1024;       // threads of the one workgroup that folds their partial sums
+constexpr int64_t kTokHere = 16384;  // positions that this workgroup sums itself: 16 a thread
 
 // The logits as the kernels see them: element strides of sequence, position and class.
 struct Logits {
@@ -546,177 +547,222 @@ __global__ __launch_bounds__(kTokThreads) void tok_row_grad_kernel(TokArgs a, in
 
 // ---- positions next to each other in memory: a lane takes VEC of them, walking the class planes ----
 
-// Planes of one position group in registers: CREG classes at most, so the logits are read once for maximum, sum and
-// gradient; CREG = 0: any number, eight planes at a time, read again for the gradient.
-template <typename T, int VEC>
-struct __attribute__((aligned(sizeof(T) * VEC))) Group { T v[VEC]; };
+// A position group's logits of one class as they lie in memory, and their values.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+template <typename T, int VEC> struct GroupOf;
+template <> struct GroupOf<float, 4> { typedef u32x4 type; };
+template <> struct GroupOf<_Float16, 4> { typedef u32x2 type; };
+template <> struct GroupOf<__bf16, 4> { typedef u32x2 type; };
+template <typename T> struct GroupOf<T, 1> { typedef T type; };
 
+template <typename T, int VEC>
+__device__ __forceinline__ void values(const typename GroupOf<T, VEC>::type &r, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = to_f32(r);
+    } else if constexpr (sizeof(T) == 4) {
+        unpack(r, v, T());
+    } else {
+        float w[8];
+        const u32x4 wide = {r[0], r[1], 0u, 0u};
+        unpack(wide, w, T());
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = w[k];
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ typename GroupOf<T, VEC>::type grouped(const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        return (T)v[0];
+    } else if constexpr (sizeof(T) == 4) {
+        return pack<T, VEC>(v);
+    } else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        const t4 t = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        return __builtin_bit_cast(u32x2, t);
+    }
+}
+
+// As in the row kernel: packed logits from phase to phase.
+template <typename G, int N>
+__device__ __forceinline__ void forget_groups(G (&raw)[N]) {
+    if constexpr (sizeof(G) >= 8) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(raw[i]));
+    }
+}
+
+// CREG > 0: at most CREG classes, a position group's logits in registers, read once for maximum, sum and gradient;
+// CREG = 0: any number, eight planes at a time, read again for the gradient.
 template <typename T, int VEC, int CREG, int MODE>
-__global__ __launch_bounds__(kTokThreads) void tok_planes_kernel(TokArgs a, int64_t tiles) {
+__global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24 ? 3 : 2) void tok_planes_kernel(TokArgs a, int64_t tiles, int64_t first) {
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
     constexpr bool kStats = MODE == kModeGrad;          // (max, sum) given
     constexpr int K = MODE == kModePreference ? 2 : 4;  // sums of a workgroup
     constexpr bool kSums = MODE == kModePreference || MODE == kModePolicy || MODE == kModePolicyGrad;
     constexpr int kStep = 8;
+    typedef typename GroupOf<T, VEC>::type G;
     __shared__ double lds[kSums ? K * kTokThreads / kWave : 1];
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int32_t classes = (int32_t)a.x.c;
-    const float out_scale = kGrad ? a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f) : 0.f;
-    for (int64_t item = blockIdx.x; item < a.x.n * tiles; item += gridDim.x) {
-        const int64_t n = item / tiles, l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
-        double sums[K];
+    const int64_t item = first + blockIdx.x, n = item / tiles;
+    const int64_t l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
+    double sums[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) sums[k] = 0.0;
-        if (l0 < a.x.l) {
-            const T *x = (const T *)a.x.x + n * a.x.sn + l0 * a.x.sl;
-            T *g = kGrad ? (T *)a.grad + n * a.g_sn + l0 * a.g_sl : nullptr;
-            const int64_t at = n * a.x.l + l0;
-            int32_t y[VEC];         // the label, or -1
-            int kind[VEC];
-            bool any = false;
+    for (int k = 0; k < K; ++k) sums[k] = 0.0;
+    if (l0 < a.x.l) {
+        const T *x = (const T *)a.x.x + n * a.x.sn + l0 * a.x.sl;
+        const int64_t at = n * a.x.l + l0;
+        const auto plane = [&](int32_t c) { return *reinterpret_cast<const G *>(x + (int64_t)c * a.x.sc); };
+        int32_t y[VEC];         // the label, or -1
+        int kind[VEC];
+        bool any = false;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const int64_t label = a.y.y[n * a.y.sn + (l0 + k) * a.y.sl];
-                kind[k] = label_kind(label, a.y.ignore, a.x.c);
-                y[k] = kind[k] == kCounted ? (int32_t)label : -1;
-                any |= kind[k] == kCounted;
-            }
-            float m[VEC], s[VEC], xl[VEC], w[VEC];
-            Group<T, VEC> raw[CREG > 0 ? CREG : 1];
+        for (int k = 0; k < VEC; ++k) {
+            const int64_t label = a.y.y[n * a.y.sn + (l0 + k) * a.y.sl];
+            kind[k] = label_kind(label, a.y.ignore, a.x.c);
+            y[k] = kind[k] == kCounted ? (int32_t)label : -1;
+            any |= kind[k] == kCounted;
+        }
+        float m[VEC], s[VEC], xl[VEC], w[VEC], v[VEC];
+        G raw[CREG > 0 ? CREG : kStep];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                m[k] = -INFINITY;
-                s[k] = xl[k] = w[k] = 0.f;
-            }
-            if (any && kStats) {
+        for (int k = 0; k < VEC; ++k) {
+            m[k] = -INFINITY;
+            s[k] = xl[k] = w[k] = 0.f;
+        }
+        if (any && kStats) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    if (kind[k] == kCounted) {
-                        const float2 st = a.stats_in[at + k];
-                        m[k] = st.x;
-                        s[k] = st.y;
-                    }
-            }
-            if (any && CREG > 0) {
+            for (int k = 0; k < VEC; ++k)
+                if (kind[k] == kCounted) {
+                    const float2 st = a.stats_in[at + k];
+                    m[k] = st.x;
+                    s[k] = st.y;
+                }
+        }
+        if (any && CREG > 0) {
+#pragma unroll
+            for (int c = 0; c < CREG; ++c)
+                if (c < classes) raw[c] = plane(c);
+            if (!kStats) {
 #pragma unroll
                 for (int c = 0; c < CREG; ++c)
-                    if (c < classes) raw[c] = *(const Group<T, VEC> *)(x + c * a.x.sc);
-                if (!kStats) {
+                    if (c < classes) {
+                        values<T, VEC>(raw[c], v);
 #pragma unroll
-                    for (int c = 0; c < CREG; ++c)
-                        if (c < classes) {
-#pragma unroll
-                            for (int k = 0; k < VEC; ++k) {
-                                const float v = to_f32(raw[c].v[k]);
-                                m[k] = fmaxf(m[k], v);
-                                xl[k] = y[k] == c ? v : xl[k];
-                            }
+                        for (int k = 0; k < VEC; ++k) {
+                            m[k] = fmaxf(m[k], v[k]);
+                            xl[k] = y[k] == c ? v[k] : xl[k];
                         }
-#pragma unroll
-                    for (int c = 0; c < CREG; ++c)
-                        if (c < classes) {
-#pragma unroll
-                            for (int k = 0; k < VEC; ++k) s[k] += exp_of(to_f32(raw[c].v[k]) - shift_of(m[k]), a.t);
-                        }
-                }
-            } else if (any && !kStats) {
-                for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
-                    Group<T, VEC> part[kStep];
-                    float top[VEC];
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) top[k] = m[k];
-#pragma unroll
-                    for (int j = 0; j < kStep; ++j)
-                        if (c0 + j < classes) part[j] = *(const Group<T, VEC> *)(x + (int64_t)(c0 + j) * a.x.sc);
-#pragma unroll
-                    for (int j = 0; j < kStep; ++j)
-                        if (c0 + j < classes) {
-#pragma unroll
-                            for (int k = 0; k < VEC; ++k) {
-                                const float v = to_f32(part[j].v[k]);
-                                top[k] = fmaxf(top[k], v);
-                                xl[k] = y[k] == c0 + j ? v : xl[k];
-                            }
-                        }
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        s[k] *= rescale(m[k], top[k], a.t);
-                        m[k] = top[k];
                     }
+                forget_groups(raw);
 #pragma unroll
-                    for (int j = 0; j < kStep; ++j)
-                        if (c0 + j < classes) {
+                for (int c = 0; c < CREG; ++c)
+                    if (c < classes) {
+                        values<T, VEC>(raw[c], v);
 #pragma unroll
-                            for (int k = 0; k < VEC; ++k) s[k] += exp_of(to_f32(part[j].v[k]) - shift_of(m[k]), a.t);
-                        }
-                }
+                        for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
+                    }
             }
-            float each[VEC];     // factor of a class's exponential in the gradient, and what else its value gets
+        } else if (any && !kStats) {
+            for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
+                float top[VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const int64_t l = l0 + k;
-                each[k] = 0.f;
-                if (!kStats) {
-                    const float logp = kind[k] == kCounted ? (xl[k] - shift_of(m[k])) * a.t.inv - log_of(s[k])
-                                       : kind[k] == kBad   ? NAN : 0.f;
-                    a.logp[at + k] = logp;
-                    if (a.stats) a.stats[at + k] = make_float2(m[k], s[k]);
-                    if (MODE == kModePreference && kind[k] != kIgnored) {
-                        sums[0] += (double)logp - (double)a.ref[at + k];
-                        sums[1] += 1.0;
+                for (int k = 0; k < VEC; ++k) top[k] = m[k];
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+                    if (c0 + j < classes) raw[j] = plane(c0 + j);
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+                    if (c0 + j < classes) {
+                        values<T, VEC>(raw[j], v);
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) {
+                            top[k] = fmaxf(top[k], v[k]);
+                            xl[k] = y[k] == c0 + j ? v[k] : xl[k];
+                        }
                     }
-                    if ((MODE == kModePolicy || MODE == kModePolicyGrad) && kind[k] != kIgnored) {
-                        const PolicyTerm t = policy_term(a.policy, logp, at + k, n, l);
-                        sums[0] += t.surrogate;
-                        sums[1] += t.far;
-                        sums[2 % K] += t.over ? 1.0 : 0.0;
-                        sums[3 % K] += 1.0;
-                        w[k] = kind[k] == kBad ? NAN : t.dlogp * (MODE == kModePolicyGrad ? a.share[n] : 0.f);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    s[k] *= rescale(m[k], top[k], a.t);
+                    m[k] = top[k];
+                }
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+                    if (c0 + j < classes) {
+                        values<T, VEC>(raw[j], v);
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
                     }
-                    if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at + k] = w[k];
-                } else if (kind[k] == kCounted) {
-                    w[k] = a.weight[n * a.w_sn + l * a.w_sl];
-                } else {
-                    w[k] = kind[k] == kBad ? NAN : 0.f;
+            }
+        }
+        float each[VEC];     // factor of a class's exponential in the gradient; where nothing is counted the value itself
+        const float out_scale = kGrad ? a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f) : 0.f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const int64_t l = l0 + k;
+            each[k] = 0.f;
+            if (!kStats) {
+                const float logp = kind[k] == kCounted ? (xl[k] - shift_of(m[k])) * a.t.inv - log_of(s[k])
+                                   : kind[k] == kBad   ? NAN : 0.f;
+                a.logp[at + k] = logp;
+                if (a.stats) a.stats[at + k] = make_float2(m[k], s[k]);
+                if (MODE == kModePreference && kind[k] != kIgnored) {
+                    sums[0] += (double)logp - (double)a.ref[at + k];
+                    sums[1] += 1.0;
                 }
-                if (kGrad) {
-                    w[k] *= out_scale;
-                    each[k] = kind[k] == kCounted ? -w[k] / s[k] : w[k];
+                if ((MODE == kModePolicy || MODE == kModePolicyGrad) && kind[k] != kIgnored) {
+                    const PolicyTerm t = policy_term(a.policy, logp, at + k, n, l);
+                    sums[0] += t.surrogate;
+                    sums[1] += t.far;
+                    sums[2 % K] += t.over ? 1.0 : 0.0;
+                    sums[3 % K] += 1.0;
+                    w[k] = kind[k] == kBad ? NAN : t.dlogp * (MODE == kModePolicyGrad ? a.share[n] : 0.f);
                 }
+                if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at + k] = w[k];
+            } else if (kind[k] == kCounted) {
+                w[k] = a.weight[n * a.w_sn + l * a.w_sl];
+            } else {
+                w[k] = kind[k] == kBad ? NAN : 0.f;
             }
             if (kGrad) {
-                const auto store = [&](const Group<T, VEC> &from, int32_t c) {
-                    Group<T, VEC> to;
+                w[k] *= out_scale;
+                each[k] = kind[k] == kCounted ? -w[k] / s[k] : w[k];
+            }
+        }
+        if (kGrad) {
+            T *g = (T *)a.grad + n * a.g_sn + l0 * a.g_sl;
+            const auto store = [&](const G &from, int32_t c) {
+                values<T, VEC>(from, v);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        const float e = each[k] * exp_of(to_f32(from.v[k]) - shift_of(m[k]), a.t);
-                        to.v[k] = (T)(kind[k] == kCounted ? (y[k] == c ? e + w[k] : e) : each[k]);
-                    }
-                    *(Group<T, VEC> *)(g + (int64_t)c * a.g_sc) = to;
-                };
-                if (CREG > 0) {
+                for (int k = 0; k < VEC; ++k) {
+                    const float e = each[k] * exp_of(v[k] - shift_of(m[k]), a.t);
+                    v[k] = kind[k] == kCounted ? (y[k] == c ? e + w[k] : e) : each[k];
+                }
+                *reinterpret_cast<G *>(g + (int64_t)c * a.g_sc) = grouped<T, VEC>(v);
+            };
+            if (CREG > 0) {
+                forget_groups(raw);
 #pragma unroll
-                    for (int c = 0; c < CREG; ++c)
-                        if (c < classes) store(raw[c], c);
-                } else {
-                    for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
-                        Group<T, VEC> part[kStep];
+                for (int c = 0; c < CREG; ++c)
+                    if (c < classes) store(raw[c], c);
+            } else {
+                for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
 #pragma unroll
-                        for (int j = 0; j < kStep; ++j)
-                            if (any && c0 + j < classes) part[j] = *(const Group<T, VEC> *)(x + (int64_t)(c0 + j) * a.x.sc);
+                    for (int j = 0; j < kStep; ++j)
+                        if (any && c0 + j < classes) raw[j] = plane(c0 + j);
 #pragma unroll
-                        for (int j = 0; j < kStep; ++j)
-                            if (c0 + j < classes) store(part[j], c0 + j);
-                    }
+                    for (int j = 0; j < kStep; ++j)
+                        if (c0 + j < classes) store(raw[j], c0 + j);
                 }
             }
         }
-        if (kSums) {
-            block_sums<K>(sums, lds, kTokThreads);
-            if (threadIdx.x == 0)
+    }
+    if (kSums) {
+        block_sums<K>(sums, lds, kTokThreads);
+        if (threadIdx.x == 0)
 #pragma unroll
-                for (int k = 0; k < K; ++k) a.part[item * K + k] = sums[k];
-        }
+            for (int k = 0; k < K; ++k) a.part[item * K + k] = sums[k];
     }
 }
 
@@ -738,6 +784,21 @@ template <int WHAT>
 constexpr int sum_terms() { return WHAT == kSumCount ? 1 : WHAT == kSumPreference ? 2 : 4; }
 
 template <int WHAT>
+__device__ __forceinline__ void sum_position(const SumArgs &a, int64_t n, int64_t l, double (&v)[sum_terms<WHAT>()]) {
+    constexpr int K = sum_terms<WHAT>();
+    const int64_t at = n * a.l + l;
+    if (a.y.y[n * a.y.sn + l * a.y.sl] == a.y.ignore) return;
+    v[K - 1] += 1.0;
+    if (WHAT == kSumPreference) v[0] += (double)a.logp[at] - (double)a.ref[at];
+    if (WHAT == kSumPolicy) {
+        const PolicyTerm t = policy_term(a.policy, a.logp[at], at, n, l);
+        v[0] += t.surrogate;
+        v[1 % K] += t.far;
+        v[2 % K] += t.over ? 1.0 : 0.0;
+    }
+}
+
+template <int WHAT>
 __global__ __launch_bounds__(kTokThreads) void tok_sum_kernel(SumArgs a) {
     constexpr int K = sum_terms<WHAT>();
     __shared__ double lds[K * kTokThreads / kWave];
@@ -747,18 +808,8 @@ __global__ __launch_bounds__(kTokThreads) void tok_sum_kernel(SumArgs a) {
         double v[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] = 0.0;
-        for (int64_t l = chunk * (int64_t)kTokChunk + threadIdx.x; l < end; l += kTokThreads) {
-            const int64_t at = n * a.l + l;
-            if (a.y.y[n * a.y.sn + l * a.y.sl] == a.y.ignore) continue;
-            v[K - 1] += 1.0;
-            if (WHAT == kSumPreference) v[0] += (double)a.logp[at] - (double)a.ref[at];
-            if (WHAT == kSumPolicy) {
-                const PolicyTerm t = policy_term(a.policy, a.logp[at], at, n, l);
-                v[0] += t.surrogate;
-                v[1 % K] += t.far;
-                v[2 % K] += t.over ? 1.0 : 0.0;
-            }
-        }
+#pragma unroll 8
+        for (int64_t l = chunk * (int64_t)kTokChunk + threadIdx.x; l < end; l += kTokThreads) sum_position<WHAT>(a, n, l, v);
         block_sums<K>(v, lds, kTokThreads);
         if (threadIdx.x == 0)
 #pragma unroll
@@ -766,47 +817,67 @@ __global__ __launch_bounds__(kTokThreads) void tok_sum_kernel(SumArgs a) {
     }
 }
 
+// The sums of every sequence by one workgroup of kTokFold threads, for calls of few positions: part[n, ways, K], a wave each.
+template <int WHAT>
+__device__ __forceinline__ void sums_here(const SumArgs &a, int64_t ways) {
+    constexpr int K = sum_terms<WHAT>();
+    for (int64_t item = threadIdx.x / kWave; item < a.n * ways; item += kTokFold / kWave) {
+        const int64_t n = item / ways, way = item - n * ways;
+        double v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = 0.0;
+#pragma unroll 2
+        for (int64_t l = way * kWave + (threadIdx.x & 63); l < a.l; l += ways * kWave) sum_position<WHAT>(a, n, l, v);
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) a.part[item * K + k] = v[k];
+    }
+    __threadfence_block();
+    __syncthreads();
+}
+
+// Each sequence's partial sums, folded by the lanes of a wave and handed to `take(n, sums)` in its first lane.
+template <int K, typename F>
+__device__ __forceinline__ void fold_sequences(const double *part, int64_t n, int64_t chunks, F take) {
+    for (int64_t i = threadIdx.x / kWave; i < n; i += kTokFold / kWave) {
+        double v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = 0.0;
+        for (int64_t c = threadIdx.x & 63; c < chunks; c += kWave)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += part[(i * chunks + c) * K + k];
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+        if ((threadIdx.x & 63) == 0) take(i, v);
+    }
+}
+
 // share[n]: what one position of sequence n counts in the mean over all counted positions (token), or in the mean over
-// sequences of each one's mean.
-__global__ __launch_bounds__(kTokFold) void tok_share_kernel(const double *part, int64_t n, int64_t chunks, int per_sequence,
-                                                             float *share) {
+// sequences of each one's mean.  `ways` > 0: the positions are counted here.
+__global__ __launch_bounds__(kTokFold) void tok_share_kernel(SumArgs a, int64_t ways, int per_sequence, float *share) {
     __shared__ double lds[kTokFold / kWave];
-    double all = 0.0;
-    if (!per_sequence) {
-        double v[1] = {0.0};
-        for (int64_t i = threadIdx.x; i < n * chunks; i += kTokFold) v[0] += part[i];
-        block_sums<1>(v, lds, kTokFold);
-        all = v[0];
+    if (ways) sums_here<kSumCount>(a, ways);
+    const int64_t chunks = ways ? ways : a.chunks;
+    if (per_sequence) {
+        fold_sequences<1>(a.part, a.n, chunks, [&](int64_t i, const double (&v)[1]) {
+            share[i] = (float)(1.0 / (fmax(v[0], 1.0) * (double)a.n));
+        });
+        return;
     }
-    for (int64_t i = threadIdx.x; i < n; i += kTokFold) {
-        double count = all, weight = 1.0;
-        if (per_sequence) {
-            count = 0.0;
-            weight = (double)n;
-            for (int64_t k = 0; k < chunks; ++k) count += part[i * chunks + k];
-        }
-        share[i] = (float)(1.0 / (fmax(count, 1.0) * weight));
-    }
+    double v[1] = {0.0};
+    for (int64_t i = threadIdx.x; i < a.n * chunks; i += kTokFold) v[0] += a.part[i];
+    block_sums<1>(v, lds, kTokFold);
+    for (int64_t i = threadIdx.x; i < a.n; i += kTokFold) share[i] = (float)(1.0 / fmax(v[0], 1.0));
 }
 
 struct PreferenceEnd {
-    const double *part;     // [n, chunks, 2]
-    int64_t n, chunks;
     float beta, smoothing;
     int ipo, average;
     float *total, *rewards, *weight;   // [1], [n], [n]: d total / d logp of every counted position of sequence n
+    double *ratio;                     // [n, 2] scratch: a sequence's log ratio, and what its positions count
 };
-
-__device__ __forceinline__ double sequence_total(const PreferenceEnd &e, int64_t i, double &count) {
-    double sum = 0.0;
-    count = 0.0;
-    for (int64_t k = 0; k < e.chunks; ++k) {
-        sum += e.part[(i * e.chunks + k) * 2];
-        count += e.part[(i * e.chunks + k) * 2 + 1];
-    }
-    count = e.average ? fmax(count, 1.0) : 1.0;
-    return sum / count;
-}
 
 // softplus(-x) = -log sigmoid(x), and sigmoid, without overflow on either side.
 __device__ __forceinline__ double minus_log_sigmoid(double x) { return log1p(exp(-fabs(x))) + fmax(-x, 0.0); }
@@ -815,13 +886,20 @@ __device__ __forceinline__ double sigmoid(double x) {
     return x >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
 }
 
-__global__ __launch_bounds__(kTokFold) void tok_preference_kernel(PreferenceEnd e) {
+__global__ __launch_bounds__(kTokFold) void tok_preference_kernel(SumArgs a, int64_t ways, PreferenceEnd e) {
     __shared__ double lds[kTokFold / kWave];
-    const int64_t half = e.n / 2;
+    if (ways) sums_here<kSumPreference>(a, ways);
+    fold_sequences<2>(a.part, a.n, ways ? ways : a.chunks, [&](int64_t i, const double (&v)[2]) {
+        const double count = e.average ? fmax(v[1], 1.0) : 1.0;
+        e.ratio[2 * i] = v[0] / count;
+        e.ratio[2 * i + 1] = count;
+    });
+    __threadfence_block();
+    __syncthreads();
+    const int64_t half = a.n / 2;
     double v[1] = {0.0};
     for (int64_t i = threadIdx.x; i < half; i += kTokFold) {
-        double na, nb;
-        const double sa = sequence_total(e, i, na), sb = sequence_total(e, half + i, nb);
+        const double sa = e.ratio[2 * i], sb = e.ratio[2 * (half + i)];
         const double h = sa - sb, b = (double)e.beta, eps = (double)e.smoothing;
         double dh;
         if (e.ipo) {
@@ -834,24 +912,25 @@ __global__ __launch_bounds__(kTokFold) void tok_preference_kernel(PreferenceEnd 
         }
         e.rewards[i] = (float)(b * sa);
         e.rewards[half + i] = (float)(b * sb);
-        e.weight[i] = (float)(dh / (double)half / na);
-        e.weight[half + i] = (float)(-dh / (double)half / nb);
+        e.weight[i] = (float)(dh / (double)half / e.ratio[2 * i + 1]);
+        e.weight[half + i] = (float)(-dh / (double)half / e.ratio[2 * (half + i) + 1]);
     }
     block_sums<1>(v, lds, kTokFold);
     if (threadIdx.x == 0) *e.total = (float)(v[0] / (double)half);
 }
 
 // out4 = {total, surrogate, kl, share of the counted positions where the clipping holds}
-__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(const double *part, int64_t n, int64_t chunks, const float *share,
-                                                                  float kl, float *out4) {
+__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, const float *share, float kl, float *out4) {
     __shared__ double lds[4 * kTokFold / kWave];
+    if (ways) sums_here<kSumPolicy>(a, ways);
+    const int64_t chunks = ways ? ways : a.chunks;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t i = threadIdx.x; i < n * chunks; i += kTokFold) {
+    for (int64_t i = threadIdx.x; i < a.n * chunks; i += kTokFold) {
         const double each = (double)share[i / chunks];
-        v[0] += part[i * 4] * each;
-        v[1] += part[i * 4 + 1] * each;
-        v[2] += part[i * 4 + 2];
-        v[3] += part[i * 4 + 3];
+        v[0] += a.part[i * 4] * each;
+        v[1] += a.part[i * 4 + 1] * each;
+        v[2] += a.part[i * 4 + 2];
+        v[3] += a.part[i * 4 + 3];
     }
     block_sums<4>(v, lds, kTokFold);
     if (threadIdx.x == 0) {
@@ -860,6 +939,13 @@ __global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(const double *
         out4[2] = (float)v[1];
         out4[3] = (float)(v[2] / fmax(v[3], 1.0));
     }
+}
+
+// How many waves of the folding workgroup share a sequence where it takes the sums itself; 0: they are too many for it.
+int64_t ways_of(int64_t n, int64_t l) {
+    if (n == 0 || l > kTokHere / n) return 0;
+    const int64_t ways = kTokFold / kWave / n, most = ceil_div(l, kWave);
+    return ways < 1 ? 1 : ways > most ? (most ? most : 1) : ways;
 }
 
 int64_t chunks_of(int64_t l) { return l > kTokChunk ? ceil_div(l, kTokChunk) : 1; }
@@ -910,15 +996,15 @@ int launch_row(const TokArgs &a, hipStream_t stream) {
 // workgroup of 1024.
 template <typename T, int MODE>
 int launch_rows(const TokArgs &a, hipStream_t stream) {
-    const int64_t vecs = a.x.c / vec_elements<T>() + 1;    // (less than NV + 1 for all lanes together: the ragged one is extra)
-    if (vecs <= 64 * 2) return launch_row<T, 64, 2, MODE>(a, stream);
-    if (vecs <= 64 * 8) return launch_row<T, 64, 8, MODE>(a, stream);
-    if (vecs <= 256 * 4) return launch_row<T, 256, 4, MODE>(a, stream);
-    if (vecs <= 256 * 8) return launch_row<T, 256, 8, MODE>(a, stream);
-    if (vecs <= 512 * 8) return launch_row<T, 512, 8, MODE>(a, stream);
-    if (vecs <= 1024 * 8) return launch_row<T, 1024, 8, MODE>(a, stream);
-    if (vecs <= 1024 * 16) return launch_row<T, 1024, 16, MODE>(a, stream);
-    if (vecs <= 1024 * 20) return launch_row<T, 1024, 20, MODE>(a, stream);
+    const auto whole = [&](int lanes) { return a.x.c / (lanes * vec_elements<T>()); };
+    if (whole(64) <= 2) return launch_row<T, 64, 2, MODE>(a, stream);
+    if (whole(64) <= 8) return launch_row<T, 64, 8, MODE>(a, stream);
+    if (whole(256) <= 4) return launch_row<T, 256, 4, MODE>(a, stream);
+    if (whole(256) <= 8) return launch_row<T, 256, 8, MODE>(a, stream);
+    if (whole(512) <= 8) return launch_row<T, 512, 8, MODE>(a, stream);
+    if (whole(1024) <= 8) return launch_row<T, 1024, 8, MODE>(a, stream);
+    if (whole(1024) <= 16) return launch_row<T, 1024, 16, MODE>(a, stream);
+    if (whole(1024) <= 20) return launch_row<T, 1024, 20, MODE>(a, stream);
     tok_long_row_kernel<T, MODE><<<grid_of(a.x.n * a.x.l), 1024, 0, stream>>>(a);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
@@ -942,16 +1028,20 @@ int64_t planes_tiles(int64_t l, bool vec) { return ceil_div(l, (int64_t)kTokThre
 template <typename T, int VEC, int MODE>
 int launch_planes(const TokArgs &a, hipStream_t stream) {
     const int64_t tiles = planes_tiles(a.x.l, VEC > 1);
-    const unsigned grid = grid_of(a.x.n * tiles);
-    if (MODE == kModeGrad || a.x.c > 32)
-        tok_planes_kernel<T, VEC, 0, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
-    else if (a.x.c <= 8)
-        tok_planes_kernel<T, VEC, 8, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
-    else if (a.x.c <= 24)
-        tok_planes_kernel<T, VEC, 24, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
-    else
-        tok_planes_kernel<T, VEC, 32, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles);
-    SPICE_LAUNCH_CHECK();
+    constexpr int64_t most = (int64_t)1 << 30;
+    for (int64_t first = 0; first < a.x.n * tiles; first += most) {
+        const int64_t left = a.x.n * tiles - first;
+        const unsigned grid = (unsigned)(left < most ? left : most);
+        if (MODE == kModeGrad || a.x.c > 32)
+            tok_planes_kernel<T, VEC, 0, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles, first);
+        else if (a.x.c <= 8)
+            tok_planes_kernel<T, VEC, 8, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles, first);
+        else if (a.x.c <= 24)
+            tok_planes_kernel<T, VEC, 24, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles, first);
+        else
+            tok_planes_kernel<T, VEC, 32, MODE><<<grid, kTokThreads, 0, stream>>>(a, tiles, first);
+        SPICE_LAUNCH_CHECK();
+    }
     return SPICE_OK;
 }
 
@@ -1001,6 +1091,12 @@ int64_t items_of(const TokArgs &a, int32_t dtype) {
     return a.x.l ? planes_tiles(a.x.l, vec) : 1;
 }
 
+// Partial sums of a call at most: a workgroup's of single positions, or the waves' of the folding workgroup.
+int64_t part_doubles(int64_t n, int64_t l) {
+    const int64_t items = l > kTokThreads ? ceil_div(l, kTokThreads) : 1, waves = kTokFold / kWave;
+    return (n * items > n + waves ? n * items : n + waves) * 4;
+}
+
 SumArgs sums_of(const TokArgs &a, double *part) {
     SumArgs s = {};
     s.logp = a.logp;
@@ -1029,8 +1125,7 @@ using namespace spice;
 
 extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
     if (n < 0 || l < 0) return 0;
-    const int64_t items = l > kTokThreads ? ceil_div(l, kTokThreads) : 1;   // the smallest items: a workgroup of single positions
-    return (size_t)(n * items * 4 * (int64_t)sizeof(double) + ((n + 1) / 2) * 8 + 64);
+    return (size_t)(part_doubles(n, l) + 2 * n + 8) * sizeof(double);
 }
 
 extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, float temperature, float *logp, float *stats,
@@ -1079,16 +1174,18 @@ extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *
     a.part = (double *)workspace;
     int rc = launch_positions<kModePreference>(a, x->dtype, s);
     if (rc) return rc;
-    const int64_t items = items_of(a, x->dtype);
-    if (route_of(a) != kByPlanes || x->l == 0) {
-        SumArgs sums = sums_of(a, a.part);
-        sums.ref = ref_logp;
+    SumArgs sums = sums_of(a, a.part);
+    sums.ref = ref_logp;
+    int64_t ways = 0;
+    if (route_of(a) == kByPlanes && x->l) {
+        sums.chunks = items_of(a, x->dtype);
+    } else if (!(ways = ways_of(x->n, x->l))) {
         rc = launch_sums<kSumPreference>(sums, s);
         if (rc) return rc;
     }
-    PreferenceEnd e = {a.part, x->n, items, p->beta, p->smoothing, p->loss_type == SPICE_PREFERENCE_IPO, p->average != 0,
-                       total, rewards, weight};
-    tok_preference_kernel<<<1, kTokFold, 0, s>>>(e);
+    PreferenceEnd e = {p->beta, p->smoothing, p->loss_type == SPICE_PREFERENCE_IPO, p->average != 0, total, rewards, weight,
+                       a.part + part_doubles(x->n, x->l)};
+    tok_preference_kernel<<<1, kTokFold, 0, s>>>(sums, ways, e);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
 }
@@ -1114,20 +1211,23 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     if (grad) grad_layout(a, grad, class_last);
     a.part = (double *)workspace;
     SumArgs sums = sums_of(a, a.part);
-    const int64_t items = items_of(a, x->dtype);
-    float *share = (float *)(a.part + x->n * (items > sums.chunks ? items : sums.chunks) * 4);
+    float *share = (float *)(a.part + part_doubles(x->n, x->l));
     a.share = share;
-    int rc = launch_sums<kSumCount>(sums, s);
+    int64_t ways = ways_of(x->n, x->l);
+    int rc = ways ? SPICE_OK : launch_sums<kSumCount>(sums, s);
     if (rc) return rc;
-    tok_share_kernel<<<1, kTokFold, 0, s>>>(sums.part, x->n, sums.chunks, p->reduction == SPICE_POLICY_SEQUENCE, share);
+    tok_share_kernel<<<1, kTokFold, 0, s>>>(sums, ways, p->reduction == SPICE_POLICY_SEQUENCE, share);
     SPICE_LAUNCH_CHECK();
     rc = grad ? launch_positions<kModePolicyGrad>(a, x->dtype, s) : launch_positions<kModePolicy>(a, x->dtype, s);
     if (rc) return rc;
-    if (route_of(a) != kByPlanes || x->l == 0) {
+    if (route_of(a) == kByPlanes && x->l) {
+        sums.chunks = items_of(a, x->dtype);
+        ways = 0;
+    } else if (!ways) {
         rc = launch_sums<kSumPolicy>(sums, s);
         if (rc) return rc;
     }
-    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(a.part, x->n, items, share, p->kl_weight, out4);
+    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(sums, ways, share, p->kl_weight, out4);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
 }
