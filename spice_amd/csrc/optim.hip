@@ -57,6 +57,25 @@ __device__ __forceinline__ bool on16(const void *p) { return (reinterpret_cast<u
 template <typename T, int K>
 struct __attribute__((aligned(sizeof(T) * K))) Vec { T v[K]; };
 
+// Past the caches: what a step reads and writes once would leave its dirty lines in the memory-side cache, to be written
+// back under the next call's reads (a 39.5 M parameter step with its norm: 266 us through the caches, 234 past them).
+// The norm's own read goes through them: the update behind it finds part of the gradients there.
+template <typename V>
+__device__ __forceinline__ V take_once(const V *p) {
+    if constexpr (sizeof(V) == 16) {
+        return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4_t *)p));
+    } else {
+        return __builtin_bit_cast(V, __builtin_nontemporal_load((const unsigned long long *)p));
+    }
+}
+template <typename V>
+__device__ __forceinline__ void put_once(V *p, const V &v) {
+    if constexpr (sizeof(V) == 16) {
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), (u32x4_t *)p);
+    } else {
+        __builtin_nontemporal_store(__builtin_bit_cast(unsigned long long, v), (unsigned long long *)p);
+    }
+}
 // NaN-keeping maximum
 __device__ __forceinline__ double max_keep(double a, double b) { return (a > b || a != a) ? a : b; }
 
@@ -94,15 +113,16 @@ __global__ __launch_bounds__(kOptThreads) void grad_norm_kernel(TableOf<1> t, do
         typedef Vec<T, K> VecTK;
         const Vec<T, K> *gv = (const Vec<T, K> *)g;
         const uint32_t nv = n / K;
-        // eight loads in flight a lane; two chains of sums
+        // UN loads in flight a lane; two chains of sums
+        constexpr int UN = sizeof(T) == 4 ? 8 : 4;
         double two = 0.0;
         uint32_t i = threadIdx.x;
-        for (; i + 7 * kOptThreads < nv; i += 8 * kOptThreads) {
-            u32x4_t x[8];
+        for (; i + (UN - 1) * kOptThreads < nv; i += UN * kOptThreads) {
+            u32x4_t x[UN];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __builtin_nontemporal_load((const u32x4_t *)(gv + i + j * kOptThreads));
+            for (int j = 0; j < UN; ++j) x[j] = *(const u32x4_t *)(gv + i + j * kOptThreads);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < UN; ++j) {
                 const Vec<T, K> v = __builtin_bit_cast(VecTK, x[j]);
 #pragma unroll
                 for (int k = 0; k < K; k += 2) {
@@ -186,7 +206,8 @@ __global__ __launch_bounds__(kOptThreads) void grad_clip_kernel(TableOf<2> t, co
             Vec<O, K> y;
 #pragma unroll
             for (int k = 0; k < K; ++k) y.v[k] = (O)(opt_f32(x.v[k]) * c);
-            ((Vec<O, K> *)out)[i] = y;
+            typedef Vec<O, K> VO;
+            put_once((VO *)out + i, y);
         }
         done = nv * K;
     }
@@ -218,17 +239,19 @@ __global__ __launch_bounds__(kOptThreads) void adam_kernel(TableOf<4> t, AdamArg
     float *m = (float *)t.p[2][e] + at, *v = (float *)t.p[3][e] + at;
     const uint32_t n = min(t.each, t.numel[e] - at);
     uint32_t done = 0;
+    typedef Vec<T, 4> V4T;
+    typedef Vec<float, 4> V4F;
     if (on16(p) && on16(g) && on16(m) && on16(v)) {
         const uint32_t nv = n / 4;
         for (uint32_t i = threadIdx.x; i < nv; i += kOptThreads) {
-            Vec<T, 4> pv = ((const Vec<T, 4> *)p)[i];
+            Vec<T, 4> pv = take_once((const V4T *)p + i);
             const Vec<T, 4> gv = ((const Vec<T, 4> *)g)[i];
-            Vec<float, 4> mv = ((const Vec<float, 4> *)m)[i], vv = ((const Vec<float, 4> *)v)[i];
+            Vec<float, 4> mv = take_once((const V4F *)m + i), vv = take_once((const V4F *)v + i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) adam_take<T>(pv.v[k], gv.v[k], mv.v[k], vv.v[k], a, c, rate, root);
-            ((Vec<T, 4> *)p)[i] = pv;
-            ((Vec<float, 4> *)m)[i] = mv;
-            ((Vec<float, 4> *)v)[i] = vv;
+            put_once((V4T *)p + i, pv);
+            put_once((V4F *)m + i, mv);
+            put_once((V4F *)v + i, vv);
         }
         done = nv * 4;
     }
