@@ -624,7 +624,8 @@ int spice_policy_loss(const spice_logits *logits, const spice_labels *labels, co
  * `grads`, `params`, ... are HOST arrays of `count` device pointers (aligned to
  * their element), numel a host array of element counts; they are read before the
  * call returns.  dtype 0 = fp32, 1 = fp16, 2 = bf16, one for all tensors of a call.
- * record: 4 device floats, {norm, clip factor, and two of the Adam step's}.
+ * record: 4 device floats, {norm, clip factor, and two of the Adam step's}; an Adam step that neither clips nor counts
+ * on the device leaves it as it is.
  * ------------------------------------------------------------------------- */
 #define SPICE_NORM_L2 0
 #define SPICE_NORM_INF 1
@@ -641,6 +642,11 @@ int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int
  * moved where the factor is 1); other overlaps are not allowed. */
 int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
                     int32_t count, const float *record, void *stream);
+
+/* Both in one call (and one launch where the tensors hold few elements). */
+int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
+                         int32_t count, int32_t norm_type, float max_norm, float *record, void *workspace,
+                         size_t workspace_bytes, void *stream);
 
 typedef struct spice_adam_params {
     double lr, beta1, beta2, eps, weight_decay;

@@ -176,6 +176,8 @@ SIGNATURES = {
                                   c_size_t, c_void_p]),
     "spice_grad_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_void_p,
                                   c_void_p]),
+    "spice_grad_norm_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_int32,
+                                       c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "spice_adam_step": (c_int32, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64),
                                   c_int32, c_int32, POINTER(AdamParams), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                   c_void_p]),

@@ -157,8 +157,31 @@ struct RecordArgs {
     float *record;
 };
 
+// The step's two factors, by a wave that does not wait for the norm.
+__device__ __forceinline__ void record_step(const RecordArgs &a) {
+    int64_t t = a.host_step;
+    if (a.step) {
+        t = *a.step + 1;
+        *a.step = t;
+    }
+    a.record[2] = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
+    a.record[3] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+}
+
+__device__ __forceinline__ float record_norm(const RecordArgs &a, double norm) {
+    double c = 1.0;
+    if (a.clip) {
+        c = a.max_norm / (norm + 1e-6);
+        if (c > 1.0) c = 1.0;
+    }
+    a.record[0] = (float)norm;
+    a.record[1] = (float)c;
+    return (float)c;
+}
+
 __global__ __launch_bounds__(kOptFold) void grad_record_kernel(RecordArgs a) {
     __shared__ double lds[kOptFold / kWave];
+    if (a.adam && threadIdx.x == kOptFold - 1) record_step(a);
     double norm = 0.0;
     if (a.norm_in) {
         norm = (double)*a.norm_in;
@@ -169,22 +192,39 @@ __global__ __launch_bounds__(kOptFold) void grad_record_kernel(RecordArgs a) {
         for (int64_t i = threadIdx.x; i < a.parts; i += kOptFold) norm += a.part[i];
         norm = sqrt(norm_fold<false>(norm, lds, kOptFold));
     }
-    if (threadIdx.x != 0) return;
-    double c = 1.0;
-    if (a.clip) {
-        c = a.max_norm / (norm + 1e-6);
-        if (c > 1.0) c = 1.0;
+    if (threadIdx.x == 0) record_norm(a, norm);
+}
+
+// Small calls: one workgroup takes the norm, leaves the record and, with outputs, clips; its waves share the items.
+template <typename T, typename O, bool INF, bool CLIP>
+__global__ __launch_bounds__(kOptFold) void grad_here_kernel(TableOf<CLIP ? 2 : 1> t, int32_t items, RecordArgs a) {
+    __shared__ double lds[kOptFold / kWave];
+    __shared__ float factor;
+    constexpr int kWaves = kOptFold / kWave;
+    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if (a.adam && threadIdx.x == kOptFold - 1) record_step(a);
+    double acc = 0.0;
+    for (uint32_t item = wave; item < (uint32_t)items; item += kWaves) {
+        const int e = entry_of(t, item);
+        const uint32_t at = (item - t.first[e]) * t.each, n = min(t.each, t.numel[e] - at);
+        const T *g = (const T *)t.p[0][e] + at;
+#pragma unroll 8
+        for (uint32_t i = lane; i < n; i += kWave) acc = norm_take<T, INF>(acc, g[i]);
     }
-    a.record[0] = (float)norm;
-    a.record[1] = (float)c;
-    if (a.adam) {
-        int64_t t = a.host_step;
-        if (a.step) {
-            t = *a.step + 1;
-            *a.step = t;
+    acc = norm_fold<INF>(acc, lds, kOptFold);
+    if (threadIdx.x == 0) factor = record_norm(a, INF ? acc : sqrt(acc));
+    if constexpr (CLIP) {
+        __syncthreads();
+        const float c = factor;
+        for (uint32_t item = wave; item < (uint32_t)items; item += kWaves) {
+            const int e = entry_of(t, item);
+            const uint32_t at = (item - t.first[e]) * t.each, n = min(t.each, t.numel[e] - at);
+            const T *g = (const T *)t.p[0][e] + at;
+            O *out = (O *)t.p[1][e] + at;
+            if (c == 1.f && (const void *)g == (const void *)out) continue;
+#pragma unroll 8
+            for (uint32_t i = lane; i < n; i += kWave) out[i] = (O)(opt_f32(g[i]) * c);
         }
-        a.record[2] = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
-        a.record[3] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
     }
 }
 
@@ -215,6 +255,7 @@ __global__ __launch_bounds__(kOptThreads) void grad_clip_kernel(TableOf<2> t, co
 }
 
 struct AdamArgs {
+    float rate, root;                 // record[2] and [3] where there is no record
     float a1, a2, eps, decay, keep;   // a = 1 - beta, taken in fp64 (1 - 0.999f is 1e-5 of itself off); keep = 1 - lr * decay with decoupled decay, else 1; decay = 0 then
 };
 
@@ -231,7 +272,7 @@ __device__ __forceinline__ void adam_take(T &p, T g, float &m, float &v, const A
 
 template <typename T>
 __global__ __launch_bounds__(kOptThreads) void adam_kernel(TableOf<4> t, AdamArgs a, const float *record) {
-    const float c = record[1], rate = record[2], root = record[3];
+    const float c = record ? record[1] : 1.f, rate = record ? record[2] : a.rate, root = record ? record[3] : a.root;
     const int e = entry_of(t, blockIdx.x);
     const uint32_t at = (blockIdx.x - t.first[e]) * t.each;
     T *p = (T *)t.p[0][e] + at;
@@ -314,6 +355,18 @@ int for_tables(void *const *const (&ptrs)[PTRS], const int64_t (&bytes)[PTRS], c
     return t.count ? launch(t, before, items) : SPICE_OK;
 }
 
+// Calls of few elements, whose latency counts: one workgroup's work.  Its 1024 threads read 32 elements each.
+constexpr int64_t kOptHere = 32768;
+constexpr uint32_t kOptHereItem = 512;
+
+bool few(const int64_t *numel, int32_t count, int entries) {
+    int64_t total = 0;
+    if (count > entries) return false;
+    for (int32_t i = 0; i < count; ++i)
+        if ((total += numel[i]) > kOptHere) return false;
+    return true;
+}
+
 bool pointers_ok(void *const *p, const int64_t *numel, int32_t count, int64_t bytes) {
     if (count && !p) return false;
     for (int32_t i = 0; i < count; ++i)
@@ -335,6 +388,50 @@ int launch_norm(void *const *grads, const int64_t *numel, int32_t count, int64_t
         SPICE_LAUNCH_CHECK();
         return (int)SPICE_OK;
     });
+}
+
+template <typename T>
+int launch_norm_here(void *const *grads, const int64_t *numel, int32_t count, const RecordArgs &a, hipStream_t s) {
+    void *const *const p[1] = {grads};
+    const int64_t b[1] = {(int64_t)sizeof(T)};
+    bool done = false;
+    const auto launch = [&](const TableOf<1> &t, int64_t, int64_t items) {
+        if (a.inf)
+            grad_here_kernel<T, T, true, false><<<1, kOptFold, 0, s>>>(t, (int32_t)items, a);
+        else
+            grad_here_kernel<T, T, false, false><<<1, kOptFold, 0, s>>>(t, (int32_t)items, a);
+        done = true;
+        SPICE_LAUNCH_CHECK();
+        return (int)SPICE_OK;
+    };
+    const int rc = for_tables<1>(p, b, numel, count, kOptHereItem, launch);
+    if (rc || done) return rc;
+    TableOf<1> none;      // (no elements at all: a norm of 0)
+    none.count = 0;
+    none.each = kOptHereItem;
+    return launch(none, 0, 0);
+}
+
+template <typename T, typename O>
+int launch_clip_here(void *const *grads, void *const *out, const int64_t *numel, int32_t count, const RecordArgs &a, hipStream_t s) {
+    void *const *const p[2] = {grads, out};
+    const int64_t b[2] = {(int64_t)sizeof(T), (int64_t)sizeof(O)};
+    bool done = false;
+    const auto launch = [&](const TableOf<2> &t, int64_t, int64_t items) {
+        if (a.inf)
+            grad_here_kernel<T, O, true, true><<<1, kOptFold, 0, s>>>(t, (int32_t)items, a);
+        else
+            grad_here_kernel<T, O, false, true><<<1, kOptFold, 0, s>>>(t, (int32_t)items, a);
+        done = true;
+        SPICE_LAUNCH_CHECK();
+        return (int)SPICE_OK;
+    };
+    const int rc = for_tables<2>(p, b, numel, count, kOptHereItem, launch);
+    if (rc || done) return rc;
+    TableOf<2> none;
+    none.count = 0;
+    none.each = kOptHereItem;
+    return launch(none, 0, 0);
 }
 
 template <typename T, typename O>
@@ -370,28 +467,72 @@ extern "C" size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t 
     return (size_t)(item_count(numel, count, item_elements(numel, count)) * (int64_t)sizeof(double) + 64);
 }
 
-extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
-                               float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream) {
-    if (dtype < 0 || dtype > 2 || !counts_ok(numel, count) || !pointers_ok(grads, numel, count, type_bytes(dtype)) || !record ||
-        !workspace || !aligned8(workspace) || norm_type < 0 || norm_type > 1 || !(max_norm >= 0.f))
-        return SPICE_ERR_ARG;
-    if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
-    hipStream_t s = (hipStream_t)stream;
-    double *part = (double *)workspace;
-    int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, norm_type, part, s)
-             : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, norm_type, part, s)
-                          : launch_norm<__bf16>(grads, numel, count, 2, norm_type, part, s);
+namespace spice {
+namespace {
+
+// The norm of the call's gradients and the record from it.
+int norm_and_record(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, RecordArgs &a, double *part,
+                    hipStream_t s) {
+    if (few(numel, count, table_entries<1>()))
+        return dtype == 0   ? launch_norm_here<float>(grads, numel, count, a, s)
+               : dtype == 1 ? launch_norm_here<_Float16>(grads, numel, count, a, s)
+                            : launch_norm_here<__bf16>(grads, numel, count, a, s);
+    const int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, a.inf, part, s)
+                   : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, a.inf, part, s)
+                                : launch_norm<__bf16>(grads, numel, count, 2, a.inf, part, s);
     if (rc) return rc;
-    RecordArgs a = {};
     a.part = part;
     a.parts = item_count(numel, count, item_elements(numel, count));
+    grad_record_kernel<<<1, kOptFold, 0, s>>>(a);
+    SPICE_LAUNCH_CHECK();
+    return SPICE_OK;
+}
+
+bool norm_ok(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type, float max_norm,
+             const float *record, const void *workspace) {
+    return dtype >= 0 && dtype <= 2 && counts_ok(numel, count) && pointers_ok(grads, numel, count, type_bytes(dtype)) && record &&
+           workspace && aligned8(workspace) && norm_type >= 0 && norm_type <= 1 && max_norm >= 0.f;
+}
+
+RecordArgs norm_record(int32_t norm_type, float max_norm, float *record) {
+    RecordArgs a = {};
     a.inf = norm_type == SPICE_NORM_INF;
     a.clip = 1;
     a.max_norm = (double)max_norm;
     a.record = record;
-    grad_record_kernel<<<1, kOptFold, 0, s>>>(a);
-    SPICE_LAUNCH_CHECK();
-    return SPICE_OK;
+    return a;
+}
+
+}  // namespace
+}  // namespace spice
+
+extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
+                               float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!norm_ok(grads, numel, count, dtype, norm_type, max_norm, record, workspace)) return SPICE_ERR_ARG;
+    if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
+    RecordArgs a = norm_record(norm_type, max_norm, record);
+    return norm_and_record(grads, numel, count, dtype, a, (double *)workspace, (hipStream_t)stream);
+}
+
+extern "C" int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
+                                    int32_t count, int32_t norm_type, float max_norm, float *record, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    if (!norm_ok(grads, numel, count, dtype, norm_type, max_norm, record, workspace) || !(out_dtype == dtype || out_dtype == 0) ||
+        !pointers_ok(out, numel, count, type_bytes(out_dtype)))
+        return SPICE_ERR_ARG;
+    if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
+    RecordArgs a = norm_record(norm_type, max_norm, record);
+    hipStream_t s = (hipStream_t)stream;
+    if (few(numel, count, table_entries<2>())) {
+        if (dtype == 0) return launch_clip_here<float, float>(grads, out, numel, count, a, s);
+        if (dtype == 1)
+            return out_dtype == 0 ? launch_clip_here<_Float16, float>(grads, out, numel, count, a, s)
+                                  : launch_clip_here<_Float16, _Float16>(grads, out, numel, count, a, s);
+        return out_dtype == 0 ? launch_clip_here<__bf16, float>(grads, out, numel, count, a, s)
+                              : launch_clip_here<__bf16, __bf16>(grads, out, numel, count, a, s);
+    }
+    const int rc = norm_and_record(grads, numel, count, dtype, a, (double *)workspace, s);
+    return rc ? rc : spice_grad_clip(grads, dtype, out, out_dtype, numel, count, record, stream);
 }
 
 extern "C" int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
@@ -423,15 +564,6 @@ extern "C" int spice_adam_step(void *const *params, void *const *grads, void *co
     if (take && workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     RecordArgs r = {};
-    int rc = SPICE_OK;
-    if (take) {
-        r.part = (const double *)workspace;
-        r.parts = item_count(numel, count, item_elements(numel, count));
-        rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, 0, (double *)workspace, s)
-             : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, 0, (double *)workspace, s)
-                          : launch_norm<__bf16>(grads, numel, count, 2, 0, (double *)workspace, s);
-        if (rc) return rc;
-    }
     r.norm_in = clip ? norm : nullptr;
     r.clip = clip;
     r.adam = 1;
@@ -442,14 +574,23 @@ extern "C" int spice_adam_step(void *const *params, void *const *grads, void *co
     r.host_step = p->step;
     r.step = step;
     r.record = record;
-    grad_record_kernel<<<1, kOptFold, 0, s>>>(r);
-    SPICE_LAUNCH_CHECK();
-    AdamArgs a;
+    AdamArgs a = {};
     a.a1 = (float)(1.0 - p->beta1);
     a.a2 = (float)(1.0 - p->beta2);
     a.eps = (float)p->eps;
     a.decay = p->decoupled ? 0.f : (float)p->weight_decay;
     a.keep = p->decoupled ? (float)(1.0 - p->lr * p->weight_decay) : 1.f;
+    if (take) {
+        const int rc = norm_and_record(grads, numel, count, dtype, r, (double *)workspace, s);
+        if (rc) return rc;
+    } else if (clip || step) {
+        grad_record_kernel<<<1, kOptFold, 0, s>>>(r);
+        SPICE_LAUNCH_CHECK();
+    } else {    // nothing that only the device knows
+        a.rate = (float)(p->lr / (1.0 - pow(p->beta1, (double)p->step)));
+        a.root = (float)(1.0 / sqrt(1.0 - pow(p->beta2, (double)p->step)));
+        record = nullptr;
+    }
     return dtype == 0   ? launch_adam<float>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
            : dtype == 1 ? launch_adam<_Float16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
                         : launch_adam<__bf16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s);

@@ -16,6 +16,7 @@ namespace {
 constexpr int kTokThreads = 256;
 constexpr int kTokChunk = 2048;      // positions of one workgroup of the passes over positions
 constexpr int kTokFold = 1024;       // threads of the one workgroup that folds their partial sums
+constexpr int64_t kTokCount = 2048;  // positions that every workgroup counts for itself: a launch less ([1,7,32000] fp16)
 constexpr int64_t kTokHere = 16384;  // positions that this workgroup sums itself: 16 a thread
 
 // The logits as the kernels see them: element strides of sequence, position and class.
@@ -163,12 +164,6 @@ __device__ __forceinline__ void block_sums(double (&v)[K], double *lds, int thre
     __syncthreads();
 }
 
-// ---- one position a workgroup, any strides ----
-
-// Logp: logp and (max, sum) of each position.  Grad: weight * d logp / d x from them.  Preference, Policy: logp, and what the
-// loss sums over positions.  PolicyGrad: the policy loss's gradient behind that.
-enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kModePolicyGrad = 4 };
-
 struct TokArgs {
     Logits x;
     Labels y;
@@ -186,13 +181,44 @@ struct TokArgs {
     int64_t g_sn, g_sl, g_sc;
     Policy policy;
     const float *ref;       // kModePreference
-    const float *share;     // [n] what a position of sequence n counts in the mean
+    const float *share;     // [n] what a position of sequence n counts in the mean; NULL: counted where it is needed
+    int per_sequence;
     double *part;           // sums of each workgroup's item
 };
+
+// What a position of sequence n counts in the mean, from the labels: THREADS threads count all of them (few: kTokCount),
+// a wave by itself or a workgroup with `lds`.
+template <int THREADS>
+__device__ __forceinline__ float share_here(const TokArgs &a, int64_t n, int *lds) {
+    const int64_t first = a.per_sequence ? n * a.x.l : 0, end = a.per_sequence ? first + a.x.l : a.x.n * a.x.l;
+    int count = 0;
+    for (int64_t i = first + threadIdx.x % THREADS; i < end; i += THREADS) {
+        const int64_t k = (uint32_t)i / (uint32_t)a.x.l;
+        count += a.y.y[k * a.y.sn + (i - k * a.x.l) * a.y.sl] != a.y.ignore;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, kWave);
+    if (THREADS > kWave) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x / kWave] = count;
+        __syncthreads();
+        count = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / kWave; ++w) count += lds[w];
+    }
+    return (float)(1.0 / ((double)(count > 1 ? count : 1) * (a.per_sequence ? (double)a.x.n : 1.0)));
+}
+
+// ---- one position a workgroup, any strides ----
+
+// Logp: logp and (max, sum) of each position.  Grad: weight * d logp / d x from them.  Preference, Policy: logp, and what the
+// loss sums over positions.  PolicyGrad: the policy loss's gradient behind that.
+enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kModePolicyGrad = 4 };
+
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
     __shared__ float lds[2 * kTokThreads / kWave];
+    __shared__ int counts[kTokThreads / kWave];
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int64_t total = a.x.n * a.x.l;
     for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
@@ -233,7 +259,7 @@ __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
             else if (kind == kCounted && MODE == kModeGrad)
                 w = a.weight[n * a.w_sn + l * a.w_sl];
             else if (kind == kCounted)
-                w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+                w = policy_term(a.policy, logp, at, n, l).dlogp * (a.share ? a.share[n] : share_here<kTokThreads>(a, n, counts));
             if (MODE == kModePolicyGrad && a.weight_out && threadIdx.x == 0) a.weight_out[at] = w;
             if (kind == kCounted) w *= a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f);
             const float each = kind == kCounted ? w / s : w;
@@ -357,6 +383,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     constexpr int kBlock = LANES < kTokThreads ? kTokThreads : LANES;
     constexpr bool kGrad = MODE == kModePolicyGrad;
     __shared__ float lds[2 * kBlock / kWave];
+    __shared__ int counts[kBlock / kWave];
     const int64_t at = first + (int64_t)blockIdx.x * (kBlock / LANES) + __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
     if (at >= a.x.n * a.x.l) return;
     const int32_t lane = threadIdx.x % LANES, classes = (int32_t)a.x.c, whole = classes / (LANES * K);
@@ -366,6 +393,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
     const int kind = label_kind(y, a.y.ignore, a.x.c);
     float m = -INFINITY, s = 0.f, logp = kind == kBad ? NAN : 0.f;
+    float share = 0.f;
     u32x4 raw[NV], last;
     if (kind == kCounted) {
         const T *mine = x + lane * K;
@@ -374,6 +402,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
         for (int i = 0; i < NV; ++i)
             if (i < whole) raw[i] = read_vec<kGrad>(mine + i * LANES * K);
         last = load_vec<T>(x + tail, left);
+        if (kGrad) share = a.share ? a.share[n] : share_here<LANES>(a, n, counts);   // (under the logits' loads)
         float v[K];
         unpack(last, v, T());
 #pragma unroll
@@ -407,7 +436,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     if (kGrad) {
         T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
         float w = kind == kBad ? NAN : 0.f;
-        if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+        if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * share;
         if (a.weight_out && lane == 0) a.weight_out[at] = w;
         const float shift = shift_of(m);
         w *= a.t.inv * a.host_scale;
@@ -440,6 +469,7 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
     constexpr int K = vec_elements<T>(), kBlock = 1024, kStep = 4;
     constexpr bool kGrad = MODE == kModePolicyGrad;
     __shared__ float lds[2 * kBlock / kWave];
+    __shared__ int counts[kBlock / kWave];
     const int64_t total = a.x.n * a.x.l;
     const int32_t classes = (int32_t)a.x.c;
     for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
@@ -487,7 +517,8 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
         if (kGrad) {
             T *g = (T *)a.grad + n * a.g_sn + l * a.g_sl;
             float w = kind == kBad ? NAN : 0.f;
-            if (kind == kCounted) w = policy_term(a.policy, logp, at, n, l).dlogp * a.share[n];
+            if (kind == kCounted)
+                w = policy_term(a.policy, logp, at, n, l).dlogp * (a.share ? a.share[n] : share_here<kBlock>(a, n, counts));
             if (a.weight_out && threadIdx.x == 0) a.weight_out[at] = w;
             const float shift = shift_of(m);
             w *= a.t.inv * a.host_scale;
@@ -617,10 +648,13 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
     constexpr int kStep = 8;
     typedef typename GroupOf<T, VEC>::type G;
     __shared__ double lds[kSums ? K * kTokThreads / kWave : 1];
+    __shared__ int counts[kTokThreads / kWave];
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int32_t classes = (int32_t)a.x.c;
     const int64_t item = first + blockIdx.x, n = item / tiles;
     const int64_t l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
+    float share = 0.f;
+    if (MODE == kModePolicyGrad) share = a.share ? a.share[n] : share_here<kTokThreads>(a, n, counts);
     double sums[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) sums[k] = 0.0;
@@ -734,7 +768,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
                     sums[1] += t.far;
                     sums[2 % K] += t.over ? 1.0 : 0.0;
                     sums[3 % K] += 1.0;
-                    w[k] = kind[k] == kBad ? NAN : t.dlogp * (MODE == kModePolicyGrad ? a.share[n] : 0.f);
+                    w[k] = kind[k] == kBad ? NAN : t.dlogp * share;
                 }
                 if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at + k] = w[k];
             } else if (kind[k] == kCounted) {
@@ -944,20 +978,33 @@ __device__ __forceinline__ void policy_end(double surrogate, double far, double 
     out4[3] = (float)(over / fmax(count, 1.0));
 }
 
-__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, const float *share, float kl, float *out4) {
+// The end of the policy loss.  `each` [n, 4]: scratch.
+__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, int per_sequence, double *each, float kl,
+                                                                  float *out4) {
     __shared__ double lds[4 * kTokFold / kWave];
     if (ways) sums_here<kSumPolicy>(a, ways);
     const int64_t chunks = ways ? ways : a.chunks;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t i = threadIdx.x; i < a.n * chunks; i += kTokFold) {
-        const double each = (double)share[(uint32_t)i / (uint32_t)chunks];
-        v[0] += a.part[i * 4] * each;
-        v[1] += a.part[i * 4 + 1] * each;
-        v[2] += a.part[i * 4 + 2];
-        v[3] += a.part[i * 4 + 3];
+    if (per_sequence) {
+        fold_sequences<4>(a.part, a.n, chunks, [&](int64_t i, const double (&u)[4]) {
+            const double share = 1.0 / (fmax(u[3], 1.0) * (double)a.n);
+            each[4 * i] = u[0] * share;
+            each[4 * i + 1] = u[1] * share;
+            each[4 * i + 2] = u[2];
+            each[4 * i + 3] = u[3];
+        });
+        __threadfence_block();
+        __syncthreads();
     }
+    const double *from = per_sequence ? each : a.part;
+    for (int64_t i = threadIdx.x; i < (per_sequence ? a.n : a.n * chunks); i += kTokFold)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += from[4 * i + k];
     block_sums<4>(v, lds, kTokFold);
-    if (threadIdx.x == 0) policy_end(v[0], v[1], v[2], v[3], kl, out4);
+    if (threadIdx.x == 0) {
+        const double share = per_sequence ? 1.0 : 1.0 / fmax(v[3], 1.0);
+        policy_end(v[0] * share, v[1] * share, v[2], v[3], kl, out4);
+    }
 }
 
 // How many waves of the folding workgroup share a sequence where it takes the sums itself; 0: they are too many for it.
@@ -1144,7 +1191,7 @@ using namespace spice;
 
 extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
     if (n < 0 || l < 0) return 0;
-    return (size_t)(part_doubles(n, l) + 2 * n + 8) * sizeof(double);
+    return (size_t)(part_doubles(n, l) + 4 * n + 8) * sizeof(double);
 }
 
 extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, float temperature, float *logp, float *stats,
@@ -1233,13 +1280,18 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     double *scratch = a.part + part_doubles(x->n, x->l);
     float *share = (float *)scratch;
     a.share = share;
+    a.per_sequence = p->reduction == SPICE_POLICY_SEQUENCE;
     const bool planes = route_of(a) == kByPlanes && x->l;
     int64_t ways = ways_of(x->n, x->l);
     int rc = SPICE_OK;
-    if (!ways) rc = launch_sums<kSumCount>(sums, s);
-    if (rc) return rc;
-    tok_share_kernel<<<1, kTokFold, 0, s>>>(sums, ways, p->reduction == SPICE_POLICY_SEQUENCE, share);
-    SPICE_LAUNCH_CHECK();
+    if (!grad || x->n * x->l <= kTokCount) {
+        a.share = nullptr;
+    } else {
+        if (!ways) rc = launch_sums<kSumCount>(sums, s);
+        if (rc) return rc;
+        tok_share_kernel<<<1, kTokFold, 0, s>>>(sums, ways, a.per_sequence, share);
+        SPICE_LAUNCH_CHECK();
+    }
     rc = grad ? launch_positions<kModePolicyGrad>(a, x->dtype, s) : launch_positions<kModePolicy>(a, x->dtype, s);
     if (rc) return rc;
     if (planes) {
@@ -1249,7 +1301,7 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
         rc = launch_sums<kSumPolicy>(sums, s);
         if (rc) return rc;
     }
-    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(sums, ways, share, p->kl_weight, out4);
+    tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(sums, ways, a.per_sequence, scratch, p->kl_weight, out4);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
 }

@@ -14,6 +14,7 @@
 //   update_confusion_matrix        baseline/eval/metrics.py:8-19          -> confusion_update
 //   argmax + update                baseline/eval/inference.py:47-48       -> argmax_confusion_update
 #include <ATen/ATen.h>
+#include <ATen/core/List.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -1003,10 +1004,11 @@ Tensor token_logprobs_grad(const Tensor &logits, const Tensor &labels, const Ten
     return grad;
 }
 
-// (total [], rewards [N], weight [N], stats): the gradient is token_logprobs_grad on the last two.
-std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor &logits, const Tensor &labels, const Tensor &ref_logprobs,
-                                                           int64_t class_dim, double temperature, int64_t ignore_index,
-                                                           double beta, double smoothing, int64_t loss_type, bool average) {
+// (total [], rewards [N], grad) with want_grad; else (total, rewards, weight [N], stats), whose last two are what
+// token_logprobs_grad takes for the gradient.
+std::vector<Tensor> preference_loss(const Tensor &logits, const Tensor &labels, const Tensor &ref_logprobs, int64_t class_dim,
+                                    double temperature, int64_t ignore_index, double beta, double smoothing, int64_t loss_type,
+                                    bool average, bool want_grad, double grad_scale) {
     const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "preference_loss");
     check_positions(ref_logprobs, "ref_logprobs", labels);
     TORCH_CHECK_VALUE(v.x.n >= 2 && v.x.n % 2 == 0, "preference_loss: the first axis must hold the preferred half and the other "
@@ -1016,23 +1018,41 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor &logits,
     TORCH_CHECK_VALUE(loss_type != SPICE_PREFERENCE_IPO || smoothing == 0.0, "preference_loss: ipo takes no label_smoothing");
     c10::DeviceGuard guard(logits.device());
     const auto f32 = logits.options().dtype(at::kFloat);
-    Tensor total = at::empty({}, f32), rewards = at::empty({v.x.n}, f32), weight = at::empty({v.x.n}, f32);
-    Tensor logp = at::empty(labels.sizes(), f32), stats = stats_for(labels, f32), ws = loss_workspace(v, f32);
+    const int64_t positions = v.x.n * v.x.l, ws_bytes = (int64_t)spice_token_loss_workspace_bytes(v.x.n, v.x.l);
+    Tensor total = at::empty({}, f32), rewards = at::empty({v.x.n}, f32), weight, stats;
+    // the workspace, logp and, where only the gradient below needs them, weight and statistics in one piece
+    Tensor scratch = at::empty({ws_bytes / 4 + positions + (want_grad ? 2 * positions + v.x.n : 0)}, f32);
+    float *logp = scratch.data_ptr<float>() + ws_bytes / 4, *stats_p, *weight_p;
+    if (want_grad) {
+        stats_p = scratch.data_ptr<float>() + ws_bytes / 4;
+        logp = stats_p + 2 * positions;
+        weight_p = logp + positions;
+    } else {
+        weight = at::empty({v.x.n}, f32);
+        stats = stats_for(labels, f32);
+        stats_p = stats.data_ptr<float>();
+        weight_p = weight.data_ptr<float>();
+    }
     spice_preference_params p;
     p.temperature = (float)temperature;
     p.beta = (float)beta;
     p.smoothing = (float)smoothing;
     p.loss_type = (int32_t)loss_type;
     p.average = average ? 1 : 0;
+    void *stream = current_stream(logits);
     check_rc(spice_preference_loss(&v.x, &v.y, ref_logprobs.data_ptr<float>(), &p, total.data_ptr<float>(),
-                                   rewards.data_ptr<float>(), weight.data_ptr<float>(), logp.data_ptr<float>(),
-                                   stats.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(logits)),
+                                   rewards.data_ptr<float>(), weight_p, logp, stats_p, scratch.data_ptr(), (size_t)ws_bytes, stream),
              "spice_preference_loss");
-    return std::make_tuple(total, rewards, weight, stats);
+    if (!want_grad) return {total, rewards, weight, stats};
+    Tensor grad = at::empty(logits.sizes(), logits.options());
+    check_rc(spice_token_logprobs_grad(&v.x, &v.y, (float)temperature, stats_p, weight_p, 1, 0, (float)grad_scale, nullptr, 0,
+                                       v.last ? 1 : 0, grad.data_ptr(), stream),
+             "spice_token_logprobs_grad");
+    return {total, rewards, grad};
 }
 
-// (out4, logp, grad, stats, weight): the last three without elements where they are not wanted
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor &logits, const Tensor &labels, const Tensor &old_logprobs,
+// (out4, logp[, grad[, stats, weight]])
+std::vector<Tensor> policy_loss(const Tensor &logits, const Tensor &labels, const Tensor &old_logprobs,
                                                const Tensor &advantages, const c10::optional<Tensor> &ref_logprobs,
                                                int64_t class_dim, double temperature, int64_t ignore_index, double clip_low,
                                                double clip_high, double kl_weight, int64_t reduction, bool want_grad,
@@ -1051,9 +1071,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor &log
     c10::DeviceGuard guard(logits.device());
     const auto f32 = logits.options().dtype(at::kFloat);
     Tensor out4 = at::empty({4}, f32), logp = at::empty(labels.sizes(), f32), ws = loss_workspace(v, f32);
-    Tensor none = at::empty({0}, f32), grad = want_grad ? at::empty(logits.sizes(), logits.options()) : none;
+    Tensor grad, stats, weight;
+    if (want_grad) grad = at::empty(logits.sizes(), logits.options());
     want_weight = want_weight && want_grad;
-    Tensor stats = want_weight ? stats_for(labels, f32) : none, weight = want_weight ? at::empty(labels.sizes(), f32) : none;
+    if (want_weight) {
+        stats = stats_for(labels, f32);
+        weight = at::empty(labels.sizes(), f32);
+    }
     spice_policy_params p;
     p.temperature = (float)temperature;
     p.clip_low = (float)clip_low;
@@ -1068,56 +1092,68 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor &log
                                want_weight ? weight.data_ptr<float>() : nullptr, v.last ? 1 : 0,
                                want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), current_stream(logits)),
              "spice_policy_loss");
-    return std::make_tuple(out4, logp, grad, stats, weight);
+    if (want_weight) return {out4, logp, grad, stats, weight};
+    if (want_grad) return {out4, logp, grad};
+    return {out4, logp};
 }
 
 // ---- (10) gradient norm, clipping, Adam ---------------------------------------------------------
 
-struct TensorTable {
-    std::vector<void *> p;
-    int32_t code;
-};
+using TensorList = c10::List<Tensor>;
 
-// Device pointers of tensors that are walked in memory order: any strides without gaps.
-TensorTable table_of(const std::vector<Tensor> &ts, const char *name, const Tensor &like, at::ScalarType type) {
-    TensorTable t;
-    t.code = type == at::kFloat ? 0 : type == at::kHalf ? 1 : 2;
-    t.p.reserve(ts.size());
-    for (const Tensor &x : ts) {
-        TORCH_CHECK(x.is_cuda(), name, " is on ", x.device(),
-                    "; the MI355X path has no CPU implementation (move the tensor to a HIP device)");
-        TORCH_CHECK_TYPE(x.scalar_type() == type, name, " must be ", type, ", got ", x.scalar_type());
-        check_same_device(like, x, name);
-        TORCH_CHECK_VALUE(x.is_non_overlapping_and_dense(), name, " must be dense (contiguous in some order of its axes)");
-        t.p.push_back(x.data_ptr());
-    }
-    return t;
-}
+int32_t type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : 2; }
 
 at::ScalarType float_type(const Tensor &t, const char *name) {
     logits_code(t, name);
     return t.scalar_type();
 }
 
+// A list of tensors that are walked in memory order (any strides without gaps), as the C ABI takes it.
+struct TensorTable {
+    std::vector<void *> p;
+    std::vector<int64_t> n;
+};
+
+void fill_table(TensorTable &t, const TensorList &ts, const char *name, const Tensor &like, at::ScalarType type) {
+    const c10::Device device = like.device();
+    t.p.reserve(ts.size());
+    t.n.reserve(ts.size());
+    for (size_t i = 0; i < ts.size(); ++i) {
+        const Tensor &x = ts[i];
+        TORCH_CHECK(x.is_cuda(), name, " is on ", x.device(),
+                    "; the MI355X path has no CPU implementation (move the tensor to a HIP device)");
+        TORCH_CHECK_TYPE(x.scalar_type() == type, name, " must be ", type, ", got ", x.scalar_type());
+        TORCH_CHECK(x.device() == device, name, " is on ", x.device(), ", expected ", device);
+        TORCH_CHECK_VALUE(x.is_contiguous() || x.is_non_overlapping_and_dense(), name,
+                          " must be dense (contiguous in some order of its axes)");
+        t.p.push_back(x.data_ptr());
+        t.n.push_back(x.numel());
+    }
+}
+
 // Tensor for tensor the same shape and the same order in memory.
-void check_alike(const std::vector<Tensor> &a, const std::vector<Tensor> &b, const char *name) {
+void check_alike(const TensorList &a, const TensorList &b, const char *name) {
     TORCH_CHECK_VALUE(a.size() == b.size(), name, ": ", b.size(), " tensors, expected ", a.size());
-    for (size_t i = 0; i < a.size(); ++i)
-        TORCH_CHECK_VALUE(a[i].sizes() == b[i].sizes() && (a[i].strides() == b[i].strides() || a[i].numel() <= 1), name, "[", i,
-                          "] must have the shape and strides of its counterpart");
+    for (size_t i = 0; i < a.size(); ++i) {
+        const Tensor &x = a[i], &y = b[i];
+        TORCH_CHECK_VALUE(x.sizes() == y.sizes() && ((x.is_contiguous() && y.is_contiguous()) || x.strides() == y.strides() || x.numel() <= 1),
+                          name, "[", i, "] must have the shape and strides of its counterpart");
+    }
 }
 
 using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
 
-void add_range(const Tensor &t, Ranges &ranges) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.numel()) ranges.emplace_back(p, p + (uintptr_t)t.numel() * t.element_size());
+void add_ranges(const TensorTable &t, int64_t bytes, Ranges &ranges) {
+    for (size_t i = 0; i < t.p.size(); ++i) {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(t.p[i]);
+        if (t.n[i]) ranges.emplace_back(p, p + (uintptr_t)(t.n[i] * bytes));
+    }
 }
 
 // Tensors that a launch writes may not share memory with each other nor with what it reads: every workgroup writes its
-// own part, in no order.  `writes` is sorted here.
+// own part, in no order.  `writes` is sorted here (lists cut from one buffer come sorted already).
 void check_apart(Ranges &writes, const Ranges &reads, const char *what) {
-    std::sort(writes.begin(), writes.end());
+    if (!std::is_sorted(writes.begin(), writes.end())) std::sort(writes.begin(), writes.end());
     for (size_t i = 1; i < writes.size(); ++i)
         TORCH_CHECK_VALUE(writes[i].first >= writes[i - 1].second, what, ": two of the written tensors share memory");
     for (const auto &r : reads) {
@@ -1127,78 +1163,94 @@ void check_apart(Ranges &writes, const Ranges &reads, const char *what) {
     }
 }
 
-std::vector<int64_t> counts_of(const std::vector<Tensor> &ts) {
-    std::vector<int64_t> n;
-    n.reserve(ts.size());
-    for (const Tensor &t : ts) n.push_back(t.numel());
-    return n;
-}
-
 // Written behind autograd's back: the tensors' versions say so.
-void written(const std::vector<Tensor> &ts) {
-    for (const Tensor &t : ts)
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const TensorList &ts) {
+    for (size_t i = 0; i < ts.size(); ++i) written(ts[i]);
 }
 
 Tensor norm_workspace(const std::vector<int64_t> &n, const Tensor &like) {
     return at::empty({(int64_t)spice_grad_norm_workspace_bytes(n.data(), (int32_t)n.size())}, like.options().dtype(at::kByte));
 }
 
-Tensor grad_norm(std::vector<Tensor> grads, double max_norm, bool inf) {
+Tensor grad_norm(const TensorList &grads, double max_norm, bool inf) {
     TORCH_CHECK_VALUE(!grads.empty(), "grad_norm: no tensors");
-    const at::ScalarType type = float_type(grads[0], "grads");
-    TensorTable g = table_of(grads, "grads", grads[0], type);
+    const Tensor &like = grads[0];
+    const at::ScalarType type = float_type(like, "grads");
+    TensorTable g;
+    fill_table(g, grads, "grads", like, type);
     TORCH_CHECK_VALUE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
-    const std::vector<int64_t> n = counts_of(grads);
-    c10::DeviceGuard guard(grads[0].device());
-    Tensor record = at::empty({4}, grads[0].options().dtype(at::kFloat)), ws = norm_workspace(n, grads[0]);
-    check_rc(spice_grad_norm(g.p.data(), n.data(), (int32_t)n.size(), g.code, inf ? SPICE_NORM_INF : SPICE_NORM_L2,
-                             (float)max_norm, record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(),
-                             current_stream(grads[0])),
+    c10::DeviceGuard guard(like.device());
+    Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws = norm_workspace(g.n, like);
+    check_rc(spice_grad_norm(g.p.data(), g.n.data(), (int32_t)g.n.size(), type_code(type), inf ? SPICE_NORM_INF : SPICE_NORM_L2,
+                             (float)max_norm, record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
              "spice_grad_norm");
     return record;
 }
 
-void grad_clip(std::vector<Tensor> grads, std::vector<Tensor> out, const Tensor &record) {
+// The record of grad_norm, or one taken before; the gradients clipped into `out` (which may be `grads`).
+Tensor grad_clip(const TensorList &grads, const TensorList &out, double max_norm, bool inf, const c10::optional<Tensor> &record_in) {
     TORCH_CHECK_VALUE(!grads.empty(), "grad_clip: no tensors");
     TORCH_CHECK_VALUE(out.size() == grads.size(), "out: ", out.size(), " tensors, expected ", grads.size());
-    const at::ScalarType type = float_type(grads[0], "grads"), out_type = float_type(out[0], "out");
+    TORCH_CHECK_VALUE(max_norm >= 0.0, "grad_clip: max_norm must not be negative");
+    const Tensor &like = grads[0];
+    const at::ScalarType type = float_type(like, "grads"), out_type = float_type(out[0], "out");
     TORCH_CHECK_TYPE(out_type == type || out_type == at::kFloat, "out must be of the gradients' type or fp32, got ", out_type);
-    TensorTable g = table_of(grads, "grads", grads[0], type), o = table_of(out, "out", grads[0], out_type);
+    TensorTable g, o;
+    fill_table(g, grads, "grads", like, type);
+    fill_table(o, out, "out", like, out_type);
     check_alike(grads, out, "out");
-    check_dev(record, "record", at::kFloat);
-    check_same_device(grads[0], record, "record");
-    TORCH_CHECK_VALUE(record.numel() == 4, "record must be grad_norm's");
     Ranges writes, reads;
-    for (size_t i = 0; i < grads.size(); ++i) {   // a gradient may be its own output and nothing else's
-        add_range(out[i], writes);
-        if (grads[i].data_ptr() != out[i].data_ptr() || type != out_type) add_range(grads[i], reads);
+    add_ranges(o, c10::elementSize(out_type), writes);
+    for (size_t i = 0; i < g.p.size(); ++i) {     // a gradient may be its own output and nothing else's
+        const uintptr_t p = reinterpret_cast<uintptr_t>(g.p[i]);
+        if (g.n[i] && (g.p[i] != o.p[i] || type != out_type)) reads.emplace_back(p, p + (uintptr_t)(g.n[i] * c10::elementSize(type)));
     }
     check_apart(writes, reads, "grad_clip");
-    const std::vector<int64_t> n = counts_of(grads);
-    c10::DeviceGuard guard(grads[0].device());
-    check_rc(spice_grad_clip(g.p.data(), g.code, o.p.data(), o.code, n.data(), (int32_t)n.size(), record.data_ptr<float>(),
-                             current_stream(grads[0])),
-             "spice_grad_clip");
+    c10::DeviceGuard guard(like.device());
+    Tensor record;
+    if (record_in.has_value()) {
+        record = *record_in;
+        check_dev(record, "record", at::kFloat);
+        check_same_device(like, record, "record");
+        TORCH_CHECK_VALUE(record.numel() == 4, "record must be grad_norm's");
+        check_rc(spice_grad_clip(g.p.data(), type_code(type), o.p.data(), type_code(out_type), g.n.data(), (int32_t)g.n.size(),
+                                 record.data_ptr<float>(), current_stream(like)),
+                 "spice_grad_clip");
+    } else {
+        record = at::empty({4}, like.options().dtype(at::kFloat));
+        Tensor ws = norm_workspace(g.n, like);
+        check_rc(spice_grad_norm_clip(g.p.data(), type_code(type), o.p.data(), type_code(out_type), g.n.data(), (int32_t)g.n.size(),
+                                      inf ? SPICE_NORM_INF : SPICE_NORM_L2, (float)max_norm, record.data_ptr<float>(), ws.data_ptr(),
+                                      (size_t)ws.numel(), current_stream(like)),
+                 "spice_grad_norm_clip");
+    }
     written(out);
+    return record;
 }
 
-Tensor adam_step(std::vector<Tensor> params, std::vector<Tensor> grads, std::vector<Tensor> exp_avg, std::vector<Tensor> exp_avg_sq,
-                 c10::optional<Tensor> step, int64_t host_step, double lr, double beta1, double beta2, double eps,
+Tensor adam_step(const TensorList &params, const TensorList &grads, const TensorList &exp_avg, const TensorList &exp_avg_sq,
+                 const c10::optional<Tensor> &step, int64_t host_step, double lr, double beta1, double beta2, double eps,
                  double weight_decay, bool decoupled, double max_norm, const c10::optional<Tensor> &norm) {
     TORCH_CHECK_VALUE(!params.empty(), "adam_step: no tensors");
-    const at::ScalarType type = float_type(params[0], "params");
     const Tensor &like = params[0];
-    TensorTable p = table_of(params, "params", like, type), g = table_of(grads, "grads", like, type),
-                m = table_of(exp_avg, "exp_avg", like, at::kFloat), v = table_of(exp_avg_sq, "exp_avg_sq", like, at::kFloat);
+    const at::ScalarType type = float_type(like, "params");
+    TensorTable p, g, m, v;
+    fill_table(p, params, "params", like, type);
+    fill_table(g, grads, "grads", like, type);
+    fill_table(m, exp_avg, "exp_avg", like, at::kFloat);
+    fill_table(v, exp_avg_sq, "exp_avg_sq", like, at::kFloat);
     check_alike(params, grads, "grads");
     check_alike(params, exp_avg, "exp_avg");
     check_alike(params, exp_avg_sq, "exp_avg_sq");
     Ranges writes, reads;
-    for (size_t i = 0; i < params.size(); ++i) {
-        for (const Tensor *t : {&params[i], &exp_avg[i], &exp_avg_sq[i]}) add_range(*t, writes);
-        add_range(grads[i], reads);
-    }
+    writes.reserve(3 * p.p.size());
+    add_ranges(p, c10::elementSize(type), writes);
+    add_ranges(m, 4, writes);
+    add_ranges(v, 4, writes);
+    add_ranges(g, c10::elementSize(type), reads);
     check_apart(writes, reads, "adam_step");
     int64_t *device_step = nullptr;
     if (step.has_value()) {
@@ -1207,12 +1259,13 @@ Tensor adam_step(std::vector<Tensor> params, std::vector<Tensor> grads, std::vec
         TORCH_CHECK_VALUE(step->numel() == 1, "step must hold one count");
         device_step = step->data_ptr<int64_t>();
     }
-    const std::vector<int64_t> n = counts_of(params);
     TORCH_CHECK_VALUE(lr >= 0.0 && beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 &&
                           weight_decay >= 0.0 && (step.has_value() || host_step >= 1),
                       "adam_step: lr, eps and weight_decay must not be negative, the betas lie in [0, 1), steps count from 1");
     c10::DeviceGuard guard(like.device());
-    Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws = norm_workspace(n, like);
+    Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws;
+    const bool take = max_norm >= 0.0 && !norm.has_value();
+    if (take) ws = norm_workspace(p.n, like);
     spice_adam_params a;
     a.lr = lr;
     a.beta1 = beta1;
@@ -1222,14 +1275,14 @@ Tensor adam_step(std::vector<Tensor> params, std::vector<Tensor> grads, std::vec
     a.step = host_step;
     a.max_norm = (float)max_norm;
     a.decoupled = decoupled ? 1 : 0;
-    check_rc(spice_adam_step(p.p.data(), g.p.data(), m.p.data(), v.p.data(), n.data(), (int32_t)n.size(), p.code, &a,
-                             one_float(norm, "norm", like), device_step, record.data_ptr<float>(), ws.data_ptr(),
-                             (size_t)ws.numel(), current_stream(like)),
+    check_rc(spice_adam_step(p.p.data(), g.p.data(), m.p.data(), v.p.data(), p.n.data(), (int32_t)p.n.size(), type_code(type), &a,
+                             one_float(norm, "norm", like), device_step, record.data_ptr<float>(), take ? ws.data_ptr() : nullptr,
+                             take ? (size_t)ws.numel() : 0, current_stream(like)),
              "spice_adam_step");
     written(params);
     written(exp_avg);
     written(exp_avg_sq);
-    if (step.has_value()) written({*step});
+    if (step.has_value()) written(*step);
     return record;
 }
 
@@ -1290,12 +1343,12 @@ TORCH_LIBRARY(spice, m) {
     m.def("token_logprobs_grad(Tensor logits, Tensor labels, Tensor stats, Tensor weight, int class_dim, float temperature, "
           "int ignore_index, float scale, Tensor? device_scale, Tensor(a!)? out) -> Tensor(a!)", &token_logprobs_grad);
     m.def("preference_loss(Tensor logits, Tensor labels, Tensor ref_logprobs, int class_dim, float temperature, int ignore_index, "
-          "float beta, float smoothing, int loss_type, bool average) -> (Tensor, Tensor, Tensor, Tensor)", &preference_loss);
+          "float beta, float smoothing, int loss_type, bool average, bool want_grad, float grad_scale) -> Tensor[]", &preference_loss);
     m.def("policy_loss(Tensor logits, Tensor labels, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, int class_dim, "
           "float temperature, int ignore_index, float clip_low, float clip_high, float kl_weight, int reduction, bool want_grad, "
-          "float grad_scale, bool want_weight) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", &policy_loss);
+          "float grad_scale, bool want_weight) -> Tensor[]", &policy_loss);
     m.def("grad_norm(Tensor[] grads, float max_norm, bool inf) -> Tensor", &grad_norm);
-    m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, Tensor record) -> ()", &grad_clip);
+    m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, float max_norm, bool inf, Tensor? record) -> Tensor", &grad_clip);
     m.def("adam_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)? step, "
           "int host_step, float lr, float beta1, float beta2, float eps, float weight_decay, bool decoupled, float max_norm, "
           "Tensor? norm) -> Tensor", &adam_step);

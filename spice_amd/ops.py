@@ -924,13 +924,9 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     h = R_better - R_worse: total = mean of -log sigmoid(beta h) (label_smoothing e: (1-e) of it and e of the swapped
     pair's), or of (h - 1/(2 beta))^2 with loss_type="ipo"; rewards = beta R.  ref_logprobs: the frozen reference's
     token_logprobs for the same labels.  grad = grad_scale * d total / d logits.  logits and labels as token_logprobs."""
-    f = spice_ops()
-    total, rewards, weight, stats = f.preference_loss(logits, labels, ref_logprobs, class_dim, temperature, ignore_index, beta,
-                                                      label_smoothing, _choice(_PREFERENCE_TYPES, loss_type, "loss_type"), average)
-    if not want_grad:
-        return total, rewards, None
-    return total, rewards, f.token_logprobs_grad(logits, labels, stats, weight, class_dim, temperature, ignore_index,
-                                                 grad_scale, None, None)
+    got = spice_ops().preference_loss(logits, labels, ref_logprobs, class_dim, temperature, ignore_index, beta, label_smoothing,
+                                      _choice(_PREFERENCE_TYPES, loss_type, "loss_type"), average, want_grad, grad_scale)
+    return got[0], got[1], got[2] if want_grad else None
 
 
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
@@ -943,11 +939,10 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logprobs: torch.
     (0 without ref_logprobs), total = surrogate + kl_weight * kl, averaged over all counted positions ("token") or as the
     mean over sequences of each one's mean ("sequence"; a sequence without counted positions adds 0).  advantages fp32, one
     a sequence or one a position.  grad = grad_scale * d total / d logits, taken in the same pass over the logits.  logits and labels as token_logprobs."""
-    out4, logp, grad, _, _ = spice_ops().policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs, class_dim,
-                                                     temperature, ignore_index, clip_low, clip_high, kl_weight,
-                                                     _choice(_POLICY_REDUCTIONS, reduction, "reduction"), want_grad,
-                                                     grad_scale, False)
-    return out4, logp, grad if want_grad else None
+    got = spice_ops().policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs, class_dim, temperature, ignore_index,
+                                  clip_low, clip_high, kl_weight, _choice(_POLICY_REDUCTIONS, reduction, "reduction"), want_grad,
+                                  grad_scale, False)
+    return got[0], got[1], got[2] if want_grad else None
 
 
 # --------------------------------------------------------------------------------------
@@ -975,11 +970,12 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, norm_type: fl
     stay in place.  A NaN norm makes the gradients NaN; with error_if_nonfinite it raises first (a host synchronisation).
     Tensors as grad_norm; no two of the written ones may share memory."""
     f = spice_ops()
-    record = f.grad_norm(grads, float(max_norm), _norm_inf(norm_type))
-    if error_if_nonfinite and not bool(torch.isfinite(record[0])):
-        raise RuntimeError(f"the gradient norm of order {norm_type} is not finite: the gradients are left as they are")
-    f.grad_clip(grads, grads if out is None else out, record)
-    return record[0]
+    record = None
+    if error_if_nonfinite:
+        record = f.grad_norm(grads, float(max_norm), _norm_inf(norm_type))
+        if not bool(torch.isfinite(record[0])):
+            raise RuntimeError(f"the gradient norm of order {norm_type} is not finite: the gradients are left as they are")
+    return f.grad_clip(grads, grads if out is None else out, float(max_norm), _norm_inf(norm_type), record)[0]
 
 
 def adam_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],

@@ -190,7 +190,7 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, how, opts):
         total, rewards, weight, stats = ops.spice_ops().preference_loss(
-            logits.detach(), labels, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts)
+            logits.detach(), labels, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts, False, 1.0)
         ctx.how = how
         ctx.save_for_backward(logits, labels, stats, weight)
         ctx.mark_non_differentiable(rewards)
@@ -210,12 +210,12 @@ class _Policy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, labels, old, advantages, ref, how, opts, want):
-        out4, logp, grad, stats, weight = ops.spice_ops().policy_loss(
+        out4, logp, *saved = ops.spice_ops().policy_loss(
             logits.detach(), labels, old, advantages, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts,
             want, 1.0, want)
-        ctx.how = how
-        ctx.grad = grad if want else None
-        ctx.save_for_backward(logits, labels, stats, weight)
+        if want:
+            ctx.how, ctx.grad = how, saved[0]
+            ctx.save_for_backward(logits, labels, *saved[1:])
         parts = out4.unbind()
         total, rest = parts[0].clone(), [p.clone() for p in parts[1:]]
         ctx.mark_non_differentiable(logp, *rest)
