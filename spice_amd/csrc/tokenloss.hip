@@ -539,7 +539,8 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
 }
 
 // weight * d logp / d x of rows whose maximum and sum are known: a workgroup takes kGradVecs vectors a lane of one row.
-constexpr int kGradVecs = 4;
+// ([8,1024,32000] bf16, loss + gradient: 241 us with 1, 181 with 2, 188 with 4 and 8)
+constexpr int kGradVecs = 2;
 
 template <typename T>
 __global__ __launch_bounds__(kTokThreads) void tok_row_grad_kernel(TokArgs a, int64_t pieces) {
