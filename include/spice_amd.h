@@ -589,9 +589,9 @@ typedef struct spice_preference_params {
  * logp - ref_logp, h_i = R_i - R_{n/2+i}, total = mean over pairs of the loss of h_i; rewards[n] = beta * R_n.
  * weight[n] = d total / d logp of every counted position of sequence n: spice_token_logprobs_grad(weight, 1, 0) on the
  * stats written here is the gradient.  ref_logp [n,l] fp32 (0 or anything finite where ignored: it is not read there).
- * Sums in fp64, in a fixed order. */
+ * Log ratios and sums in fp64, in a fixed order.  ratio [n,l]: scratch. */
 int spice_preference_loss(const spice_logits *logits, const spice_labels *labels, const float *ref_logp,
-                          const spice_preference_params *params, float *total, float *rewards, float *weight, float *logp,
+                          const spice_preference_params *params, float *total, float *rewards, float *weight, float *ratio,
                           float *stats, void *workspace, size_t workspace_bytes, void *stream);
 
 #define SPICE_POLICY_TOKEN 0    /* mean over all counted positions */
