@@ -327,7 +327,9 @@ def _own(state):
         return [logp, ops.token_logprobs_grad(logits, labels, lse, state["weight"], temperature=case["temperature"], **how)]
     if case["kind"] == "preference":
         return list(ops.preference_loss(logits, labels, state["ref"], beta=case["beta"],
-                                        label_smoothing=case["smoothing"] if case["loss"] == "sigmoid" else 0.0, loss_type=case["loss"], average=case["average"], want_grad=True, grad_scale=case["scale"], **how))
+                                        label_smoothing=case["smoothing"] if case["loss"] == "sigmoid" else 0.0,
+                                        loss_type=case["loss"], average=case["average"], want_grad=True,
+                                        grad_scale=case["scale"], **how))
     return list(ops.policy_loss(logits, labels, state["old"], state["advantages"],
                                 ref_logprobs=state["ref"] if case["kl"] else None, clip_low=0.2, clip_high=0.25,
                                 kl_weight=case["kl"], reduction=case["reduction"], temperature=case["temperature"],
