@@ -80,7 +80,11 @@ __device__ __forceinline__ double log_of(float s) {
 
 // A label's log-probability from its distance to the maximum and the sum, in fp64: a sequence's log ratio is a small
 // difference of thousands of them, and rounding each to fp32 (2^-22 at 4 to 8) would show in it.
-__device__ __forceinline__ double logp_of(float d, float s, Temper t) { return (double)d * t.exact_inv - log_of(s); }
+__device__ __forceinline__ double logp_of(float d, double s, Temper t) {
+    const float near = (float)s;
+    const double rest = near > 0.f && near < INFINITY ? (s - (double)near) / s : 0.0;
+    return (double)d * t.exact_inv - (log_of(near) + rest);
+}
 
 // What a position's label says.
 enum { kCounted = 0, kIgnored = 1, kBad = 2 };
@@ -95,31 +99,40 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f
 // place holder 0 may lie far above `to`).
 __device__ __forceinline__ float rescale(float m, float to, Temper t) { return m == -INFINITY ? 0.f : exp_of(m - to, t); }
 
-// (m, s) of the workgroup from every thread's running maximum and sum; in every thread afterwards.
+// The sum of exponentials of a row beyond fp32's precision: what the logarithm is taken of, and its fp32 value.
+__device__ __forceinline__ double wide_sum(double v, int lanes) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        if (o < lanes) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+// (m, s) of the workgroup from every thread's running maximum and sum; in every thread afterwards.  The threads' sums are
+// added up in fp64: their own roundings average out over the threads, a last few additions' would not.
 template <int THREADS>
-__device__ __forceinline__ void fold_max_sum(float &m, float &s, Temper t, float *lds) {
+__device__ __forceinline__ double fold_max_sum(float &m, float s, Temper t, double *lds) {
     constexpr int waves = THREADS / kWave;
     float all = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-    s *= rescale(m, all, t);
-    s = wave_sum(s);
+    double sum = wide_sum((double)(s * rescale(m, all, t)), kWave);
     if (waves > 1) {
         __syncthreads();   // (the last fold's reads)
         if ((threadIdx.x & 63) == 0) {
-            lds[threadIdx.x / kWave] = all;
-            lds[waves + threadIdx.x / kWave] = s;
+            lds[threadIdx.x / kWave] = sum;
+            lds[waves + threadIdx.x / kWave] = (double)all;
         }
         __syncthreads();
-        float top = lds[0];
+        float top = (float)lds[waves];
 #pragma unroll
-        for (int w = 1; w < waves; ++w) top = fmaxf(top, lds[w]);
-        s = 0.f;
+        for (int w = 1; w < waves; ++w) top = fmaxf(top, (float)lds[waves + w]);
+        sum = 0.0;
 #pragma unroll
-        for (int w = 0; w < waves; ++w) s += lds[waves + w] * rescale(lds[w], top, t);
+        for (int w = 0; w < waves; ++w) sum += lds[w] * (double)rescale((float)lds[waves + w], top, t);
         all = top;
     }
     m = all;
+    return sum;
 }
 
 // The clipped policy loss of one position and its derivative by logp.
@@ -240,7 +253,7 @@ enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kMode
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
-    __shared__ float lds[2 * kTokThreads / kWave];
+    __shared__ double lds[2 * kTokThreads / kWave];
     __shared__ int counts[kTokThreads / kWave];
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int64_t total = a.x.n * a.x.l;
@@ -262,8 +275,9 @@ __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
                     }
                     s += exp_of(v - shift_of(m), a.t);
                 }
-                fold_max_sum<kTokThreads>(m, s, a.t, lds);
-                logp = logp_of(to_f32(x[y * a.x.sc]) - shift_of(m), s, a.t);
+                const double sum = fold_max_sum<kTokThreads>(m, s, a.t, lds);
+                logp = logp_of(to_f32(x[y * a.x.sc]) - shift_of(m), sum, a.t);
+                s = (float)sum;
             } else if (kind == kBad) {
                 logp = NAN;
             }
@@ -378,18 +392,16 @@ __device__ __forceinline__ void grad_of(float (&v)[K], float m, float each, floa
 
 // (m, s) of LANES neighbouring lanes; LANES > 64: of the workgroup.
 template <int LANES>
-__device__ __forceinline__ void fold_row(float &m, float &s, Temper t, float *lds) {
+__device__ __forceinline__ double fold_row(float &m, float s, Temper t, double *lds) {
     if (LANES <= kWave) {
         float all = m;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-        s *= rescale(m, all, t);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
+        const double sum = wide_sum((double)(s * rescale(m, all, t)), LANES);
         m = all;
-    } else {
-        fold_max_sum<LANES>(m, s, t, lds);
+        return sum;
     }
+    return fold_max_sum<LANES>(m, s, t, lds);
 }
 
 // The packed row is all that is kept from one phase to the next: unpacked values that the compiler would carry along
@@ -408,7 +420,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     constexpr int kBlock = LANES < kTokThreads ? kTokThreads : LANES;
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad, kStats = MODE == kModeGrad;
     constexpr bool kLong = LANES >= kWave;     // rows of many lines each, read and stored past the caches
-    __shared__ float lds[2 * kBlock / kWave];
+    __shared__ double lds[2 * kBlock / kWave];
     __shared__ int counts[kBlock / kWave];
     if (kStats && a.unless_one && *a.scale == 1.f) return;
     float share = 0.f;
@@ -470,8 +482,9 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
 #pragma unroll
                     for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
                 }
-            fold_row<LANES>(m, s, a.t, lds);
-            logp = logp_of(xl - shift_of(m), s, a.t);
+            const double sum = fold_row<LANES>(m, s, a.t, lds);
+            logp = logp_of(xl - shift_of(m), sum, a.t);
+            s = (float)sum;
         }
     }
     if (!kStats && lane == 0) leave_logp(a, at, logp, m, s, ref);
@@ -511,7 +524,7 @@ template <typename T, int MODE>
 __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
     constexpr int K = vec_elements<T>(), kBlock = 1024, kStep = 4;
     constexpr bool kGrad = MODE == kModePolicyGrad;
-    __shared__ float lds[2 * kBlock / kWave];
+    __shared__ double lds[2 * kBlock / kWave];
     __shared__ int counts[kBlock / kWave];
     const int64_t total = a.x.n * a.x.l;
     const int32_t classes = (int32_t)a.x.c;
@@ -554,8 +567,9 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
                         for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
                     }
             }
-            fold_row<kBlock>(m, s, a.t, lds);
-            logp = logp_of(to_f32(x[y]) - shift_of(m), s, a.t);
+            const double sum = fold_row<kBlock>(m, s, a.t, lds);
+            logp = logp_of(to_f32(x[y]) - shift_of(m), sum, a.t);
+            s = (float)sum;
         }
         if (threadIdx.x == 0) leave_logp(a, at, logp, m, s, ref);
         if (kGrad) {
@@ -672,6 +686,29 @@ __device__ __forceinline__ typename GroupOf<T, VEC>::type grouped(const float (&
     }
 }
 
+// A group at any element's address.
+template <typename T, int VEC>
+struct __attribute__((packed, aligned(sizeof(T)))) GroupAt { typename GroupOf<T, VEC>::type v; };
+
+// ONCE: see read_vec.
+template <bool ONCE, typename T, int VEC>
+__device__ __forceinline__ typename GroupOf<T, VEC>::type read_group(const T *p) {
+    const GroupAt<T, VEC> *at = reinterpret_cast<const GroupAt<T, VEC> *>(p);
+    return ONCE ? __builtin_nontemporal_load(&at->v) : at->v;
+}
+
+// Positions from `from` on of a group's gradient (the ones in front of it are another lane's).
+template <typename T, int VEC>
+__device__ __forceinline__ void store_group(T *p, int from, const float (&v)[VEC]) {
+    if (from == 0) {
+        __builtin_nontemporal_store(grouped<T, VEC>(v), &reinterpret_cast<GroupAt<T, VEC> *>(p)->v);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+        if (k >= from) p[k] = (T)v[k];
+}
+
 // As in the row kernel: packed logits from phase to phase.
 template <typename G, int N>
 __device__ __forceinline__ void forget_groups(G (&raw)[N]) {
@@ -697,19 +734,19 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int32_t classes = (int32_t)a.x.c;
     const int64_t item = first + blockIdx.x, n = item / tiles;
-    const int64_t l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
+    int64_t l0 = ((item - n * tiles) * kTokThreads + threadIdx.x) * VEC;
+    const bool live = l0 < a.x.l;
+    const int dup = live && l0 + VEC > a.x.l ? (int)(l0 + VEC - a.x.l) : 0;   // the last group reaches back into the one before
+    l0 -= dup;
     float share = 0.f;
     if (MODE == kModePolicyGrad) share = a.share ? a.share[n] : share_here<kTokThreads>(a, n, counts);
     double sums[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) sums[k] = 0.0;
-    if (l0 < a.x.l) {
+    if (live) {
         const T *x = (const T *)a.x.x + n * a.x.sn + l0 * a.x.sl;
         const int64_t at = n * a.x.l + l0;
-        const auto plane = [&](int32_t c) {
-            const G *p = reinterpret_cast<const G *>(x + (int64_t)c * a.x.sc);
-            return kOnce ? __builtin_nontemporal_load(p) : *p;
-        };
+        const auto plane = [&](int32_t c) { return read_group<kOnce, T, VEC>(x + (int64_t)c * a.x.sc); };
         int32_t y[VEC];         // the label, or -1
         int kind[VEC];
         bool any = false;
@@ -804,21 +841,23 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
             const int64_t l = l0 + k;
             each[k] = 0.f;
             if (!kStats) {
-                const double logp = kind[k] == kCounted ? logp_of(xl[k] - shift_of(m[k]), s[k], a.t) : kind[k] == kBad ? NAN : 0.0;
-                leave_logp(a, at + k, logp, m[k], s[k], 0.f);
-                if (MODE == kModePreference && kind[k] != kIgnored) {
+                const double logp = kind[k] == kCounted ? logp_of(xl[k] - shift_of(m[k]), (double)s[k], a.t) : kind[k] == kBad ? NAN : 0.0;
+                if (k >= dup) leave_logp(a, at + k, logp, m[k], s[k], 0.f);
+                if (MODE == kModePreference && kind[k] != kIgnored && k >= dup) {
                     sums[0] += logp - (double)a.ref[at + k];
                     sums[1] += 1.0;
                 }
                 if ((MODE == kModePolicy || MODE == kModePolicyGrad) && kind[k] != kIgnored) {
                     const PolicyTerm t = policy_term(a.policy, in[k], (float)logp);
-                    sums[0] += t.surrogate;
-                    sums[1] += t.far;
-                    sums[2 % K] += t.over ? 1.0 : 0.0;
-                    sums[3 % K] += 1.0;
+                    if (k >= dup) {
+                        sums[0] += t.surrogate;
+                        sums[1] += t.far;
+                        sums[2 % K] += t.over ? 1.0 : 0.0;
+                        sums[3 % K] += 1.0;
+                    }
                     w[k] = kind[k] == kBad ? NAN : t.dlogp * share;
                 }
-                if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at + k] = w[k];
+                if (MODE == kModePolicyGrad && a.weight_out && k >= dup) a.weight_out[at + k] = w[k];
             } else if (kind[k] == kCounted) {
                 w[k] = a.weight[n * a.w_sn + l * a.w_sl];
             } else {
@@ -838,7 +877,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
                     const float e = each[k] * exp_of(v[k] - shift_of(m[k]), a.t);
                     v[k] = kind[k] == kCounted ? (y[k] == c ? e + w[k] : e) : each[k];
                 }
-                __builtin_nontemporal_store(grouped<T, VEC>(v), reinterpret_cast<G *>(g + (int64_t)c * a.g_sc));
+                store_group<T, VEC>(g + (int64_t)c * a.g_sc, dup, v);
             };
             if (CREG > 0) {
                 forget_groups(raw);
@@ -887,7 +926,10 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
     __shared__ int counts[kTokThreads / kWave];
     if (MODE == kModeGrad && a.unless_one && *a.scale == 1.f) return;
     const int32_t classes = (int32_t)a.x.c;
-    const int64_t item = first + blockIdx.x, n = item / tiles, start = (item - n * tiles) * kSplitTile;
+    // the last tile reaches back into the one before it, whose positions (the first `dup`) are that one's to write
+    const int64_t item = first + blockIdx.x, n = item / tiles, tile = (item - n * tiles) * kSplitTile;
+    const int dup = a.x.l >= kSplitTile && tile + kSplitTile > a.x.l ? (int)(tile + kSplitTile - a.x.l) : 0;
+    const int64_t start = tile - dup;
     const int32_t group = threadIdx.x / RUN, pos = (threadIdx.x % RUN) * VEC;
     const int64_t l0 = start + pos;
     const bool live = l0 < a.x.l;
@@ -911,10 +953,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
         any |= y[k] >= 0;
     }
     const T *x = (const T *)a.x.x + n * a.x.sn + l0 * a.x.sl;
-    const auto plane = [&](int32_t c) {
-        const G *p = reinterpret_cast<const G *>(x + (int64_t)c * a.x.sc);
-        return kOnce ? __builtin_nontemporal_load(p) : *p;
-    };
+    const auto plane = [&](int32_t c) { return read_group<kOnce, T, VEC>(x + (int64_t)c * a.x.sc); };
     G raw[kStep];
     float v[VEC];
     if (!kStats) {
@@ -978,22 +1017,26 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
             w = yq >= 0 ? a.weight[n * a.w_sn + l * a.w_sl] : yq == -2 ? NAN : 0.f;
         } else {
             for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, part[g][q].x);
-            for (int g = 0; g < GROUPS; ++g) s += part[g][q].y * rescale(part[g][q].x, m, a.t);
-            const double exact = yq >= 0 ? logp_of(at_label[q] - shift_of(m), s, a.t) : yq == -2 ? (double)NAN : 0.0;
-            leave_logp(a, at, exact, m, s, 0.f);
-            if (MODE == kModePreference && yq != -1) {
+            double sum = 0.0;
+            for (int g = 0; g < GROUPS; ++g) sum += (double)(part[g][q].y * rescale(part[g][q].x, m, a.t));
+            s = (float)sum;
+            const double exact = yq >= 0 ? logp_of(at_label[q] - shift_of(m), sum, a.t) : yq == -2 ? (double)NAN : 0.0;
+            if (q >= dup) leave_logp(a, at, exact, m, s, 0.f);
+            if (MODE == kModePreference && yq != -1 && q >= dup) {
                 sums[0] += exact - (double)a.ref[at];
                 sums[1] += 1.0;
             }
             if ((MODE == kModePolicy || MODE == kModePolicyGrad) && yq != -1) {
                 const PolicyTerm t = policy_term(a.policy, policy_in(a.policy, at, n, l), (float)exact);
-                sums[0] += t.surrogate;
-                sums[1] += t.far;
-                sums[2 % K] += t.over ? 1.0 : 0.0;
-                sums[3 % K] += 1.0;
+                if (q >= dup) {
+                    sums[0] += t.surrogate;
+                    sums[1] += t.far;
+                    sums[2 % K] += t.over ? 1.0 : 0.0;
+                    sums[3 % K] += 1.0;
+                }
                 w = yq == -2 ? NAN : t.dlogp * share;
             }
-            if (MODE == kModePolicyGrad && a.weight_out) a.weight_out[at] = w;
+            if (MODE == kModePolicyGrad && a.weight_out && q >= dup) a.weight_out[at] = w;
         }
         if (kGrad) {
             w *= a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f);
@@ -1011,7 +1054,8 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
     }
     if (kGrad) {
         __syncthreads();
-        if (!live) return;
+        if (!live || pos + VEC <= dup) return;
+        const int from = dup > pos ? dup - pos : 0;
         T *g = (T *)a.grad + n * a.g_sn + l0 * a.g_sl;
         float m[VEC], each[VEC], w[VEC];
 #pragma unroll
@@ -1037,7 +1081,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
                         const float e = each[k] * exp_of(v[k] - m[k], a.t);
                         v[k] = y[k] >= 0 ? (y[k] == c0 + j * GROUPS ? e + w[k] : e) : each[k];
                     }
-                    __builtin_nontemporal_store(grouped<T, VEC>(v), reinterpret_cast<G *>(g + (int64_t)(c0 + j * GROUPS) * a.g_sc));
+                    store_group<T, VEC>(g + (int64_t)(c0 + j * GROUPS) * a.g_sc, from, v);
                 }
             if (HOLD > 0) break;
         }
@@ -1315,14 +1359,11 @@ int launch_rows(const TokArgs &a, hipStream_t stream) {
 // Neighbouring positions a lane of the planes kernels takes, and the most classes that one lane walks alone.
 constexpr int kPlanesVec = 4, kPlanesClasses = 32;
 
-// Whether VEC neighbouring positions of every plane can move as one aligned word.
-template <typename T>
+// Four positions a lane, at any alignment; the last group of a sequence reaches back into the one before, so there have to
+// be as many positions as a lane (or, with many classes, a workgroup) takes, or a multiple of four.
 bool planes_vec(const TokArgs &a) {
-    const int64_t bytes = kPlanesVec * (int64_t)sizeof(T);
-    const auto whole = [&](int64_t stride) { return stride * (int64_t)sizeof(T) % bytes == 0; };
-    return a.x.sl == 1 && a.x.l % kPlanesVec == 0 && whole(a.x.sc) && (a.x.n == 1 || whole(a.x.sn)) &&
-           reinterpret_cast<uintptr_t>(a.x.x) % bytes == 0 &&
-           (!a.grad || (reinterpret_cast<uintptr_t>(a.grad) % bytes == 0 && a.g_sl == 1));
+    const int64_t least = a.x.c > kPlanesClasses ? kSplitTile : kPlanesVec;
+    return a.x.l >= least || a.x.l % kPlanesVec == 0;
 }
 
 int64_t planes_tiles(int64_t l, bool vec) { return ceil_div(l, (int64_t)kTokThreads * (vec ? kPlanesVec : 1)); }
@@ -1380,7 +1421,7 @@ int launch_typed(const TokArgs &a, hipStream_t stream) {
     const int64_t total = a.x.n * a.x.l;
     const int route = route_of(a);
     if (route == kByPlanes)
-        return planes_vec<T>(a) ? launch_planes<T, kPlanesVec, MODE>(a, stream) : launch_planes<T, 1, MODE>(a, stream);
+        return planes_vec(a) ? launch_planes<T, kPlanesVec, MODE>(a, stream) : launch_planes<T, 1, MODE>(a, stream);
     // rows and any strides: the sums over positions are a pass of their own over logp
     constexpr int mode = MODE == kModePreference || MODE == kModePolicy ? kModeLogp : MODE;
     if (route == kByRows) return launch_rows<T, mode>(a, stream);
@@ -1398,10 +1439,9 @@ int launch_positions(const TokArgs &a, int32_t dtype, hipStream_t stream) {
 }
 
 // Items a sequence's partial sums come in: the planes kernel's tiles, or the chunks of the pass over logp.
-int64_t items_of(const TokArgs &a, int32_t dtype) {
+int64_t items_of(const TokArgs &a) {
     if (route_of(a) != kByPlanes) return chunks_of(a.x.l);
-    const bool vec = dtype == 0 ? planes_vec<float>(a) : dtype == 1 ? planes_vec<_Float16>(a) : planes_vec<__bf16>(a);
-    return !a.x.l ? 1 : a.x.c > kPlanesClasses ? ceil_div(a.x.l, kSplitTile) : planes_tiles(a.x.l, vec);
+    return !a.x.l ? 1 : a.x.c > kPlanesClasses ? ceil_div(a.x.l, kSplitTile) : planes_tiles(a.x.l, planes_vec(a));
 }
 
 // Partial sums of a call at most: the workgroups' of the split planes kernel, or the waves' of the folding workgroup.
@@ -1491,7 +1531,7 @@ extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *
     SumArgs sums = sums_of(a, a.part);
     int64_t ways = 0;
     if (route_of(a) == kByPlanes && x->l) {
-        sums.chunks = items_of(a, x->dtype);
+        sums.chunks = items_of(a);
     } else if (!(ways = ways_of(x->n, x->l))) {
         rc = launch_sums<kSumPreference>(sums, s);
         if (rc) return rc;
@@ -1542,7 +1582,7 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     rc = grad ? launch_positions<kModePolicyGrad>(a, x->dtype, s) : launch_positions<kModePolicy>(a, x->dtype, s);
     if (rc) return rc;
     if (planes) {
-        sums.chunks = items_of(a, x->dtype);
+        sums.chunks = items_of(a);
         ways = 0;
     } else if (!ways) {
         rc = launch_sums<kSumPolicy>(sums, s);

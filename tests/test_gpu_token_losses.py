@@ -30,6 +30,10 @@ SHAPES = [
     ("last", 1, (2,), 150001, torch.float32), ("last", 2, (700,), 5, torch.float32), ("last", 1, (130,), 64, torch.bfloat16),
     ("planes", 1, (1,), 1, torch.float32), ("planes", 2, (7, 9), 5, torch.float32), ("planes", 2, (16, 16), 21, torch.float32),
     ("planes", 3, (33,), 19, torch.bfloat16), ("planes", 2, (64, 36), 21, torch.float16), ("planes", 2, (5, 3), 150, torch.float32),
+    ("planes", 2, (12, 40), 200, torch.float32), ("planes", 1, (700,), 300, torch.bfloat16), ("planes", 2, (301,), 60, torch.float16),
+    ("planes", 1, (601,), 100, torch.float32), ("planes", 1, (129,), 33, torch.float32), ("planes", 2, (260,), 128, torch.float16),
+    ("last", 3, (50,), 31, torch.float32), ("last", 3, (50,), 127, torch.float32), ("last", 2, (33,), 255, torch.float16),
+    ("last", 2, (9,), 767, torch.float32), ("last", 2, (9,), 20479, torch.float32), ("last", 1, (2,), 86015, torch.float32),
     ("planes", 1, (9000,), 2, torch.float16), ("planes", 1, (40, 41), 64, torch.bfloat16), ("planes", 2, (6,), 3001, torch.float32),
 ]
 IDS = ["%s-%d-%s-%d-%s" % (s[0], s[1], "x".join(map(str, s[2])), s[3], str(s[4])[6:]) for s in SHAPES]
@@ -254,7 +258,8 @@ def _ratio_tol(x, want, keep, d, t, average):
 
 PAIRS = [("last", 2, (1,), 11, torch.float32), ("last", 4, (37,), 1031, torch.bfloat16), ("last", 2, (9,), 50001, torch.float16),
          ("last", 6, (5000,), 7, torch.float32), ("last", 2, (), 300, torch.float32), ("planes", 4, (24, 20), 21, torch.float32),
-         ("planes", 2, (70, 70), 5, torch.float16), ("planes", 64, (3,), 19, torch.bfloat16)]
+         ("planes", 2, (70, 70), 5, torch.float16), ("planes", 64, (3,), 19, torch.bfloat16), ("planes", 2, (30, 22), 150, torch.float32),
+         ("planes", 4, (700,), 300, torch.float16), ("last", 2, (3000,), 90, torch.float32)]
 
 
 @pytest.mark.parametrize("shape", PAIRS, ids=lambda s: "%s-%d-%s-%d" % (s[0], s[1], "x".join(map(str, s[2])), s[3]))
@@ -327,7 +332,9 @@ def test_preference_sides_and_extremes(dev):
 ROWS = [("last", 1, (1,), 9, torch.float32), ("last", 3, (41,), 1025, torch.bfloat16), ("last", 2, (7,), 50001, torch.float16),
         ("last", 2, (3,), 140001, torch.bfloat16), ("last", 5, (4500,), 6, torch.float32), ("last", 4, (), 700, torch.float32),
         ("planes", 3, (24, 20), 21, torch.float32), ("planes", 2, (70, 70), 5, torch.float16), ("planes", 40, (3,), 19, torch.bfloat16),
-        ("planes", 1, (30, 5), 100, torch.float32)]
+        ("planes", 1, (30, 5), 100, torch.float32), ("planes", 2, (30, 22), 150, torch.float32), ("planes", 4, (700,), 300, torch.float16),
+        ("last", 3, (20,), 21, torch.float32), ("last", 3, (20,), 100, torch.bfloat16), ("last", 2, (600,), 300, torch.float32),
+        ("planes", 3, (5, 7), 1000, torch.float32)]
 
 
 @pytest.mark.parametrize("shape", ROWS, ids=lambda s: "%s-%d-%s-%d" % (s[0], s[1], "x".join(map(str, s[2])), s[3]))
