@@ -74,8 +74,9 @@ __device__ __forceinline__ double log_of(float s) {
     float r = __builtin_fmaf(q, 1.f / 9.f, 1.f / 7.f);
     r = __builtin_fmaf(r, q, 1.f / 5.f);
     r = __builtin_fmaf(r, q, 1.f / 3.f);
-    const float g = t + t;
-    return (double)e * 0.69314718055994530942 + ((double)g + (double)(g * q * r));
+    // t to fp64's precision: one Newton step of the quotient
+    const double num = (double)f - 1.0, den = (double)f + 1.0, exact = (double)t + (num - (double)t * den) * (double)(1.f / (f + 1.f));
+    return (double)e * 0.69314718055994530942 + (2.0 * exact + (double)(2.f * t * q * r));
 }
 
 // A label's log-probability from its distance to the maximum and the sum, in fp64: a sequence's log ratio is a small
