@@ -543,8 +543,8 @@ int spice_conv3x3_bn_act_f16(const void *x, const void *weight9, void *y, int64_
  * With m = max_c x_c, s = sum_c exp((x_c - m) / T):
  *   logp = (x_label - m) / T - log s          (0 where the label is ignore_index)
  * A label that is neither ignore_index nor in [0, c) gives NaN: logp, the loss and
- * that position's gradient.  Positions with ignore_index are never read; their
- * gradient is zero.  ignore_index must not be a class.
+ * that position's gradient.  Nothing that belongs to a position with ignore_index is
+ * used; its gradient is zero.  ignore_index must not be a class.
  * ------------------------------------------------------------------------- */
 typedef struct spice_logits {
     const void *data;
@@ -588,7 +588,7 @@ typedef struct spice_preference_params {
 /* Sequences i < n/2 are preferred to sequences n/2 + i (n even, >= 2).  R_n = sum (or mean) over the counted positions of
  * logp - ref_logp, h_i = R_i - R_{n/2+i}, total = mean over pairs of the loss of h_i; rewards[n] = beta * R_n.
  * weight[n] = d total / d logp of every counted position of sequence n: spice_token_logprobs_grad(weight, 1, 0) on the
- * stats written here is the gradient.  ref_logp [n,l] fp32 (0 or anything finite where ignored: it is not read there).
+ * stats written here is the gradient.  ref_logp [n,l] fp32 (anything where ignored).
  * Log ratios and sums in fp64, in a fixed order.  ratio [n,l]: scratch. */
 int spice_preference_loss(const spice_logits *logits, const spice_labels *labels, const float *ref_logp,
                           const spice_preference_params *params, float *total, float *rewards, float *weight, float *ratio,

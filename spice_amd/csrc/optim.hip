@@ -80,6 +80,7 @@ __device__ __forceinline__ void put_once(V *p, const V &v) {
         __builtin_nontemporal_store(__builtin_bit_cast(unsigned long long, v), (unsigned long long *)p);
     }
 }
+
 // NaN-keeping maximum
 __device__ __forceinline__ double max_keep(double a, double b) { return (a > b || a != a) ? a : b; }
 
@@ -347,7 +348,8 @@ int for_tables(void *const *const (&ptrs)[PTRS], const int64_t (&bytes)[PTRS], c
             t.numel[t.count] = (uint32_t)n;
             t.first[t.count] = (uint32_t)items;
             items += ceil_div(n, each);
-            if (++t.count == table_entries<PTRS>()) {
+            // (an entry has 2^30 / each items at most, and a launch's threads are counted in 32 bits)
+            if (++t.count == table_entries<PTRS>() || items >= ((int64_t)1 << 22)) {
                 const int rc = launch(t, before, items);
                 if (rc) return rc;
                 before += items;

@@ -251,7 +251,6 @@ __device__ __forceinline__ float share_here(const TokArgs &a, int64_t n, int *ld
 // loss sums over positions.  PolicyGrad: the policy loss's gradient behind that.
 enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kModePolicyGrad = 4 };
 
-
 template <typename T, int MODE>
 __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
     __shared__ double lds[2 * kTokThreads / kWave];
@@ -719,10 +718,12 @@ __device__ __forceinline__ void forget_groups(G (&raw)[N]) {
     }
 }
 
-// CREG > 0: at most CREG classes, a position group's logits in registers, read once for maximum, sum and gradient;
-// CREG = 0: any number, eight planes at a time, read again for the gradient.
+// CREG > 0: at most CREG classes, a position group's logits in registers, read once for maximum, sum and gradient.
+// CREG = 0: the gradient alone, eight planes at a time.
 template <typename T, int VEC, int CREG, int MODE>
-__global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24 ? 3 : 2) void tok_planes_kernel(TokArgs a, int64_t tiles, int64_t first) {
+__global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24 ? 3 : 2) void tok_planes_kernel(TokArgs a, int64_t tiles,
+                                                                                                                int64_t first) {
+    static_assert(CREG > 0 || MODE == kModeGrad, "without registers for the classes there is only the gradient");
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
     constexpr bool kStats = MODE == kModeGrad;          // (max, sum) given
     constexpr int K = MODE == kModePreference ? 2 : 4;  // sums of a workgroup
@@ -799,37 +800,6 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
                 for (int c = 0; c < CREG; ++c)
                     if (c < classes) {
                         values<T, VEC>(raw[c], v);
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
-                    }
-            }
-        } else if (any && !kStats) {
-            for (int32_t c0 = 0; c0 < classes; c0 += kStep) {
-                float top[VEC];
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) top[k] = m[k];
-#pragma unroll
-                for (int j = 0; j < kStep; ++j)
-                    if (c0 + j < classes) raw[j] = plane(c0 + j);
-#pragma unroll
-                for (int j = 0; j < kStep; ++j)
-                    if (c0 + j < classes) {
-                        values<T, VEC>(raw[j], v);
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k) {
-                            top[k] = fmaxf(top[k], v[k]);
-                            xl[k] = y[k] == c0 + j ? v[k] : xl[k];
-                        }
-                    }
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    s[k] *= rescale(m[k], top[k], a.t);
-                    m[k] = top[k];
-                }
-#pragma unroll
-                for (int j = 0; j < kStep; ++j)
-                    if (c0 + j < classes) {
-                        values<T, VEC>(raw[j], v);
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
                     }
@@ -1095,12 +1065,12 @@ struct SumArgs {
     const float *logp;
     const float *ratio;     // preference: logp - ref
     Labels y;
-    int64_t n, l, c, chunks;
+    int64_t n, l, chunks;
     Policy policy;
     double *part;           // [n, chunks, K]
 };
 
-// Positions counted of sequence blockIdx.y's chunk blockIdx.x, and their sums:
+// What is summed over the counted positions of a sequence (the count is the last term):
 //   kSumCount: {count};  kSumPreference: {sum logp - ref, count};  kSumPolicy: {sum surrogate, sum far, clipped, count}.
 enum { kSumCount = 0, kSumPreference = 1, kSumPolicy = 2 };
 template <int WHAT>
@@ -1289,6 +1259,8 @@ int64_t ways_of(int64_t n, int64_t l) {
 int64_t chunks_of(int64_t l) { return l > kTokChunk ? ceil_div(l, kTokChunk) : 1; }
 unsigned grid_of(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
+constexpr int64_t kThreadsMost = (int64_t)1 << 31;   // threads of a launch: a grid's are counted in 32 bits
+
 bool logits_ok(const spice_logits *x) {
     return x && x->n >= 0 && x->l >= 0 && x->c >= 1 && x->c <= 0x7fffffff - 65536 && x->dtype >= 0 && x->dtype <= 2 &&
            (x->data || x->n == 0 || x->l == 0) &&
@@ -1321,7 +1293,7 @@ void grad_layout(TokArgs &a, void *grad, int32_t class_last) {
 template <typename T, int LANES, int NV, int MODE>
 int launch_row(const TokArgs &a, hipStream_t stream) {
     constexpr int block = LANES < kTokThreads ? kTokThreads : LANES, rows = block / LANES;
-    constexpr int64_t most = (int64_t)1 << 30;
+    constexpr int64_t most = kThreadsMost / LANES;
     for (int64_t first = 0; first < a.x.n * a.x.l; first += most) {
         const int64_t left = a.x.n * a.x.l - first;
         tok_row_kernel<T, LANES, NV, MODE><<<(unsigned)ceil_div(left < most ? left : most, rows), block, 0, stream>>>(a, first);
@@ -1344,16 +1316,16 @@ int launch_rows(const TokArgs &a, hipStream_t stream) {
         SPICE_LAUNCH_CHECK();
         return SPICE_OK;
     } else {
-    if (whole(64) <= 8) return launch_row<T, 64, 8, MODE>(a, stream);
-    if (whole(256) <= 4) return launch_row<T, 256, 4, MODE>(a, stream);
-    if (whole(256) <= 8) return launch_row<T, 256, 8, MODE>(a, stream);
-    if (whole(512) <= 8) return launch_row<T, 512, 8, MODE>(a, stream);
-    if (whole(1024) <= 8) return launch_row<T, 1024, 8, MODE>(a, stream);
-    if (whole(1024) <= 16) return launch_row<T, 1024, 16, MODE>(a, stream);
-    if (whole(1024) <= 20) return launch_row<T, 1024, 20, MODE>(a, stream);
-    tok_long_row_kernel<T, MODE><<<grid_of(a.x.n * a.x.l), 1024, 0, stream>>>(a);
-    SPICE_LAUNCH_CHECK();
-    return SPICE_OK;
+        if (whole(64) <= 8) return launch_row<T, 64, 8, MODE>(a, stream);
+        if (whole(256) <= 4) return launch_row<T, 256, 4, MODE>(a, stream);
+        if (whole(256) <= 8) return launch_row<T, 256, 8, MODE>(a, stream);
+        if (whole(512) <= 8) return launch_row<T, 512, 8, MODE>(a, stream);
+        if (whole(1024) <= 8) return launch_row<T, 1024, 8, MODE>(a, stream);
+        if (whole(1024) <= 16) return launch_row<T, 1024, 16, MODE>(a, stream);
+        if (whole(1024) <= 20) return launch_row<T, 1024, 20, MODE>(a, stream);
+        tok_long_row_kernel<T, MODE><<<grid_of(a.x.n * a.x.l), 1024, 0, stream>>>(a);
+        SPICE_LAUNCH_CHECK();
+        return SPICE_OK;
     }
 }
 
@@ -1374,7 +1346,7 @@ int launch_planes(const TokArgs &a, hipStream_t stream) {
     const bool split = a.x.c > kPlanesClasses;
     const int64_t tiles = split ? ceil_div(a.x.l, kSplitTile) : planes_tiles(a.x.l, VEC > 1);
     constexpr int groups = kTokThreads * VEC / kSplitTile;
-    constexpr int64_t most = (int64_t)1 << 30;
+    constexpr int64_t most = kThreadsMost / kTokThreads;
     for (int64_t first = 0; first < a.x.n * tiles; first += most) {
         const int64_t left = a.x.n * tiles - first;
         const unsigned grid = (unsigned)(left < most ? left : most);
@@ -1458,7 +1430,6 @@ SumArgs sums_of(const TokArgs &a, double *part) {
     s.y = a.y;
     s.n = a.x.n;
     s.l = a.x.l;
-    s.c = a.x.c;
     s.chunks = chunks_of(a.x.l);
     s.policy = a.policy;
     s.part = part;

@@ -423,6 +423,9 @@ def test_nothing_counted_and_no_positions(dev):
             assert (out == 0).all() and (logp == 0).all() and (grad == 0).all()
         total, rewards, grad = ops.preference_loss(x, y, f, want_grad=True, average=True, **how)
         assert abs(total.item() - math.log(2)) <= 2 * U and (rewards == 0).all() and (grad == 0).all()
+    out, logp, grad = ops.policy_loss(torch.zeros(0, 3, 9, device=dev), torch.zeros(0, 3, dtype=torch.int64, device=dev),
+                                      torch.zeros(0, 3, device=dev), torch.ones(0, device=dev), class_dim=-1, want_grad=True)
+    assert (out == 0).all() and logp.shape == (0, 3) and grad.shape == (0, 3, 9)
     x, y, f = torch.zeros(2, 0, 9, device=dev), torch.zeros(2, 0, dtype=torch.int64, device=dev), torch.zeros(2, 0, device=dev)
     assert ops.token_logprobs(x, y, class_dim=-1)[0].shape == (2, 0)
     out, _, grad = ops.policy_loss(x, y, f, torch.ones(2, device=dev), class_dim=-1, want_grad=True)
@@ -454,11 +457,11 @@ def test_differentiable_logprobs_and_their_views(dev):
     x = torch.randn(2, 6, 5, 30, generator=torch.Generator().manual_seed(4)).to(dev).transpose(1, 2).requires_grad_(True)
     y = torch.randint(0, 30, (2, 5, 6), generator=torch.Generator().manual_seed(5)).to(dev)
     logp = token_logprobs(x, y.int(), class_dim=-1)
-    (-logp.mean()).backward()
+    assert logp.requires_grad
     v = x.detach().cpu().double().requires_grad_(True)
     want = -ot.token_logprobs(v, y.cpu(), class_dim=-1)[0].mean()
     g64, = torch.autograd.grad(want, v)
-    _close(x.grad if False else torch.autograd.grad(-token_logprobs(x, y, class_dim=-1).mean(), x)[0], g64,
+    _close(torch.autograd.grad(-token_logprobs(x, y, class_dim=-1).mean(), x)[0], g64,
            _grad_tol(v.detach().float(), g64, torch.full(y.shape, 1 / 60, dtype=torch.float64), -1, 1.0))
     with torch.no_grad():
         assert not token_logprobs(x, y, class_dim=-1).requires_grad
