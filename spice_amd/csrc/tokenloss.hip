@@ -124,12 +124,13 @@ __device__ __forceinline__ double fold_max_sum(float &m, float s, Temper t, doub
             lds[waves + threadIdx.x / kWave] = (double)all;
         }
         __syncthreads();
-        float top = (float)lds[waves];
+        // every lane takes one wave's pair: all of them in every thread cost 16 exponentials a thread, 2 us of a row
+        const int w = threadIdx.x & (waves - 1);
+        const float mine = (float)lds[waves + w];
+        float top = mine;
 #pragma unroll
-        for (int w = 1; w < waves; ++w) top = fmaxf(top, (float)lds[waves + w]);
-        sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < waves; ++w) sum += lds[w] * (double)rescale((float)lds[waves + w], top, t);
+        for (int o = waves / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+        sum = wide_sum(lds[w] * (double)rescale(mine, top, t), waves);
         all = top;
     }
     m = all;
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
                     for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
                 }
             const double sum = fold_row<LANES>(m, s, a.t, lds);
-            logp = logp_of(xl - shift_of(m), sum, a.t);
+            if (kGrad || lane == 0) logp = logp_of(xl - shift_of(m), sum, a.t);
             s = (float)sum;
         }
     }
