@@ -1303,22 +1303,34 @@ int launch_row(const TokArgs &a, hipStream_t stream) {
     return SPICE_OK;
 }
 
-// How many lanes hold a row, by its full 16-byte vectors: as few as keep at most 8 a lane, then 16 and 20 with a whole
-// workgroup of 1024.
+// Full vectors a lane of 4 and of 16 lanes a row: shorter rows share a wave.
+constexpr int kShort4 = 8, kShort4Grad = 3, kShort16 = 6;
+
+// How many lanes hold a row, by its full 16-byte vectors: as few as can keep them, so that a wave's fixed work (labels,
+// fold, logarithm) is shared by many rows.  Forward / policy loss / gradient in us, bf16, 2^27 logits or 2^20 rows in all:
+//   c = 64: 4 lanes 38 / 90 / 53, 16 lanes 102 / 176 / 98;   c = 256: 4 lanes 49 / 131 / 105, 16 lanes 75 / 156 / 102,
+//   64 lanes 208 / 323 / 177;   c = 512: 16 lanes 53 / 129 / 96, 64 lanes 116 / 204 / 102;   c = 1000: 16 lanes
+//   50 / 130 / 106, 64 lanes 67 / 129 / 83;   c = 4096: 64 lanes 46 / 109 / 84, 256 lanes 69 / 143 / 86;   c = 16384:
+//   256 lanes 47 / 111, 512 lanes 55 / 123;   c = 32000: 512 lanes 49 / 113, 1024 lanes 55 / 149;   c = 131072: 16 vectors
+//   of 1024 lanes 61 / 133, the long row kernel 56 / 135 (8 rows: 11.3 / 26.7 and 13.0 / 29.4).
+// 4 lanes store a gradient in pieces of 64 bytes, which costs at odd widths (c = 150, gradient: 187, with 16 lanes 156): the
+// gradient by itself leaves them earlier; the policy loss does not (205 against 222), so that its sums are the same with a
+// gradient and without one.  The gradient by itself is also shared among workgroups sooner (kGradVecs vectors a lane;
+// c = 2000: 84 with 64 lanes a row, 99 so; c = 4096: 84 and 77).
 template <typename T, int MODE>
 int launch_rows(const TokArgs &a, hipStream_t stream) {
+    constexpr int short4 = MODE == kModeGrad ? kShort4Grad : kShort4;
     const auto whole = [&](int lanes) { return a.x.c / (lanes * vec_elements<T>()); };
-    if (whole(4) <= 1) return launch_row<T, 4, 1, MODE>(a, stream);
-    if (whole(16) <= 1) return launch_row<T, 16, 1, MODE>(a, stream);
-    if (whole(64) <= 2) return launch_row<T, 64, 2, MODE>(a, stream);
-    if constexpr (MODE == kModeGrad) {      // longer rows: without the row's other phases
+    if (whole(4) <= short4) return launch_row<T, 4, short4, MODE>(a, stream);
+    if (whole(16) <= kShort16) return launch_row<T, 16, kShort16, MODE>(a, stream);
+    if constexpr (MODE == kModeGrad) {
+        if (whole(64) <= 4) return launch_row<T, 64, 4, MODE>(a, stream);
         const int64_t pieces = ceil_div(a.x.c, (int64_t)kGradVecs * kTokThreads * vec_elements<T>());
         tok_row_grad_kernel<T><<<grid_of(a.x.n * a.x.l * pieces), kTokThreads, 0, stream>>>(a, pieces);
         SPICE_LAUNCH_CHECK();
         return SPICE_OK;
     } else {
         if (whole(64) <= 8) return launch_row<T, 64, 8, MODE>(a, stream);
-        if (whole(256) <= 4) return launch_row<T, 256, 4, MODE>(a, stream);
         if (whole(256) <= 8) return launch_row<T, 256, 8, MODE>(a, stream);
         if (whole(512) <= 8) return launch_row<T, 512, 8, MODE>(a, stream);
         if (whole(1024) <= 8) return launch_row<T, 1024, 8, MODE>(a, stream);
@@ -1387,7 +1399,7 @@ int route_of(const TokArgs &a) {
 
 // Rows of several sequences that share a wave: it cannot count each one's labels.
 bool rows_share_waves(const TokArgs &a, int32_t dtype) {
-    return route_of(a) == kByRows && a.per_sequence && a.x.n > 1 && a.x.c / (16 * (dtype == 0 ? 4 : 8)) <= 1;
+    return route_of(a) == kByRows && a.per_sequence && a.x.n > 1 && a.x.c / (16 * (dtype == 0 ? 4 : 8)) <= kShort16;
 }
 
 template <typename T, int MODE>

@@ -538,3 +538,18 @@ def test_refusals_on_the_device(dev):
     ]:
         with pytest.raises(kind, match=text):
             call()
+
+
+# both sides of the row width where each form of the row kernels ends (full 16-byte vectors of 4, 16, 64, 256 lanes ...),
+# in sequences short enough that a wave's rows belong to several of them
+WIDTHS = [31, 32, 33, 63, 64, 127, 128, 143, 144, 287, 288, 447, 448, 895, 896, 1279, 1280, 2303, 2304, 2559, 2560, 4607, 4608,
+          9215, 9216, 18431, 18432, 36863, 36864]
+
+
+@pytest.mark.parametrize("c", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_at_the_ends_of_their_forms(dev, c, dtype):
+    shape = ("last", 5, (7,), c, dtype) if c < 2000 else ("last", 2, (3,), c, dtype)
+    test_token_logprobs_and_gradient(dev, shape, 0.7)
+    test_policy_loss(dev, shape, "sequence", 0.2, 0.7, True)
+    test_policy_loss(dev, shape, "token", 0.0, 1.0, False)
