@@ -729,7 +729,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
     constexpr bool kStats = MODE == kModeGrad;          // (max, sum) given
     constexpr int K = MODE == kModePreference ? 2 : 4;  // sums of a workgroup
     constexpr bool kSums = MODE == kModePreference || MODE == kModePolicy || MODE == kModePolicyGrad;
-    constexpr bool kOnce = MODE == kModePolicyGrad && CREG > 0;   // the logits' only reader (see read_vec)
+    constexpr bool kOnce = MODE == kModePolicyGrad && CREG > 0 && VEC > 1;   // the logits' only reader (see read_vec)
     constexpr int kStep = 8;
     typedef typename GroupOf<T, VEC>::type G;
     __shared__ double lds[kSums ? K * kTokThreads / kWave : 1];
@@ -888,7 +888,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
     constexpr int RUN = kSplitTile / VEC, GROUPS = kTokThreads / RUN, kStep = HOLD > 0 ? HOLD : 8;
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
     constexpr bool kStats = MODE == kModeGrad;
-    constexpr bool kOnce = MODE == kModePolicyGrad && HOLD > 0;
+    constexpr bool kOnce = MODE == kModePolicyGrad && HOLD > 0 && VEC > 1;
     constexpr int K = MODE == kModePreference ? 2 : 4;
     constexpr bool kSums = MODE == kModePreference || MODE == kModePolicy || MODE == kModePolicyGrad;
     typedef typename GroupOf<T, VEC>::type G;
@@ -1345,11 +1345,13 @@ int launch_rows(const TokArgs &a, hipStream_t stream) {
 // Neighbouring positions a lane of the planes kernels takes, and the most classes that one lane walks alone.
 constexpr int kPlanesVec = 4, kPlanesClasses = 32;
 
+bool next_to_each_other(const TokArgs &a) { return a.x.sl == 1 && (!a.grad || a.g_sl == 1); }
+
 // Four positions a lane, at any alignment; the last group of a sequence reaches back into the one before, so there have to
 // be as many positions as a lane (or, with many classes, a workgroup) takes, or a multiple of four.
 bool planes_vec(const TokArgs &a) {
     const int64_t least = a.x.c > kPlanesClasses ? kSplitTile : kPlanesVec;
-    return a.x.l >= least || a.x.l % kPlanesVec == 0;
+    return next_to_each_other(a) && (a.x.l >= least || a.x.l % kPlanesVec == 0);
 }
 
 int64_t planes_tiles(int64_t l, bool vec) { return ceil_div(l, (int64_t)kTokThreads * (vec ? kPlanesVec : 1)); }
@@ -1385,16 +1387,16 @@ int launch_planes(const TokArgs &a, hipStream_t stream) {
     return SPICE_OK;
 }
 
-// Which kernel takes a call: rows where the classes are neighbours in memory, planes where the positions are, any strides
-// else.
+// Which kernel takes a call: rows where the classes are neighbours in memory, planes (where the positions are not
+// neighbours, or the gradient's are not, one a lane), and a workgroup a position for few positions of many classes.
 enum { kByRows, kByPlanes, kByAny };
 int route_of(const TokArgs &a) {
-    if (a.x.sc == 1) return !a.grad || a.g_sc == 1 ? kByRows : kByAny;   // (channels last: its gradient is in planes)
-    // few positions and many classes: a workgroup a position fills more of the chip than 64 positions a workgroup (256
-    // positions of 3001 classes: 6.5 against 41 us, of 150 classes 6.3 both; 4096 of 1000: 22 against 17)
-    if (a.x.c > 256 && a.x.n * a.x.l <= 512) return kByAny;
-    if (a.x.sl == 1 && (!a.grad || a.g_sl == 1)) return kByPlanes;
-    return kByAny;
+    if (a.x.sc == 1 && (!a.grad || a.g_sc == 1)) return kByRows;   // (channels last: its gradient is in planes)
+    // a workgroup a position fills more of the chip than 64 positions a workgroup (256 positions of 3001 classes: 6.5 against
+    // 41 us, of 150 classes 6.3 both; 4096 of 1000: 22 against 17); strided, 512 of 150: 6 / 14 / 6 us forward / policy /
+    // gradient against 8 / 18 / 8, 4096 of 150: 13 / 34 / 16 against 8 / 21 / 8, 65536 of 150: 117 / 219 / 159 against 16 / 43 / 22
+    const bool few = a.x.n * a.x.l <= 512;
+    return few && a.x.c > (next_to_each_other(a) ? 256 : kPlanesClasses) ? kByAny : kByPlanes;
 }
 
 // Rows of several sequences that share a wave: it cannot count each one's labels.

@@ -53,9 +53,11 @@ def _inputs(layout, n, positions, c, dtype, seed=0, ignore=None):
     y = torch.randint(0, c, (n, *positions), generator=g)
     x.scatter_add_(-1, y.unsqueeze(-1), torch.full((n, *positions, 1), 4.0))
     y = torch.where(torch.rand(n, *positions, generator=g) < 1 / 6, ignore, y)
+    if layout != "last":
+        x = x.movedim(-1, 1)
     if layout == "planes":
-        x = x.movedim(-1, 1).contiguous()
-    return x.to(dtype), y, 1 if layout == "planes" else -1, ignore
+        x = x.contiguous()
+    return x.to(dtype), y, -1 if layout == "last" else 1, ignore
 
 
 def _last(t, class_dim):
@@ -379,7 +381,10 @@ def test_policy_loss(dev, shape, reduction, kl, t, each):
     _close(grad, g64, _grad_tol(x, g64, torch.where(keep, w, zero), d, t)
            + (torch.where(keep, dw, zero) / t).unsqueeze(d if d == 1 else -1), "grad")
     plain = ops.policy_loss(*args, ref_logprobs=refd, **opts)
-    assert torch.equal(plain[0], out) and torch.equal(plain[1], logp) and plain[2] is None
+    if shape[0] != "channels last":     # (there the pass with a gradient, whose order is another one, is another kernel)
+        assert torch.equal(plain[0], out) and torch.equal(plain[1], logp)
+    _close(plain[1], lp, tl, "logp without a gradient")
+    assert plain[2] is None
     # the module: the same gradient for an upstream factor of 1 and of `scale`, and from a second backward
     loss = ClippedPolicyLoss(clip_low=0.2, clip_high=0.3, kl_weight=kl, reduction=reduction, **how)
     leaf = x.to(dev).requires_grad_(True)
@@ -553,3 +558,47 @@ def test_rows_at_the_ends_of_their_forms(dev, c, dtype):
     test_token_logprobs_and_gradient(dev, shape, 0.7)
     test_policy_loss(dev, shape, "sequence", 0.2, 0.7, True)
     test_policy_loss(dev, shape, "token", 0.0, 1.0, False)
+
+
+# logits whose classes lie next to each other and whose gradient's positions do: one position a lane, or a workgroup
+@pytest.mark.parametrize("n, positions, c", [(2, (20, 30), 21), (2, (1, 7), 21), (4, (9,), 6), (2, (17, 31), 40), (2, (300,), 300),
+                                             (2, (8, 16), 150), (2, (301,), 1000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_channels_last_logits(dev, n, positions, c, dtype):
+    shape = ("channels last", n, positions, c, dtype)
+    x = _inputs(*shape)[0]
+    assert x.to(dev).stride() == x.stride() and not x.to(dev).is_contiguous()
+    test_token_logprobs_and_gradient(dev, shape, 0.7)
+    test_preference_loss(dev, shape, "sigmoid", 0.1, True)
+    test_policy_loss(dev, shape, "token", 0.0, 1.0, False)
+    test_policy_loss(dev, shape, "sequence", 0.2, 0.7, True)
+
+
+@pytest.mark.parametrize("c", [5, 21, 40, 300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_second_position_of_many(dev, c, dtype):
+    """Planes whose positions lie two apart: the same bounds as the dense tensor's."""
+    wide = (2.0 * torch.randn(2, c, 403, 2, generator=torch.Generator().manual_seed(31))).to(dtype)
+    y = torch.randint(0, c, (2, 403), generator=torch.Generator().manual_seed(32))
+    y[1, ::5] = -100
+    how = dict(class_dim=1, ignore_index=-100)
+    x, view = wide[..., 0].contiguous(), wide.to(dev)[..., 0]
+    assert view.stride(2) == 2
+    v = x.double().requires_grad_(True)
+    want, _ = ot.token_logprobs(v, y, **how)
+    g64, = torch.autograd.grad(want.sum(), v)
+    logp, stats = ops.token_logprobs(view, y.to(dev), **how)
+    _close(logp, want.detach(), _bounds(x, 1, 1.0)[1] + 2 * U * want.detach().abs(), "logp")
+    grad = ops.token_logprobs_grad(view, y.to(dev), stats, torch.ones(2, device=dev), **how)
+    _close(grad, g64, _grad_tol(x, g64, torch.ones(y.shape, dtype=torch.float64), 1, 1.0), "grad")
+    # the policy loss at its own sample: ratio 1, so total = -mean A and the gradient -A logp's share of the mean
+    adv = torch.tensor([0.5, -2.0], device=dev)
+    out, again, pg = ops.policy_loss(view, y.to(dev), logp, adv, want_grad=True, **how)
+    # (the ratio of two passes' logp is off by their difference, which both bounds hold)
+    tl = _bounds(x, 1, 1.0)[1] + 2 * U * want.detach().abs()
+    _close(again, want.detach(), tl, "policy logp")
+    keep = (y != -100).double()
+    a64 = adv.cpu().double()[:, None] * keep / keep.sum()
+    _close(out[0], -a64.sum(), (a64.abs() * (2 * tl + 4 * U)).sum() + 4 * U, "total")
+    p64, = torch.autograd.grad(-(ot.token_logprobs(v, y, **how)[0] * a64).sum(), v)
+    _close(pg, p64, _grad_tol(x, p64, a64.abs() * (1 + 2 * tl + 4 * U), 1, 1.0) + (a64.abs() * (2 * tl + 4 * U)).unsqueeze(1), "policy grad")
