@@ -16,7 +16,7 @@ namespace {
 constexpr int kTokThreads = 256;
 constexpr int kTokChunk = 2048;      // positions of one workgroup of the passes over positions
 constexpr int kTokFold = 1024;       // threads of the one workgroup that folds their partial sums
-constexpr int64_t kTokCount = 2048;  // positions that every workgroup counts for itself: a launch less ([1,7,32000] fp16)
+constexpr int64_t kTokCount = 2048;  // positions that every workgroup counts for itself: a launch less ([1,7,32000] fp16: 14.8 us, 17.4 with)
 constexpr int64_t kTokHere = 4096;   // positions that this workgroup sums itself: 4 a thread
 
 // The logits as the kernels see them: element strides of sequence, position and class.
@@ -252,6 +252,9 @@ __device__ __forceinline__ float share_here(const TokArgs &a, int64_t n, int *ld
 // loss sums over positions.  PolicyGrad: the policy loss's gradient behind that.
 enum { kModeLogp = 0, kModeGrad = 1, kModePreference = 2, kModePolicy = 3, kModePolicyGrad = 4 };
 
+// For few positions of many classes at any stride, where a workgroup a position is what fills the chip (route_of); bound by
+// latency: one pass for maximum and sum, a second over the same lines for the gradient.  fp32 [1,3001,256] planes: forward
+// 8.4 us, gradient 16, policy loss with both and its end launch 28.
 template <typename T, int MODE>
 __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
     __shared__ double lds[2 * kTokThreads / kWave];
@@ -413,6 +416,16 @@ __device__ __forceinline__ void forget(u32x4 (&raw)[NV]) {
     for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
 }
 
+// A row is read once, as 16-byte loads at whatever address it starts, and stays packed in registers: maximum, exponentials
+// and gradient are taken from there, so the bytes of the logits (and of the gradient) bound it.  LANES and NV: launch_rows.
+// bf16, 5.9 TB/s being the card's large copy:
+//   [1,1,32000] forward 5.0 us (one workgroup: a load, two barriers);   [8,1024,32000] forward 104 us (5.0 TB/s);
+//   [4,1023,50001] forward 65 us, a third of the rows ignored (4.1 TB/s: rows start at odd addresses);
+//   [8,512,131072] policy loss, logits in and gradient out, two fifths ignored, 307 us (5.5 TB/s; one row fills a compute
+//   unit's registers, so its loads do not run under the last row's stores).
+// A wave's fixed work (labels, fold, logarithm: about 1000 cycles) bounds rows of under 256 classes: 2^20 of 21 bf16 classes
+// take 33 us where their bytes are 7.
+//
 // Vector i of lane j holds the classes from (i LANES + j) K on: the first `whole` are full in every lane (the same count in
 // all of them), the one behind is ragged, filled up with -inf.  Fewer than 64 lanes: several rows a wave.
 template <typename T, int LANES, int NV, int MODE>
@@ -520,7 +533,10 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     }
 }
 
-// Rows longer than the registers of a workgroup: read twice, the maximum and sum running along.
+// Rows longer than the registers of a workgroup: four vectors a thread at a time, the maximum and sum running along (one
+// rescaling a step), and for the gradient read again, mostly from the memory-side cache.  Bound by the bytes: bf16
+// [1,4096,200000] forward 405 us (4.0 TB/s: each step's loads wait for the step before), policy loss 819 (the logits twice and
+// the gradient: 6.0 TB/s).
 template <typename T, int MODE>
 __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
     constexpr int K = vec_elements<T>(), kBlock = 1024, kStep = 4;
@@ -597,8 +613,10 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
     }
 }
 
-// weight * d logp / d x of rows whose maximum and sum are known: a workgroup takes kGradVecs vectors a lane of one row.
-// ([8,1024,32000] bf16, loss + gradient: 241 us with 1, 181 with 2, 188 with 4 and 8)
+// weight * d logp / d x of rows whose maximum and sum are known: a stream, nothing to fold, so a workgroup takes kGradVecs
+// vectors a lane of one row, whatever the row's length ([8,1024,32000] bf16, loss + gradient: 241 us with 1, 181 with 2, 188
+// with 4 and 8).  Bound by the bytes: bf16 [8,1024,32000] 184 us (5.7 TB/s); behind a preference loss that ignores two fifths
+// of the rows 116 us (7.1, part of the reads from the memory-side cache); [4,1023,50001], a third ignored, 104 us (6.5).
 constexpr int kGradVecs = 2;
 
 template <typename T>
@@ -721,6 +739,12 @@ __device__ __forceinline__ void forget_groups(G (&raw)[N]) {
 
 // CREG > 0: at most CREG classes, a position group's logits in registers, read once for maximum, sum and gradient.
 // CREG = 0: the gradient alone, eight planes at a time.
+// Four positions a lane make a wave's load of a plane 1 KB (fp32) in one instruction; all classes of a lane are in flight at
+// once, nothing is exchanged between lanes, and the loss's sums leave as one item a workgroup.  Bound by the bytes: fp32
+// [8,21,512x512] forward of the preference loss 43 us and its gradient 54 (218 and 386 MB with labels and statistics: 5.1 and
+// 7.2 TB/s, the reads partly from the memory-side cache), policy loss with gradient 62 (394 MB: 6.3).  Workgroups of 64, 128,
+// 512: 84, 84, 86 us for the whole policy loss, 77 with 256.  VEC = 1 takes any strides: channels last with a gradient in
+// planes, the same size, policy loss 150 us in all (each lane reads its own row's lines, the gradient's stores are whole).
 template <typename T, int VEC, int CREG, int MODE>
 __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24 ? 3 : 2) void tok_planes_kernel(TokArgs a, int64_t tiles,
                                                                                                                 int64_t first) {
@@ -881,6 +905,9 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
 // 64 neighbouring positions a workgroup: RUN lanes of VEC positions, and kTokThreads / RUN groups of them that take every
 // kTokThreads / RUN-th class, eight planes in flight a lane.  The groups' maxima and sums meet in LDS, where one wave
 // finishes the positions.  HOLD > 0: at most HOLD classes a group, kept for the gradient; HOLD = 0: any number, read again.
+// (One lane walking all classes: [1,150,1024] fp32 26 / 24 / 56 us forward / gradient / policy, so 6.4 / 6.0 / 13.)  Bound by
+// the bytes on large calls, 64 positions being 256 bytes a plane and load: fp32 [8,150,128x128] forward 18.8 us (4.2 TB/s),
+// gradient 28.6 (5.5), policy loss 45.7 with its count and end; [1,1000,512x512] 223 (4.7), 439 (4.8), 545.
 constexpr int kSplitTile = 64;
 
 template <typename T, int VEC, int HOLD, int MODE>
@@ -1092,6 +1119,8 @@ __device__ __forceinline__ void sum_position(const SumArgs &a, int64_t n, int64_
     }
 }
 
+// A pass over labels and log-probabilities, kTokChunk positions a workgroup; latency bounds it: 5 us for 8192 positions of a
+// loss as for the labels of 2^21 (17 MB).
 template <int WHAT>
 __global__ __launch_bounds__(kTokThreads) void tok_sum_kernel(SumArgs a) {
     constexpr int K = sum_terms<WHAT>();
@@ -1149,7 +1178,8 @@ __device__ __forceinline__ void fold_sequences(const double *part, int64_t n, in
 }
 
 // share[n]: what one position of sequence n counts in the mean over all counted positions (token), or in the mean over
-// sequences of each one's mean.  `ways` > 0: the positions are counted here.
+// sequences of each one's mean.  `ways` > 0: the positions are counted here.  One workgroup, latency: 4.5 us.  (Counts added
+// up by every workgroup of the loss's pass: [8,21,512x512] 78 to 84 us, 75 with this launch: each waits for them.)
 __global__ __launch_bounds__(kTokFold) void tok_share_kernel(SumArgs a, int64_t ways, int per_sequence, float *share) {
     __shared__ double lds[kTokFold / kWave];
     if (ways) sums_here<kSumCount>(a, ways);
@@ -1180,6 +1210,8 @@ __device__ __forceinline__ double sigmoid(double x) {
     return x >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
 }
 
+// The end of the preference loss: every sequence's log ratio from its partial sums, the pairs' losses, and what one position
+// of each sequence weighs in the gradient.  One workgroup, latency: 5.1 us, with 37 or with 2^18 positions a sequence.
 __global__ __launch_bounds__(kTokFold) void tok_preference_kernel(SumArgs a, int64_t ways, PreferenceEnd e) {
     __shared__ double lds[kTokFold / kWave];
     if (ways) sums_here<kSumPreference>(a, ways);
@@ -1221,7 +1253,8 @@ __device__ __forceinline__ void policy_end(double surrogate, double far, double 
     out4[3] = (float)(over / fmax(count, 1.0));
 }
 
-// The end of the policy loss.  `each` [n, 4]: scratch.
+// The end of the policy loss.  `each` [n, 4]: scratch.  One workgroup, latency: 6.0 us.  (By the last workgroup of the loss's
+// pass, told by a ticket: 100 us for [8,21,512x512], 79 at that time with launches of their own.)
 __global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, int per_sequence, double *each, float kl,
                                                                   float *out4) {
     __shared__ double lds[4 * kTokFold / kWave];
