@@ -427,7 +427,8 @@ __device__ __forceinline__ void forget(u32x4 (&raw)[NV]) {
 // take 33 us where their bytes are 7.
 //
 // Vector i of lane j holds the classes from (i LANES + j) K on: the first `whole` are full in every lane (the same count in
-// all of them), the one behind is ragged, filled up with -inf.  Fewer than 64 lanes: several rows a wave.
+// all of them), the one behind is ragged: it reaches back (value by value, bf16, 894,784 rows of 150: policy loss 205 us, 154
+// so), or is filled up with -inf.  Fewer than 64 lanes: several rows a wave.
 template <typename T, int LANES, int NV, int MODE>
 __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 ? 6 : 4) void tok_row_kernel(TokArgs a, int64_t first) {
     constexpr int K = vec_elements<T>();
@@ -445,6 +446,8 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
     if (at >= a.x.n * a.x.l) return;
     const int32_t lane = threadIdx.x % LANES, classes = (int32_t)a.x.c, whole = classes / (LANES * K);
     const int32_t tail = (whole * LANES + lane) * K, left = classes - tail;
+    // the row's last classes, fewer than a vector: the row's last K instead, whose first `again` are another lane's too
+    const int32_t again = left > 0 && left < K && classes >= K ? K - left : 0, from = tail - again;
     const int64_t n = at / a.x.l, l = at - n * a.x.l;
     const T *x = (const T *)a.x.x + n * a.x.sn + l * a.x.sl;
     const int64_t y = a.y.y[n * a.y.sn + l * a.y.sl];
@@ -461,7 +464,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (i < whole) raw[i] = read_vec<MODE == kModePolicyGrad && kLong>(mine + i * LANES * K);
-        last = load_vec<T>(x + tail, left);
+        last = load_vec<T>(x + from, left + again);
         if constexpr (kStats) {
             const float2 st = a.stats_in[at];
             m = st.x;
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
             forget<NV>(raw);
             unpack(last, v, T());
 #pragma unroll
-            for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+            for (int k = 0; k < K; ++k) s += k < again ? 0.f : exp_of(v[k] - shift, a.t);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (i < whole) {
@@ -523,8 +526,8 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
                     store_vec<kLong>(mine + i * LANES * K, K, v);
                 }
             unpack(last, v, T());
-            grad_of<K>(v, shift, each, w, (int32_t)y, tail, a.t);
-            if (left > 0) store_vec<kLong>(g + tail, left, v);
+            grad_of<K>(v, shift, each, w, (int32_t)y, from, a.t);
+            if (left > 0) store_vec<kLong>(g + from, left + again, v);      // (two lanes store the same values there)
         } else {
 #pragma unroll
             for (int k = 0; k < K; ++k) v[k] = each;
@@ -1346,8 +1349,8 @@ constexpr int kShort4 = 8, kShort4Grad = 3, kShort16 = 6;
 //   50 / 130 / 106, 64 lanes 67 / 129 / 83;   c = 4096: 64 lanes 46 / 109 / 84, 256 lanes 69 / 143 / 86;   c = 16384:
 //   256 lanes 47 / 111, 512 lanes 55 / 123;   c = 32000: 512 lanes 49 / 113, 1024 lanes 55 / 149;   c = 131072: 16 vectors
 //   of 1024 lanes 61 / 133, the long row kernel 56 / 135 (8 rows: 11.3 / 26.7 and 13.0 / 29.4).
-// 4 lanes store a gradient in pieces of 64 bytes, which costs at odd widths (c = 150, gradient: 187, with 16 lanes 156): the
-// gradient by itself leaves them earlier; the policy loss does not (205 against 222), so that its sums are the same with a
+// 4 lanes store a gradient in pieces of 64 bytes, which costs at odd widths (c = 200, gradient: 136, with 16 lanes 106): the
+// gradient by itself leaves them earlier; the policy loss does not (161 against 166), so that its sums are the same with a
 // gradient and without one.  The gradient by itself is also shared among workgroups sooner (kGradVecs vectors a lane;
 // c = 2000: 84 with 64 lanes a row, 99 so; c = 4096: 84 and 77).
 template <typename T, int MODE>
