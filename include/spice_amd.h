@@ -623,20 +623,25 @@ int spice_policy_loss(const spice_logits *logits, const spice_labels *labels, co
  *
  * `grads`, `params`, ... are HOST arrays of `count` device pointers (aligned to
  * their element), numel a host array of element counts; they are read before the
- * call returns.  dtype 0 = fp32, 1 = fp16, 2 = bf16, one for all tensors of a call.
+ * call returns.  dtype 0 = fp32, 1 = fp16, 2 = bf16, one for all tensors of a call
+ * (but spice_grad_norm_of_types).
  * record: 4 device floats, {norm, clip factor, and two of the Adam step's}; an Adam step that neither clips nor counts
  * on the device leaves it as it is.
  * ------------------------------------------------------------------------- */
 #define SPICE_NORM_L2 0
 #define SPICE_NORM_INF 1
 
-/* Bytes of workspace of spice_grad_norm and of spice_adam_step with clipping; nothing in it has to be cleared. */
+/* Bytes of workspace of the norms and of spice_adam_step with clipping; nothing in it has to be cleared. */
 size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t count);
 
 /* record[0] = norm over all tensors (squares summed in fp64, fixed order), record[1] = min(1, max_norm / (norm + 1e-6)).
  * A NaN or infinite gradient makes the norm NaN or infinite and the factor NaN or 0. */
 int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
                     float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same over tensors of several types: dtypes [count] on the host. */
+int spice_grad_norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *numel, int32_t count, int32_t norm_type,
+                             float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
 
 /* out = record[1] * grads, rounded once to out_dtype (the gradients' own, or fp32).  out may be grads (then nothing is
  * moved where the factor is 1); other overlaps are not allowed. */

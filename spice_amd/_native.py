@@ -174,6 +174,8 @@ SIGNATURES = {
     "spice_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int32]),
     "spice_grad_norm": (c_int32, [POINTER(c_void_p), POINTER(c_int64), c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
                                   c_size_t, c_void_p]),
+    "spice_grad_norm_of_types": (c_int32, [POINTER(c_void_p), POINTER(c_int32), POINTER(c_int64), c_int32, c_int32, c_float,
+                                           c_void_p, c_void_p, c_size_t, c_void_p]),
     "spice_grad_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_void_p,
                                   c_void_p]),
     "spice_grad_norm_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_int32,

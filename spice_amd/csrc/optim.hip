@@ -332,24 +332,33 @@ bool counts_ok(const int64_t *numel, int32_t count) {
     return true;
 }
 
-int64_t item_count(const int64_t *numel, int32_t count, uint32_t each) {
+// The tensors of one type among a call's: all of them without `dtypes`.
+struct OfType {
+    const int32_t *dtypes;
+    int32_t dtype;
+    bool operator()(int32_t i) const { return !dtypes || dtypes[i] == dtype; }
+};
+
+int64_t item_count(const int64_t *numel, int32_t count, uint32_t each, OfType of = {}) {
     int64_t items = 0;
     const int64_t most = kOptEntryMost / each * each;
     for (int32_t i = 0; i < count; ++i)
-        for (int64_t at = 0; at < numel[i]; at += most) items += ceil_div(numel[i] - at < most ? numel[i] - at : most, each);
+        for (int64_t at = 0; of(i) && at < numel[i]; at += most) items += ceil_div(numel[i] - at < most ? numel[i] - at : most, each);
     return items;
 }
 
 // Calls launch(table, first item, items) for as many tables as the tensors need.  ptrs: PTRS host arrays of device
 // pointers; bytes: element size of each.
 template <int PTRS, typename F>
-int for_tables(void *const *const (&ptrs)[PTRS], const int64_t (&bytes)[PTRS], const int64_t *numel, int32_t count, uint32_t each, F launch) {
+int for_tables(void *const *const (&ptrs)[PTRS], const int64_t (&bytes)[PTRS], const int64_t *numel, int32_t count, uint32_t each, F launch,
+               OfType of = {}) {
     TableOf<PTRS> t;
     t.count = 0;
     t.each = each;
     int64_t items = 0, before = 0;
     const int64_t most = kOptEntryMost / each * each;
     for (int32_t i = 0; i < count; ++i) {
+        if (!of(i)) continue;
         for (int64_t at = 0; at < numel[i]; at += most) {
             const int64_t n = numel[i] - at < most ? numel[i] - at : most;
             for (int k = 0; k < PTRS; ++k) t.p[k][t.count] = (char *)ptrs[k][i] + at * bytes[k];
@@ -391,17 +400,18 @@ bool pointers_ok(void *const *p, const int64_t *numel, int32_t count, int64_t by
 int64_t type_bytes(int32_t dtype) { return dtype == 0 ? 4 : 2; }
 
 template <typename T>
-int launch_norm(void *const *grads, const int64_t *numel, int32_t count, int64_t bytes, int inf, double *part, hipStream_t s) {
+int launch_norm(void *const *grads, const int64_t *numel, int32_t count, int inf, double *part, hipStream_t s, OfType of = {}) {
     void *const *const p[1] = {grads};
-    const int64_t b[1] = {bytes};
-    return for_tables<1>(p, b, numel, count, item_elements(numel, count), [&](const TableOf<1> &t, int64_t before, int64_t items) {
+    const int64_t b[1] = {(int64_t)sizeof(T)};
+    const auto launch = [&](const TableOf<1> &t, int64_t before, int64_t items) {
         if (inf)
             grad_norm_kernel<T, true><<<(unsigned)items, kOptThreads, 0, s>>>(t, part + before);
         else
             grad_norm_kernel<T, false><<<(unsigned)items, kOptThreads, 0, s>>>(t, part + before);
         SPICE_LAUNCH_CHECK();
         return (int)SPICE_OK;
-    });
+    };
+    return for_tables<1>(p, b, numel, count, item_elements(numel, count), launch, of);
 }
 
 template <typename T>
@@ -484,17 +494,8 @@ extern "C" size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t 
 namespace spice {
 namespace {
 
-// The norm of the call's gradients and the record from it.
-int norm_and_record(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, RecordArgs &a, double *part,
-                    hipStream_t s) {
-    if (few(numel, count, table_entries<1>()))
-        return dtype == 0   ? launch_norm_here<float>(grads, numel, count, a, s)
-               : dtype == 1 ? launch_norm_here<_Float16>(grads, numel, count, a, s)
-                            : launch_norm_here<__bf16>(grads, numel, count, a, s);
-    const int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, 4, a.inf, part, s)
-                   : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, 2, a.inf, part, s)
-                                : launch_norm<__bf16>(grads, numel, count, 2, a.inf, part, s);
-    if (rc) return rc;
+// The record from the items' sums.
+int record_of(RecordArgs &a, const double *part, const int64_t *numel, int32_t count, hipStream_t s) {
     a.part = part;
     a.parts = item_count(numel, count, item_elements(numel, count));
     grad_record_kernel<<<1, kOptFold, 0, s>>>(a);
@@ -502,6 +503,35 @@ int norm_and_record(void *const *grads, const int64_t *numel, int32_t count, int
     return SPICE_OK;
 }
 
+// The norm of the call's gradients and the record from it.
+int norm_and_record(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, RecordArgs &a, double *part,
+                    hipStream_t s) {
+    if (few(numel, count, table_entries<1>()))
+        return dtype == 0   ? launch_norm_here<float>(grads, numel, count, a, s)
+               : dtype == 1 ? launch_norm_here<_Float16>(grads, numel, count, a, s)
+                            : launch_norm_here<__bf16>(grads, numel, count, a, s);
+    const int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, a.inf, part, s)
+                   : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, a.inf, part, s)
+                                : launch_norm<__bf16>(grads, numel, count, a.inf, part, s);
+    if (rc) return rc;
+    return record_of(a, part, numel, count, s);
+}
+
+// The same over tensors of several types: each type's launches leave their part of the items' sums, joined in fp64 like the
+// rest.  (Norms per type, rounded to fp32 and joined there: squares of 3e19 overflow, and of 3e-25 vanish.)
+int norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *numel, int32_t count, RecordArgs &a, double *part,
+                  hipStream_t s) {
+    const uint32_t each = item_elements(numel, count);
+    for (int32_t dtype = 0; dtype <= 2; ++dtype) {
+        const OfType of = {dtypes, dtype};
+        const int rc = dtype == 0   ? launch_norm<float>(grads, numel, count, a.inf, part, s, of)
+                       : dtype == 1 ? launch_norm<_Float16>(grads, numel, count, a.inf, part, s, of)
+                                    : launch_norm<__bf16>(grads, numel, count, a.inf, part, s, of);
+        if (rc) return rc;
+        part += item_count(numel, count, each, of);
+    }
+    return record_of(a, part - item_count(numel, count, each), numel, count, s);
+}
 bool norm_ok(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type, float max_norm,
              const float *record, const void *workspace) {
     return dtype >= 0 && dtype <= 2 && counts_ok(numel, count) && pointers_ok(grads, numel, count, type_bytes(dtype)) && record &&
@@ -526,6 +556,17 @@ extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t
     if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
     RecordArgs a = norm_record(norm_type, max_norm, record);
     return norm_and_record(grads, numel, count, dtype, a, (double *)workspace, (hipStream_t)stream);
+}
+
+extern "C" int spice_grad_norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *numel, int32_t count,
+                                        int32_t norm_type, float max_norm, float *record, void *workspace, size_t workspace_bytes,
+                                        void *stream) {
+    if (!norm_ok(grads, numel, count, 1, norm_type, max_norm, record, workspace) || (count && !dtypes)) return SPICE_ERR_ARG;
+    for (int32_t i = 0; i < count; ++i)
+        if (dtypes[i] < 0 || dtypes[i] > 2 || !pointers_ok(grads + i, numel + i, 1, type_bytes(dtypes[i]))) return SPICE_ERR_ARG;
+    if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
+    RecordArgs a = norm_record(norm_type, max_norm, record);
+    return norm_of_types(grads, dtypes, numel, count, a, (double *)workspace, (hipStream_t)stream);
 }
 
 extern "C" int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,

@@ -1112,9 +1112,11 @@ at::ScalarType float_type(const Tensor &t, const char *name) {
 struct TensorTable {
     std::vector<void *> p;
     std::vector<int64_t> n;
+    std::vector<int32_t> types;     // of tensors of several types
 };
 
-void fill_table(TensorTable &t, const TensorList &ts, const char *name, const Tensor &like, at::ScalarType type) {
+// type: every tensor's; none: each its own.
+void fill_table(TensorTable &t, const TensorList &ts, const char *name, const Tensor &like, c10::optional<at::ScalarType> type) {
     const c10::Device device = like.device();
     t.p.reserve(ts.size());
     t.n.reserve(ts.size());
@@ -1122,7 +1124,8 @@ void fill_table(TensorTable &t, const TensorList &ts, const char *name, const Te
         const Tensor &x = ts[i];
         TORCH_CHECK(x.is_cuda(), name, " is on ", x.device(),
                     "; the MI355X path has no CPU implementation (move the tensor to a HIP device)");
-        TORCH_CHECK_TYPE(x.scalar_type() == type, name, " must be ", type, ", got ", x.scalar_type());
+        TORCH_CHECK_TYPE(!type.has_value() || x.scalar_type() == *type, name, " must be ", *type, ", got ", x.scalar_type());
+        if (!type.has_value()) t.types.push_back(type_code(float_type(x, name)));
         TORCH_CHECK(x.device() == device, name, " is on ", x.device(), ", expected ", device);
         TORCH_CHECK_VALUE(x.is_contiguous() || x.is_non_overlapping_and_dense(), name,
                           " must be dense (contiguous in some order of its axes)");
@@ -1175,18 +1178,24 @@ Tensor norm_workspace(const std::vector<int64_t> &n, const Tensor &like) {
     return at::empty({(int64_t)spice_grad_norm_workspace_bytes(n.data(), (int32_t)n.size())}, like.options().dtype(at::kByte));
 }
 
-Tensor grad_norm(const TensorList &grads, double max_norm, bool inf) {
+Tensor grad_norm(const TensorList &grads, double max_norm, bool inf, bool any_type) {
     TORCH_CHECK_VALUE(!grads.empty(), "grad_norm: no tensors");
     const Tensor &like = grads[0];
     const at::ScalarType type = float_type(like, "grads");
     TensorTable g;
-    fill_table(g, grads, "grads", like, type);
+    fill_table(g, grads, "grads", like, any_type ? c10::nullopt : c10::make_optional(type));
     TORCH_CHECK_VALUE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
     c10::DeviceGuard guard(like.device());
     Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws = norm_workspace(g.n, like);
-    check_rc(spice_grad_norm(g.p.data(), g.n.data(), (int32_t)g.n.size(), type_code(type), inf ? SPICE_NORM_INF : SPICE_NORM_L2,
-                             (float)max_norm, record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
-             "spice_grad_norm");
+    const int32_t norm = inf ? SPICE_NORM_INF : SPICE_NORM_L2;
+    if (any_type && std::any_of(g.types.begin(), g.types.end(), [&](int32_t t) { return t != g.types[0]; }))
+        check_rc(spice_grad_norm_of_types(g.p.data(), g.types.data(), g.n.data(), (int32_t)g.n.size(), norm, (float)max_norm,
+                                          record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
+                 "spice_grad_norm_of_types");
+    else
+        check_rc(spice_grad_norm(g.p.data(), g.n.data(), (int32_t)g.n.size(), type_code(type), norm, (float)max_norm,
+                                 record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
+                 "spice_grad_norm");
     return record;
 }
 
@@ -1347,7 +1356,7 @@ TORCH_LIBRARY(spice, m) {
     m.def("policy_loss(Tensor logits, Tensor labels, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, int class_dim, "
           "float temperature, int ignore_index, float clip_low, float clip_high, float kl_weight, int reduction, bool want_grad, "
           "float grad_scale, bool want_weight) -> Tensor[]", &policy_loss);
-    m.def("grad_norm(Tensor[] grads, float max_norm, bool inf) -> Tensor", &grad_norm);
+    m.def("grad_norm(Tensor[] grads, float max_norm, bool inf, bool any_type=False) -> Tensor", &grad_norm);
     m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, float max_norm, bool inf, Tensor? record) -> Tensor", &grad_clip);
     m.def("adam_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)? step, "
           "int host_step, float lr, float beta1, float beta2, float eps, float weight_decay, bool decoupled, float max_norm, "

@@ -949,11 +949,11 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logprobs: torch.
 # gradient norm, clipping, Adam
 
 
-def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, any_type: bool = False) -> torch.Tensor:
     """Norm over all elements of all tensors (2, or float("inf"): the largest magnitude), a device scalar; no host
-    synchronisation.  The tensors: one device, one type (fp32 / fp16 / bf16), dense in any order of their axes.  Squares
-    are summed in fp64 in a fixed order."""
-    return spice_ops().grad_norm(grads, 0.0, _norm_inf(norm_type))[0]
+    synchronisation.  The tensors: one device, one type (fp32 / fp16 / bf16; with any_type each its own of them), dense
+    in any order of their axes.  Squares are summed in fp64 in a fixed order, over all types."""
+    return spice_ops().grad_norm(grads, 0.0, _norm_inf(norm_type), any_type)[0]
 
 
 def _norm_inf(norm_type: float) -> bool:

@@ -4,7 +4,7 @@ loop steps torch's Adam without clipping (pruning/trainer.py:160-228); the train
 `max_grad_norm` is set."""
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -43,13 +43,6 @@ class ClippedAdam(torch.optim.Optimizer):
         # the update walks a parameter and its gradient in memory order
         return p.grad if p.grad.stride() == p.stride() or p.numel() <= 1 else torch.empty_like(p).copy_(p.grad)
 
-    def _norm(self, grads: List[torch.Tensor]) -> torch.Tensor:
-        kinds: Dict[torch.dtype, list] = {}
-        for g in grads:
-            kinds.setdefault(g.dtype, []).append(g)
-        norms = [ops.grad_norm(k) for k in kinds.values()]
-        return norms[0] if len(norms) == 1 else torch.linalg.vector_norm(torch.stack(norms))
-
     @torch.no_grad()
     def step(self, closure=None):
         if torch.cuda.is_current_stream_capturing():
@@ -68,7 +61,7 @@ class ClippedAdam(torch.optim.Optimizer):
             return loss
         norm = None
         if self.max_grad_norm is not None and len(sets) > 1:
-            norm = self._norm([g for s in sets.values() for _, g in s])
+            norm = ops.grad_norm([g for s in sets.values() for _, g in s], any_type=True)
         for (i, steps, _), members in sets.items():
             group, states = self.param_groups[i], [self.state[p] for p, _ in members]
             got = ops.adam_step([p for p, _ in members], [g for _, g in members], [s["exp_avg"] for s in states],

@@ -291,3 +291,29 @@ def test_another_stream(dev):
             norms.append(ops.clip_grad_norm(grads, 1.0))
     torch.cuda.synchronize()
     assert all(torch.equal(n, want) for n in norms) and all(torch.equal(a, b) for a, b in zip(*sets))
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e19, 1e-25])
+def test_one_norm_over_parameters_of_two_types(dev, scale):
+    """bf16 weights beside fp32 ones: the norm is joined over both types in fp64, where squares of 1e19 and of 1e-25 are held;
+    the step that it clips is the 64-bit one.  (g' rounds with the norm, the factor and the product: the 3 u of _adam_tol.)"""
+    limit, lr = 0.5, 3e-3
+    params = [p for t in (torch.bfloat16, torch.float32, torch.float16) for p in _tensors([300, 7, 40000], t, 21)]
+    small = 1.0 if scale == 1.0 else 1e-3 if scale > 1.0 else 0.0     # (what fp16 holds)
+    grads = [g for t, s in ((torch.bfloat16, scale), (torch.float32, scale), (torch.float16, small)) for g in _tensors([300, 7, 40000], t, 22, s)]
+    leaves = [torch.nn.Parameter(p.to(dev)) for p in params]
+    for p, g in zip(leaves, grads):
+        p.grad = g.to(dev)
+    opt = ClippedAdam(leaves, lr=lr, max_grad_norm=limit)
+    opt.step()
+    norm = ot.grad_norm(grads)
+    assert abs(opt.last_grad_norm.item() - norm.item()) <= 2 * U * norm.item()
+    factor = ot.clip_factor(norm, limit).item()
+    for p, g, leaf in zip(params, grads, leaves):
+        z = torch.zeros(p.shape, dtype=torch.float64)
+        new = ot.adam(p, g, z, z, 1, factor, lr=lr)
+        tol = _adam_tol(p.double(), g.double(), z, z, new, 1, factor, lr, (0.9, 0.999), 1e-8, 0.0, p.dtype)
+        state = opt.state[leaf]
+        # (a moment below fp32's normal range is held to its least value)
+        for a, w, t in zip((leaf.detach(), state["exp_avg"], state["exp_avg_sq"]), new, tol):
+            assert ((a.cpu().double() - w).abs() <= t + 2.0 ** -149).all()

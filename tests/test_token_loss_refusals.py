@@ -184,3 +184,20 @@ def test_oracle_gradients_against_differences(loss):
     v = x.clone().requires_grad_(True)
     got, = torch.autograd.grad(f(v), v)
     assert (got - _differences(f, x)).abs().max() <= 1e-8
+
+
+def test_c_abi_checks_the_types_of_a_mixed_norm():
+    L = nat.lib()
+    n = _counts(8, 8, 8)
+    need = L.spice_grad_norm_workspace_bytes(n, 3)
+
+    def norm(p=(16, 66, 130), types=(0, 1, 2), kind=0, limit=1.0, record=16, ws=16, size=need):
+        return L.spice_grad_norm_of_types(_table(*p), (ctypes.c_int32 * 3)(*types) if types else None, n, 3, kind, limit, record, ws,
+                                          size, None)
+
+    for bad in (dict(types=(0, 1, 3)), dict(types=(-1, 1, 2)), dict(types=None), dict(p=(18, 66, 130)), dict(p=(16, 67, 130)),
+                dict(p=(16, None, 130)), dict(kind=2), dict(limit=-1.0), dict(record=None), dict(ws=None), dict(ws=12)):
+        assert norm(**bad) == nat.ERR_ARG, bad
+    assert norm(size=need - 1) == nat.ERR_WORKSPACE
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        ops.grad_norm([F, F.half()], any_type=True)
