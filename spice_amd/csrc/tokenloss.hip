@@ -512,7 +512,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
             w = kStats ? a.weight[n * a.w_sn + l * a.w_sl] : policy_term(a.policy, in, (float)logp).dlogp * share;
         if (!kStats && a.weight_out && lane == 0) a.weight_out[at] = w;
         const float shift = shift_of(m);
-        w *= a.t.inv * a.host_scale * (kStats && a.scale ? *a.scale : 1.f);
+        if (kind == kCounted) w *= a.t.inv * a.host_scale * (kStats && a.scale ? *a.scale : 1.f);   // (elsewhere 0 under any factor)
         const float each = kind == kCounted ? -w / s : w;
         float v[K];
         if (kind == kCounted) {
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
                 w = policy_term(a.policy, in, (float)logp).dlogp * (a.share ? a.share[n] : share_here<kBlock>(a, n, counts));
             if (a.weight_out && threadIdx.x == 0) a.weight_out[at] = w;
             const float shift = shift_of(m);
-            w *= a.t.inv * a.host_scale;
+            if (kind == kCounted) w *= a.t.inv * a.host_scale;
             const float each = kind == kCounted ? -w / s : w;
             for (int64_t c0 = threadIdx.x * K; c0 < classes; c0 += kBlock * K) {
                 float v[K];
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
                 w[k] = kind[k] == kBad ? NAN : 0.f;
             }
             if (kGrad) {
-                w[k] *= out_scale;
+                if (kind[k] == kCounted) w[k] *= out_scale;
                 each[k] = kind[k] == kCounted ? -w[k] / s[k] : w[k];
             }
         }
@@ -1041,7 +1041,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
             if (MODE == kModePolicyGrad && a.weight_out && q >= dup) a.weight_out[at] = w;
         }
         if (kGrad) {
-            w *= a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f);
+            if (yq >= 0) w *= a.t.inv * a.host_scale * (a.scale ? *a.scale : 1.f);
             top_of[q] = shift_of(m);
             w_of[q] = w;
             each_of[q] = yq >= 0 ? -w / s : w;

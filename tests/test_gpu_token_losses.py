@@ -602,3 +602,29 @@ def test_every_second_position_of_many(dev, c, dtype):
     _close(out[0], -a64.sum(), (a64.abs() * (2 * tl + 4 * U)).sum() + 4 * U, "total")
     p64, = torch.autograd.grad(-(ot.token_logprobs(v, y, **how)[0] * a64).sum(), v)
     _close(pg, p64, _grad_tol(x, p64, a64.abs() * (1 + 2 * tl + 4 * U), 1, 1.0) + (a64.abs() * (2 * tl + 4 * U)).unsqueeze(1), "policy grad")
+
+
+@pytest.mark.parametrize("layout, positions, c", [("last", (6,), 5000), ("last", (40,), 9), ("last", (5,), 700), ("last", (4,), 90001),
+                                                  ("planes", (8, 12), 21), ("planes", (5, 7), 70), ("planes", (6,), 3001)])
+@pytest.mark.parametrize("factor", [math.inf, math.nan])
+def test_ignored_positions_stay_zero_under_any_factor(dev, layout, positions, c, factor):
+    """An infinite or NaN factor from above (a loss scale that ran over) reaches the counted positions alone, in every kernel."""
+    x, y, d, ignore = _inputs(layout, 2, positions, c, torch.float32, seed=41)
+    y.reshape(-1)[:3] = torch.tensor([ignore, 1, ignore])
+    keep = y != ignore
+    how = dict(class_dim=d, ignore_index=ignore)
+    xd, yd = x.to(dev), y.to(dev)
+    _, stats = ops.token_logprobs(xd, yd, **how)
+    old, adv = torch.zeros(y.shape, device=dev), torch.ones(2, device=dev)
+    far = torch.full((1,), factor, device=dev)
+    leaf = xd.clone().requires_grad_(True)
+    total = ClippedPolicyLoss(kl_weight=0.1, **how)(leaf, yd, old, adv, ref_logprobs=old)["total"]
+    grads = [ops.token_logprobs_grad(xd, yd, stats, torch.ones(y.shape, device=dev), device_scale=far, **how),
+             ops.token_logprobs_grad(xd, yd, stats, adv, scale=factor, **how),
+             ops.policy_loss(xd, yd, old, adv, ref_logprobs=old, kl_weight=0.1, want_grad=True, grad_scale=factor, **how)[2],
+             ops.preference_loss(xd, yd, old, want_grad=True, grad_scale=factor, **how)[2],
+             torch.autograd.grad(far[0] * total, leaf)[0]]
+    for k, g in enumerate(grads):
+        g = _last(g, d).cpu()
+        assert (g[~keep] == 0).all(), k
+        assert not torch.isfinite(g[keep]).all(-1).any(), k
