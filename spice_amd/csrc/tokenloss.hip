@@ -96,6 +96,17 @@ __device__ __forceinline__ int label_kind(int64_t y, int64_t ignore, int64_t c) 
 // A maximum to subtract: -inf (nothing finite seen) would make -inf - -inf out of an excluded class.
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+// The sum of a few exponentials, log2 K roundings deep.  Longer sums add such trees up in fp64: once a sum in fp32 has reached
+// 1, every class below 2^-25 adds nothing to it (32,000 classes 17 below the top: logp a quarter off).
+template <int K>
+__device__ __forceinline__ double tree_sum(float (&e)[K]) {
+#pragma unroll
+    for (int o = K / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < o; ++k) e[k] += e[k + o];
+    return (double)e[0];
+}
+
 // What a sum of exponentials over maximum m is worth over maximum `to` >= m: nothing where nothing finite was seen (its
 // place holder 0 may lie far above `to`).
 __device__ __forceinline__ float rescale(float m, float to, Temper t) { return m == -INFINITY ? 0.f : exp_of(m - to, t); }
@@ -915,14 +926,15 @@ constexpr int kSplitTile = 64;
 
 template <typename T, int VEC, int HOLD, int MODE>
 __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kernel(TokArgs a, int64_t tiles, int64_t first) {
-    constexpr int RUN = kSplitTile / VEC, GROUPS = kTokThreads / RUN, kStep = HOLD > 0 ? HOLD : 8;
+    constexpr int RUN = kSplitTile / VEC, GROUPS = kTokThreads / RUN, kStep = HOLD > 0 ? HOLD : 8, kTree = 4;
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
     constexpr bool kStats = MODE == kModeGrad;
     constexpr bool kOnce = MODE == kModePolicyGrad && HOLD > 0 && VEC > 1;
     constexpr int K = MODE == kModePreference ? 2 : 4;
     constexpr bool kSums = MODE == kModePreference || MODE == kModePolicy || MODE == kModePolicyGrad;
     typedef typename GroupOf<T, VEC>::type G;
-    __shared__ float2 part[GROUPS][kSplitTile];         // (max, sum) of a group's classes
+    __shared__ float part_max[GROUPS][kSplitTile];      // of a group's classes
+    __shared__ double part_sum[GROUPS][kSplitTile];
     __shared__ float at_label[kSplitTile], top_of[kSplitTile], each_of[kSplitTile], w_of[kSplitTile];
     __shared__ int label_of[kSplitTile];                // >= 0: counted; -1: ignored; -2: no class
     __shared__ int counts[kTokThreads / kWave];
@@ -959,11 +971,12 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
     G raw[kStep];
     float v[VEC];
     if (!kStats) {
-        float m[VEC], s[VEC];
+        float m[VEC];
+        double s[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
             m[k] = -INFINITY;
-            s[k] = 0.f;
+            s[k] = 0.0;
         }
         if (any) {
             for (int32_t c0 = group; c0 < classes; c0 += kStep * GROUPS) {
@@ -985,22 +998,31 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
                     }
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    s[k] *= rescale(m[k], top[k], a.t);
+                    s[k] *= (double)rescale(m[k], top[k], a.t);
                     m[k] = top[k];
                 }
                 forget_groups(raw);
 #pragma unroll
-                for (int j = 0; j < kStep; ++j)
-                    if (c0 + j * GROUPS < classes) {
-                        values<T, VEC>(raw[j], v);
+                for (int j0 = 0; j0 < kStep; j0 += kTree) {
+                    float e[VEC][kTree] = {};
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
-                    }
+                    for (int j = 0; j < kTree; ++j)
+                        if (c0 + (j0 + j) * GROUPS < classes) {
+                            values<T, VEC>(raw[j0 + j], v);
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) e[k][j] = exp_of(v[k] - shift_of(m[k]), a.t);
+                        }
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) s[k] += tree_sum(e[k]);
+                }
                 if (HOLD > 0) break;
             }
         }
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) part[group][pos + k] = make_float2(m[k], s[k]);
+        for (int k = 0; k < VEC; ++k) {
+            part_max[group][pos + k] = m[k];
+            part_sum[group][pos + k] = s[k];
+        }
         __syncthreads();
     }
     double sums[K];
@@ -1018,9 +1040,9 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
             }
             w = yq >= 0 ? a.weight[n * a.w_sn + l * a.w_sl] : yq == -2 ? NAN : 0.f;
         } else {
-            for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, part[g][q].x);
+            for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, part_max[g][q]);
             double sum = 0.0;
-            for (int g = 0; g < GROUPS; ++g) sum += (double)(part[g][q].y * rescale(part[g][q].x, m, a.t));
+            for (int g = 0; g < GROUPS; ++g) sum += part_sum[g][q] * (double)rescale(part_max[g][q], m, a.t);
             s = (float)sum;
             const double exact = yq >= 0 ? logp_of(at_label[q] - shift_of(m), sum, a.t) : yq == -2 ? (double)NAN : 0.0;
             if (q >= dup) leave_logp(a, at, exact, m, s, 0.f);

@@ -628,3 +628,51 @@ def test_ignored_positions_stay_zero_under_any_factor(dev, layout, positions, c,
         g = _last(g, d).cpu()
         assert (g[~keep] == 0).all(), k
         assert not torch.isfinite(g[keep]).all(-1).any(), k
+
+
+def _long_tail(layout, n, positions, c, t=17.0):
+    """One class at 0 and the others at -t in every position, and what the label's log-probability and a tail class's softmax are:
+    every tail class is below half a step of a sum that has reached 1."""
+    x = torch.full((n, *positions, c), -t)
+    top = torch.randint(0, c, (n, *positions), generator=torch.Generator().manual_seed(c))
+    x.scatter_(-1, top.unsqueeze(-1), 0.0)
+    tail = math.exp(-t)
+    return (x.movedim(-1, 1).contiguous() if layout == "planes" else x), top, -math.log1p((c - 1) * tail), tail / (1 + (c - 1) * tail)
+
+
+# A tail class's exponential: exponent t log2(e) rounds by u of 24.5 (17 u of the value), the instruction 2 u: 20 u; trees of
+# them, a rescaling and the joins 7 u: the tail's sum T, and with it log(1 + T), is off by at most 27 u of itself, and rounds
+# to fp32 by u.  The tree of at most 16 exponentials that holds the 1 rounds four times at values below 2: 4 u.  What a chain of
+# fp32 additions holds back shows as hundreds of u.
+TAIL, TREE = 32, 4
+
+
+def _check_long_tail(dev, x, y, d, logp, p):
+    """x on the host, or a view on the device."""
+    x = x.to(dev)
+    how = dict(class_dim=d, ignore_index=-100)
+    got, stats = ops.token_logprobs(x, y.to(dev), **how)
+    assert (got.double() - logp).abs().max().item() <= TAIL * U * abs(logp) + TREE * U
+    out, again, _ = ops.policy_loss(x, y.to(dev), torch.full(y.shape, logp, device=dev), torch.ones(x.shape[0], device=dev), **how)
+    assert (again.double() - logp).abs().max().item() <= TAIL * U * abs(logp) + TREE * U
+    # the statistics' sum: the tree's error, that of the tail (less than u) and its rounding; a class's softmax by its exponential's
+    # 20 u, the sum's, the quotient's and the product's
+    s = stats[..., 1].double() * torch.exp(stats[..., 0].double())
+    assert (s * math.exp(logp) - 1).abs().max().item() <= (TREE + 2) * U
+    grad = _last(ops.token_logprobs_grad(x, y.to(dev), stats, torch.ones(y.shape, device=dev), **how), d)
+    want = torch.full((x.shape[0] * y[0].numel(), grad.shape[-1]), -p, device=dev, dtype=torch.float64)
+    want.scatter_(-1, y.to(dev).reshape(-1, 1), -math.expm1(logp))
+    # (at the label 1 - p is taken in fp32: the sum's error and 2 u of 1)
+    assert ((grad.double().reshape(want.shape) - want).abs() <= (TAIL + TREE) * U * p + (want > 0) * (TREE + 4) * U).all()
+
+
+@pytest.mark.parametrize("c, l, step", [(32000, 520, 1), (32001, 260, 2), (5000, 600, 1), (5000, 600, 2), (150, 600, 1), (250, 600, 1),
+                                        (60, 600, 2), (40, 600, 2)])
+def test_planes_of_many_classes_keep_a_long_tail(dev, c, l, step):
+    """More positions than a workgroup each would take, neighbouring ones and every second one."""
+    n = 1 if l > 512 else 2
+    x, y, logp, p = _long_tail("planes", n, (l,), c)
+    x = x.to(dev)
+    if step > 1:
+        x = torch.stack([x, torch.zeros_like(x)], -1)[..., 0]
+    _check_long_tail(dev, x, y, 1, logp, p)
