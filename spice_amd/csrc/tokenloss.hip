@@ -96,17 +96,6 @@ __device__ __forceinline__ int label_kind(int64_t y, int64_t ignore, int64_t c) 
 // A maximum to subtract: -inf (nothing finite seen) would make -inf - -inf out of an excluded class.
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// The sum of a few exponentials, log2 K roundings deep.  Longer sums add such trees up in fp64: once a sum in fp32 has reached
-// 1, every class below 2^-25 adds nothing to it (32,000 classes 17 below the top: logp a quarter off).
-template <int K>
-__device__ __forceinline__ double tree_sum(float (&e)[K]) {
-#pragma unroll
-    for (int o = K / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < o; ++k) e[k] += e[k + o];
-    return (double)e[0];
-}
-
 // What a sum of exponentials over maximum m is worth over maximum `to` >= m: nothing where nothing finite was seen (its
 // place holder 0 may lie far above `to`).
 __device__ __forceinline__ float rescale(float m, float to, Temper t) { return m == -INFINITY ? 0.f : exp_of(m - to, t); }
@@ -926,7 +915,7 @@ constexpr int kSplitTile = 64;
 
 template <typename T, int VEC, int HOLD, int MODE>
 __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kernel(TokArgs a, int64_t tiles, int64_t first) {
-    constexpr int RUN = kSplitTile / VEC, GROUPS = kTokThreads / RUN, kStep = HOLD > 0 ? HOLD : 8, kTree = 4;
+    constexpr int RUN = kSplitTile / VEC, GROUPS = kTokThreads / RUN, kStep = HOLD > 0 ? HOLD : 8;
     constexpr bool kGrad = MODE == kModeGrad || MODE == kModePolicyGrad;
     constexpr bool kStats = MODE == kModeGrad;
     constexpr bool kOnce = MODE == kModePolicyGrad && HOLD > 0 && VEC > 1;
@@ -1002,19 +991,18 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
                     m[k] = top[k];
                 }
                 forget_groups(raw);
+                // Four short chains a position, joined in fp64: once a sum in fp32 has reached 1, every class below 2^-25 adds
+                // nothing to it (one chain over 32,000 classes 17 below the top: logp a quarter off).
+                float e[VEC][4] = {};
 #pragma unroll
-                for (int j0 = 0; j0 < kStep; j0 += kTree) {
-                    float e[VEC][kTree] = {};
+                for (int j = 0; j < kStep; ++j)
+                    if (c0 + j * GROUPS < classes) {
+                        values<T, VEC>(raw[j], v);
 #pragma unroll
-                    for (int j = 0; j < kTree; ++j)
-                        if (c0 + (j0 + j) * GROUPS < classes) {
-                            values<T, VEC>(raw[j0 + j], v);
+                        for (int k = 0; k < VEC; ++k) e[k][j % 4] += exp_of(v[k] - shift_of(m[k]), a.t);
+                    }
 #pragma unroll
-                            for (int k = 0; k < VEC; ++k) e[k][j] = exp_of(v[k] - shift_of(m[k]), a.t);
-                        }
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) s[k] += tree_sum(e[k]);
-                }
+                for (int k = 0; k < VEC; ++k) s[k] += (double)(e[k][0] + e[k][1]) + (double)(e[k][2] + e[k][3]);
                 if (HOLD > 0) break;
             }
         }
