@@ -158,6 +158,29 @@ __device__ __forceinline__ PolicyIn policy_in(const Policy &p, int64_t at, int64
     return PolicyIn{p.adv[n * p.adv_sn + l * p.adv_sl], p.old_logp[at], p.ref ? p.ref[at] : 0.f};
 }
 
+// exp(q) - q - 1 and exp(q) - 1.  Where a policy has hardly left its reference the first is about q^2 / 2, which differences of
+// numbers near 1 would round to steps of 2^-24 (2^21 positions 1e-4 apart: a mean of -4e-9 for 5e-9): for |q| <= 1 its series,
+// q^2 sum_n q^n / (n + 2)! up to q^11 / 11! (the next term is below 2^-27 of it).
+__device__ __forceinline__ void far_of(float q, float &far, float &e1) {
+    if (fabsf(q) <= 1.f) {
+        float r = 1.f / 39916800.f;
+        r = __builtin_fmaf(r, q, 1.f / 3628800.f);
+        r = __builtin_fmaf(r, q, 1.f / 362880.f);
+        r = __builtin_fmaf(r, q, 1.f / 40320.f);
+        r = __builtin_fmaf(r, q, 1.f / 5040.f);
+        r = __builtin_fmaf(r, q, 1.f / 720.f);
+        r = __builtin_fmaf(r, q, 1.f / 120.f);
+        r = __builtin_fmaf(r, q, 1.f / 24.f);
+        r = __builtin_fmaf(r, q, 1.f / 6.f);
+        r = __builtin_fmaf(r, q, 0.5f);
+        far = q * q * r;
+        e1 = q + far;
+    } else {
+        e1 = expf(q) - 1.f;
+        far = e1 - q;
+    }
+}
+
 __device__ __forceinline__ PolicyTerm policy_term(const Policy &p, const PolicyIn &in, float logp) {
     PolicyTerm r;
     const float a = in.adv;
@@ -170,9 +193,9 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy &p, const PolicyI
     r.far = 0.f;
     if (p.ref) {
         const float q = in.ref - logp;   // log of how much likelier the reference finds the label
-        const float e = expf(q);
-        r.far = e - q - 1.f;
-        if (p.kl != 0.f) r.dlogp += p.kl * (1.f - e);
+        float e1;                        // exp(q) - 1
+        far_of(q, r.far, e1);
+        if (p.kl != 0.f) r.dlogp -= p.kl * e1;
     }
     return r;
 }

@@ -676,3 +676,32 @@ def test_planes_of_many_classes_keep_a_long_tail(dev, c, l, step):
     if step > 1:
         x = torch.stack([x, torch.zeros_like(x)], -1)[..., 0]
     _check_long_tail(dev, x, y, 1, logp, p)
+
+
+@pytest.mark.parametrize("layout, positions, c", [("last", (4000,), 9), ("last", (500,), 1000), ("last", (3,), 90001), ("planes", (80, 90), 21),
+                                                  ("planes", (40, 50), 150), ("planes", (5,), 3001)])
+@pytest.mark.parametrize("apart", [1e-5, 1e-4, 1e-2, 0.5, 3.0])
+def test_kl_of_a_policy_near_its_reference(dev, layout, positions, c, apart):
+    """exp(q) - q - 1 is about q^2 / 2: a policy that has hardly left its reference.  Against the formula in 64 bits at the
+    log-probabilities that the call gives back: q = ref - logp rounds by u of itself, which the derivative exp(q) - 1 carries;
+    the value itself by at most 14 u (ten steps of a series whose terms shrink, or the exponential's 3 u and two differences);
+    exp(q) - 1 by u q exp(q) and 10 u."""
+    x, y, d, ignore = _inputs(layout, 2, positions, c, torch.float32, seed=51)
+    how = dict(class_dim=d, ignore_index=ignore)
+    keep = y != ignore
+    xd, yd = x.to(dev), y.to(dev)
+    logp = ops.token_logprobs(xd, yd, **how)[0].cpu()
+    ref = (logp.double() + apart * torch.randn(y.shape, generator=torch.Generator().manual_seed(52), dtype=torch.float64)).float()
+    out, again, grad = ops.policy_loss(xd, yd, logp.to(dev), torch.zeros(2, device=dev), ref_logprobs=ref.to(dev), kl_weight=0.5,
+                                       want_grad=True, grad_scale=float(keep.sum()), **how)
+    q = torch.where(keep, ref.double() - again.cpu().double(), 0.0)
+    far = torch.expm1(q) - q
+    rough = 2.0 ** -52 * q.abs()         # (of this line's own subtraction)
+    want = far.sum() / keep.sum()
+    assert out[2] >= 0 and abs(out[2].item() - want.item()) <= ((14 * U * far + U * (q * torch.expm1(q)).abs() + rough).sum() / keep.sum()).item() + U * want.item()
+    w = -0.5 * torch.expm1(q)
+    v = x.double().requires_grad_(True)
+    g64, = torch.autograd.grad((ot.token_logprobs(v, y, **how)[0] * w).sum(), v)
+    # the weight: 0.5 (1 - exp(q)) and the share's product and rounding
+    extra = (w.abs() * 10 * U + 0.5 * U * q.abs() * torch.exp(q)).unsqueeze(d if d == 1 else -1)
+    _close(grad, g64, _grad_tol(x, g64, w.abs(), d, 1.0) + extra, "grad")
