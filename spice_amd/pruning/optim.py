@@ -11,6 +11,10 @@ import torch
 from .. import ops
 
 
+# what torch.optim.Adam's groups hold beside this class's options
+_ADAM_ONLY = {"amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"}
+
+
 class ClippedAdam(torch.optim.Optimizer):
     """Parameters and gradients fp32 / fp16 / bf16 on one HIP device, moments fp32.  `decoupled`: weight decay as
     p *= 1 - lr * weight_decay, else added to the gradient (torch.optim.Adam's way).  max_grad_norm: the gradients of
@@ -33,8 +37,37 @@ class ClippedAdam(torch.optim.Optimizer):
         if not state:
             state["step"] = 0
             for key in ("exp_avg", "exp_avg_sq"):
-                state[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                state[key] = self._moment_of(p)
         return state
+
+    @staticmethod
+    def _moment_of(p: torch.Tensor) -> torch.Tensor:
+        return torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format, requires_grad=False)
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Also a state of torch.optim.Adam or AdamW, but for amsgrad's and maximize's.  The moments stay fp32 (the base
+        class would cast them to their parameters' type) and take their parameters' order of axes."""
+        groups = []
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("ClippedAdam has neither amsgrad nor maximize")
+            decoupled = group.get("decoupled", group.get("decoupled_weight_decay", self.defaults["decoupled"]))
+            groups.append({**{k: v for k, v in group.items() if k not in _ADAM_ONLY}, "decoupled": bool(decoupled)})
+        keys = [key for group in groups for key in group["params"]]
+        loaded = {}
+        for key, p in zip(keys, (p for group in self.param_groups for p in group["params"])):
+            saved = state_dict["state"].get(key)
+            if not saved:
+                continue
+            if not {"step", "exp_avg", "exp_avg_sq"} <= set(saved):
+                raise ValueError(f"the state of parameter {key} is not Adam's: {sorted(saved)}")
+            loaded[p] = {"step": int(saved["step"])}
+            for name in ("exp_avg", "exp_avg_sq"):
+                if saved[name].shape != p.shape:
+                    raise ValueError(f"{name} of parameter {key} has shape {tuple(saved[name].shape)}, its parameter {tuple(p.shape)}")
+                loaded[p][name] = self._moment_of(p).copy_(saved[name])
+        super().load_state_dict({**state_dict, "state": {}, "param_groups": groups})
+        self.state.update(loaded)
 
     @staticmethod
     def _grad_of(p: torch.Tensor) -> torch.Tensor:

@@ -317,3 +317,32 @@ def test_one_norm_over_parameters_of_two_types(dev, scale):
         # (a moment below fp32's normal range is held to its least value)
         for a, w, t in zip((leaf.detach(), state["exp_avg"], state["exp_avg_sq"]), new, tol):
             assert ((a.cpu().double() - w).abs() <= t + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_steps_after_loading_are_the_uninterrupted_ones(dev, dtype):
+    """Three steps at once, and one, a saved state taken up by a model in channels-last order, then two: the same bits."""
+    start = [_tensors([4 * 3 * 2 * 5, 300], dtype, 31)[0].view(4, 3, 2, 5), _tensors([300], dtype, 32)[0]]
+    grads = [[t.view(4, 3, 2, 5) if k == 0 else t for k, t in enumerate(_tensors([120, 300], dtype, 33 + s, 0.1))] for s in range(3)]
+
+    def take(params, opt, these):
+        for gs in these:
+            for p, g in zip(params, gs):
+                p.grad = g.to(dev)
+            opt.step()
+
+    def model(values, **how):
+        return [torch.nn.Parameter(values[0].to(dev).contiguous(**how)), torch.nn.Parameter(values[1].to(dev))]
+
+    options = dict(lr=1e-2, weight_decay=0.1, max_grad_norm=0.5)
+    whole, first = model(start), model(start)
+    take(whole, ClippedAdam(whole, **options), grads)
+    opt = ClippedAdam(first, **options)
+    take(first, opt, grads[:1])
+    state = copy.deepcopy(opt.state_dict())
+    second = model([p.detach() for p in first], memory_format=torch.channels_last)
+    again = ClippedAdam(second, max_grad_norm=0.5)
+    again.load_state_dict(state)
+    take(second, again, grads[1:])
+    # (the norm's squares are added up in memory order: fp64, the same fp32 norm and factor)
+    assert all(torch.equal(a, b) for a, b in zip(whole, second))

@@ -201,3 +201,59 @@ def test_c_abi_checks_the_types_of_a_mixed_norm():
     assert norm(size=need - 1) == nat.ERR_WORKSPACE
     with pytest.raises(RuntimeError, match="no CPU implementation"):
         ops.grad_norm([F, F.half()], any_type=True)
+
+
+def _with_state(params, **options):
+    opt = ClippedAdam(params, **options)
+    for k, p in enumerate(params):
+        state = opt._state_of(p)
+        state["step"] = 3 + k
+        for j, key in enumerate(("exp_avg", "exp_avg_sq")):
+            state[key].copy_(torch.rand(p.shape, generator=torch.Generator().manual_seed(7 * k + j)))
+    return opt
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_loaded_moments_keep_their_precision_and_take_their_parameters_order(dtype):
+    make = lambda **how: [torch.nn.Parameter(torch.ones(4, 3, 2, 5, dtype=dtype).contiguous(**how)), torch.nn.Parameter(torch.ones(7, dtype=dtype))]  # noqa: E731
+    old, new = make(), make(memory_format=torch.channels_last)
+    a, b = _with_state(old, lr=2e-3, weight_decay=0.1, decoupled=True), ClippedAdam(new)
+    b.load_state_dict(a.state_dict())
+    for k, (p, q) in enumerate(zip(old, new)):
+        assert b.state[q]["step"] == 3 + k
+        for key in ("exp_avg", "exp_avg_sq"):
+            x, y = a.state[p][key], b.state[q][key]
+            assert y.dtype == torch.float32 and y.stride() == q.stride() and torch.equal(x, y) and x.data_ptr() != y.data_ptr()
+    assert b.param_groups[0]["lr"] == 2e-3 and b.param_groups[0]["decoupled"] and b.param_groups[0]["weight_decay"] == 0.1
+
+
+@pytest.mark.parametrize("kind, decoupled", [(torch.optim.Adam, False), (torch.optim.AdamW, True)])
+def test_a_state_of_torch_adam_is_taken_up(kind, decoupled):
+    p, q = torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(5))
+    a = kind([p], lr=5e-3, betas=(0.8, 0.95), weight_decay=0.2)
+    for k in range(3):
+        p.grad = torch.arange(5.0) + k
+        a.step()
+    torch.optim.lr_scheduler.ExponentialLR(a, 0.9)     # (its initial_lr stays in the groups)
+    b = ClippedAdam([q], max_grad_norm=1.0)
+    b.load_state_dict(a.state_dict())
+    assert b.state[q]["step"] == 3 and isinstance(b.state[q]["step"], int)
+    assert torch.equal(b.state[q]["exp_avg"], a.state[p]["exp_avg"]) and torch.equal(b.state[q]["exp_avg_sq"], a.state[p]["exp_avg_sq"])
+    group = b.param_groups[0]
+    assert (group["lr"], group["betas"], group["weight_decay"], group["decoupled"], group["initial_lr"]) == (5e-3, (0.8, 0.95), 0.2, decoupled, 5e-3)
+    assert not {"amsgrad", "maximize", "fused", "decoupled_weight_decay"} & set(group)
+
+
+def test_states_that_are_not_its_own_are_refused_as_a_whole():
+    p, q = torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(5))
+    sgd = torch.optim.SGD([p], lr=0.5, momentum=0.9)
+    p.grad = torch.ones(5)
+    sgd.step()
+    for state, text in ((sgd.state_dict(), "not Adam's"), (torch.optim.Adam([p], amsgrad=True).state_dict(), "amsgrad"),
+                        (torch.optim.Adam([p], maximize=True).state_dict(), "maximize"),
+                        (_with_state([torch.nn.Parameter(torch.ones(6))], lr=0.5).state_dict(), "shape"),
+                        (_with_state([p, torch.nn.Parameter(torch.ones(5))], lr=0.5).state_dict(), "parameter group")):
+        opt = ClippedAdam([q], lr=0.25)
+        with pytest.raises(ValueError, match=text):
+            opt.load_state_dict(state)
+        assert opt.param_groups[0]["lr"] == 0.25 and not opt.state[q]
