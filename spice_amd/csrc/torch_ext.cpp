@@ -879,6 +879,28 @@ Tensor conv3x3_bn_act(const Tensor &x, const Tensor &weight9, const Tensor &mean
     return out;
 }
 
+// ---- what sections (9) and (10) write ----
+
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
+
+// Tensors that a launch writes may not share memory with each other nor with what it reads: every workgroup writes its
+// own part, in no order.  `writes` is sorted here (lists cut from one buffer come sorted already).
+void check_apart(Ranges &writes, const Ranges &reads, const char *what) {
+    if (!std::is_sorted(writes.begin(), writes.end())) std::sort(writes.begin(), writes.end());
+    for (size_t i = 1; i < writes.size(); ++i)
+        TORCH_CHECK_VALUE(writes[i].first >= writes[i - 1].second, what, ": two of the written tensors share memory");
+    for (const auto &r : reads) {
+        auto w = std::lower_bound(writes.begin(), writes.end(), std::make_pair(r.second, (uintptr_t)0));   // the first behind r
+        TORCH_CHECK_VALUE(w == writes.begin() || std::prev(w)->second <= r.first, what,
+                          ": a written tensor and one that is read share memory");
+    }
+}
+
+// Written behind autograd's back: the tensors' versions say so.
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- (9) losses over label log-probabilities --------------------------------------------------
 
 // The consecutive dimensions [from, to) of t as one axis of `size` elements, `stride` apart; false when they are not one.
@@ -964,6 +986,15 @@ const float *one_float(const c10::optional<Tensor> &t, const char *name, const T
     return t->data_ptr<float>();
 }
 
+// The memory under a tensor, from its first element to behind its last.
+void add_span(const Tensor &t, Ranges &ranges) {
+    if (t.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    ranges.emplace_back(p, p + (uintptr_t)((last + 1) * t.element_size()));
+}
+
 std::tuple<Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &labels, int64_t class_dim, double temperature,
                                           int64_t ignore_index) {
     const TokenView v = token_view(logits, labels, class_dim, temperature, ignore_index, "token_logprobs");
@@ -994,6 +1025,11 @@ Tensor token_logprobs_grad(const Tensor &logits, const Tensor &labels, const Ten
         check_same_device(logits, *out, "out");
         TORCH_CHECK_VALUE(out->sizes() == logits.sizes(), "out must have the logits' shape");
         TORCH_CHECK_VALUE(device_scale.has_value(), "out holds the gradient for a device_scale of 1: give the device_scale");
+        // (a lane reads logits that another one's gradient would already have replaced)
+        Ranges writes, reads;
+        add_span(*out, writes);
+        for (const Tensor &t : {logits, labels, stats, weight, *device_scale}) add_span(t, reads);
+        check_apart(writes, reads, "token_logprobs_grad");
     }
     Tensor grad = out.has_value() ? *out : at::empty(logits.sizes(), logits.options());
     check_rc(spice_token_logprobs_grad(&v.x, &v.y, (float)temperature, stats.data_ptr<float>(), weight.data_ptr<float>(),
@@ -1001,6 +1037,7 @@ Tensor token_logprobs_grad(const Tensor &logits, const Tensor &labels, const Ten
                                        one_float(device_scale, "device_scale", logits), out.has_value() ? 1 : 0,
                                        v.last ? 1 : 0, grad.data_ptr(), current_stream(logits)),
              "spice_token_logprobs_grad");
+    if (out.has_value()) written(*out);
     return grad;
 }
 
@@ -1144,8 +1181,6 @@ void check_alike(const TensorList &a, const TensorList &b, const char *name) {
     }
 }
 
-using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
-
 void add_ranges(const TensorTable &t, int64_t bytes, Ranges &ranges) {
     for (size_t i = 0; i < t.p.size(); ++i) {
         const uintptr_t p = reinterpret_cast<uintptr_t>(t.p[i]);
@@ -1153,23 +1188,6 @@ void add_ranges(const TensorTable &t, int64_t bytes, Ranges &ranges) {
     }
 }
 
-// Tensors that a launch writes may not share memory with each other nor with what it reads: every workgroup writes its
-// own part, in no order.  `writes` is sorted here (lists cut from one buffer come sorted already).
-void check_apart(Ranges &writes, const Ranges &reads, const char *what) {
-    if (!std::is_sorted(writes.begin(), writes.end())) std::sort(writes.begin(), writes.end());
-    for (size_t i = 1; i < writes.size(); ++i)
-        TORCH_CHECK_VALUE(writes[i].first >= writes[i - 1].second, what, ": two of the written tensors share memory");
-    for (const auto &r : reads) {
-        auto w = std::lower_bound(writes.begin(), writes.end(), std::make_pair(r.second, (uintptr_t)0));   // the first behind r
-        TORCH_CHECK_VALUE(w == writes.begin() || std::prev(w)->second <= r.first, what,
-                          ": a written tensor and one that is read share memory");
-    }
-}
-
-// Written behind autograd's back: the tensors' versions say so.
-void written(const Tensor &t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 void written(const TensorList &ts) {
     for (size_t i = 0; i < ts.size(); ++i) written(ts[i]);
 }

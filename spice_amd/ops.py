@@ -909,7 +909,7 @@ def token_logprobs_grad(logits: torch.Tensor, labels: torch.Tensor, stats: torch
                         device_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scale * d(sum(weight * logp)) / d(logits) in the logits' type (rounded once), dense; `weight` fp32 of the labels'
     shape, or one value a sequence ([N]).  `device_scale`: one more factor, in device memory.  `out`: a contiguous tensor
-    that holds the gradient for a device_scale of 1 already; it is written anew where that factor is another one, and
+    that shares no memory with the others and holds the gradient for a device_scale of 1 already; it is written anew where that factor is another one, and
     left as it is, without being read, where it is 1."""
     return spice_ops().token_logprobs_grad(logits, labels, stats, weight, class_dim, temperature, ignore_index, scale,
                                            device_scale, out)

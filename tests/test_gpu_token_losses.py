@@ -705,3 +705,27 @@ def test_kl_of_a_policy_near_its_reference(dev, layout, positions, c, apart):
     # the weight: 0.5 (1 - exp(q)) and the share's product and rounding
     extra = (w.abs() * 10 * U + 0.5 * U * q.abs() * torch.exp(q)).unsqueeze(d if d == 1 else -1)
     _close(grad, g64, _grad_tol(x, g64, w.abs(), d, 1.0) + extra, "grad")
+
+
+def test_an_out_that_shares_memory_is_refused(dev):
+    """Before anything is launched; a separate one's version tells autograd of the write."""
+    x = torch.randn(2, 3, 40, generator=torch.Generator().manual_seed(1)).to(dev)
+    y = torch.zeros(2, 3, dtype=torch.int64, device=dev)
+    how = dict(class_dim=-1, ignore_index=-100)
+    _, stats = ops.token_logprobs(x, y, **how)
+    w, half = torch.ones(2, 3, device=dev), torch.full((1,), 0.5, device=dev)
+    buf = torch.zeros(1000, device=dev)
+
+    def grad(out, x=x, y=y, stats=stats, w=w, scale=half):
+        return ops.token_logprobs_grad(x, y, stats, w, device_scale=scale, out=out, **how)
+
+    want = ops.token_logprobs_grad(x, y, stats, w, scale=0.5, **how)
+    here, wide = buf[100:340].view(2, 3, 40), torch.zeros(2, 4, 40, device=dev)
+    for call in (lambda: grad(x), lambda: grad(here, stats=buf[330:342].view(2, 3, 2)), lambda: grad(here, w=buf[95:101].view(2, 3)),
+                 lambda: grad(here, scale=buf[339:340]), lambda: grad(wide.view(-1)[:240].view(2, 3, 40), x=wide[:, 1:]),
+                 lambda: grad(here, y=buf[90:102].view(torch.int64).view(2, 3))):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    assert (buf == 0).all() and (wide == 0).all()
+    version = buf._version
+    assert torch.equal(grad(here, stats=buf[340:352].view(2, 3, 2).copy_(stats)), want) and buf._version > version + 1
