@@ -811,6 +811,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
             any |= kind[k] == kCounted;
         }
         float m[VEC], s[VEC], xl[VEC], w[VEC], v[VEC];
+        double sum[VEC] = {};
         G raw[CREG > 0 ? CREG : kStep];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -847,13 +848,22 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
                         }
                     }
                 forget_groups(raw);
+                // four short chains a position, joined in fp64 (see the split kernel)
 #pragma unroll
-                for (int c = 0; c < CREG; ++c)
-                    if (c < classes) {
-                        values<T, VEC>(raw[c], v);
+                for (int c0 = 0; c0 < CREG; c0 += 16) {
+                    float e[VEC][4] = {};
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) s[k] += exp_of(v[k] - shift_of(m[k]), a.t);
-                    }
+                    for (int c = c0; c < (c0 + 16 < CREG ? c0 + 16 : CREG); ++c)
+                        if (c < classes) {
+                            values<T, VEC>(raw[c], v);
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) e[k][c % 4] += exp_of(v[k] - shift_of(m[k]), a.t);
+                        }
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) sum[k] += (double)(e[k][0] + e[k][1]) + (double)(e[k][2] + e[k][3]);
+                }
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) s[k] = (float)sum[k];
             }
         }
         float each[VEC];     // factor of a class's exponential in the gradient; where nothing is counted the value itself
@@ -863,7 +873,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
             const int64_t l = l0 + k;
             each[k] = 0.f;
             if (!kStats) {
-                const double logp = kind[k] == kCounted ? logp_of(xl[k] - shift_of(m[k]), (double)s[k], a.t) : kind[k] == kBad ? NAN : 0.0;
+                const double logp = kind[k] == kCounted ? logp_of(xl[k] - shift_of(m[k]), sum[k], a.t) : kind[k] == kBad ? NAN : 0.0;
                 if (k >= dup) leave_logp(a, at + k, logp, m[k], s[k], 0.f);
                 if (MODE == kModePreference && kind[k] != kIgnored && k >= dup) {
                     sums[0] += logp - (double)a.ref[at + k];

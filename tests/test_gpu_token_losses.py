@@ -729,3 +729,13 @@ def test_an_out_that_shares_memory_is_refused(dev):
     assert (buf == 0).all() and (wide == 0).all()
     version = buf._version
     assert torch.equal(grad(here, stats=buf[340:352].view(2, 3, 2).copy_(stats)), want) and buf._version > version + 1
+
+
+@pytest.mark.parametrize("layout, n, positions, c", [
+    ("planes", 2, (300,), 2), ("planes", 2, (300,), 8), ("planes", 2, (300,), 21), ("planes", 2, (301,), 32), ("planes", 1, (3,), 19)])
+def test_planes_of_few_classes_keep_a_tail(dev, layout, n, positions, c):
+    x, y, logp, p = _long_tail(layout, n, positions, c)
+    _check_long_tail(dev, x, y, 1, logp, p)
+    if len(positions) == 1:      # one position a lane
+        wide = x.to(dev)
+        _check_long_tail(dev, torch.stack([wide, torch.zeros_like(wide)], -1)[..., 0], y, 1, logp, p)
