@@ -100,7 +100,18 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f
 // place holder 0 may lie far above `to`).
 __device__ __forceinline__ float rescale(float m, float to, Temper t) { return m == -INFINITY ? 0.f : exp_of(m - to, t); }
 
-// The sum of exponentials of a row beyond fp32's precision: what the logarithm is taken of, and its fp32 value.
+// The sum of K exponentials as a tree, log2 K roundings deep.  A row's trees add up in fp64: a sum that has reached 1 in fp32
+// takes up no class below 2^-25 of it (255 classes 17 below the top in chains of four lanes: a quarter of 1 - p lost).
+template <int K>
+__device__ __forceinline__ double tree_sum(float (&e)[K]) {
+#pragma unroll
+    for (int o = K / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < o; ++k) e[k] += e[k + o];
+    return (double)e[0];
+}
+
+// The sum of exponentials of a row beyond fp32's precision: what the logarithm is taken of.
 __device__ __forceinline__ double wide_sum(double v, int lanes) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
@@ -108,15 +119,14 @@ __device__ __forceinline__ double wide_sum(double v, int lanes) {
     return v;
 }
 
-// (m, s) of the workgroup from every thread's running maximum and sum; in every thread afterwards.  The threads' sums are
-// added up in fp64: their own roundings average out over the threads, a last few additions' would not.
+// (m, s) of the workgroup from every thread's running maximum and sum; in every thread afterwards.
 template <int THREADS>
-__device__ __forceinline__ double fold_max_sum(float &m, float s, Temper t, double *lds) {
+__device__ __forceinline__ double fold_max_sum(float &m, double s, Temper t, double *lds) {
     constexpr int waves = THREADS / kWave;
     float all = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-    double sum = wide_sum((double)(s * rescale(m, all, t)), kWave);
+    double sum = wide_sum(s * (double)rescale(m, all, t), kWave);
     if (waves > 1) {
         __syncthreads();   // (the last fold's reads)
         if ((threadIdx.x & 63) == 0) {
@@ -294,15 +304,16 @@ __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
         double logp = 0.0;
         if (MODE != kModeGrad) {
             if (kind == kCounted) {
+                double own = 0.0;
                 for (int64_t c = threadIdx.x; c < a.x.c; c += kTokThreads) {
                     const float v = to_f32(x[c * a.x.sc]);
                     if (v > m) {
-                        s *= rescale(m, v, a.t);
+                        own *= (double)rescale(m, v, a.t);
                         m = v;
                     }
-                    s += exp_of(v - shift_of(m), a.t);
+                    own += (double)exp_of(v - shift_of(m), a.t);
                 }
-                const double sum = fold_max_sum<kTokThreads>(m, s, a.t, lds);
+                const double sum = fold_max_sum<kTokThreads>(m, own, a.t, lds);
                 logp = logp_of(to_f32(x[y * a.x.sc]) - shift_of(m), sum, a.t);
                 s = (float)sum;
             } else if (kind == kBad) {
@@ -419,12 +430,12 @@ __device__ __forceinline__ void grad_of(float (&v)[K], float m, float each, floa
 
 // (m, s) of LANES neighbouring lanes; LANES > 64: of the workgroup.
 template <int LANES>
-__device__ __forceinline__ double fold_row(float &m, float s, Temper t, double *lds) {
+__device__ __forceinline__ double fold_row(float &m, double s, Temper t, double *lds) {
     if (LANES <= kWave) {
         float all = m;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-        const double sum = wide_sum((double)(s * rescale(m, all, t)), LANES);
+        const double sum = wide_sum(s * (double)rescale(m, all, t), LANES);
         m = all;
         return sum;
     }
@@ -514,15 +525,17 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
             forget<NV>(raw);
             unpack(last, v, T());
 #pragma unroll
-            for (int k = 0; k < K; ++k) s += k < again ? 0.f : exp_of(v[k] - shift, a.t);
+            for (int k = 0; k < K; ++k) v[k] = k < again ? 0.f : exp_of(v[k] - shift, a.t);
+            double own = tree_sum(v);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (i < whole) {
                     unpack(raw[i], v, T());
 #pragma unroll
-                    for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+                    for (int k = 0; k < K; ++k) v[k] = exp_of(v[k] - shift, a.t);
+                    own += tree_sum(v);
                 }
-            const double sum = fold_row<LANES>(m, s, a.t, lds);
+            const double sum = fold_row<LANES>(m, own, a.t, lds);
             if (kGrad || lane == 0) logp = logp_of(xl - shift_of(m), sum, a.t);
             s = (float)sum;
         }
@@ -582,6 +595,7 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
         float m = -INFINITY, s = 0.f;
         double logp = kind == kBad ? NAN : 0.0;
         if (kind == kCounted) {
+            double own = 0.0;
             for (int64_t base = 0; base < classes; base += (int64_t)kStep * kBlock * K) {
                 u32x4 raw[kStep];
                 float top = m;
@@ -598,7 +612,7 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
 #pragma unroll
                         for (int k = 0; k < K; ++k) top = fmaxf(top, v[k]);
                     }
-                s *= rescale(m, top, a.t);
+                own *= (double)rescale(m, top, a.t);
                 m = top;
                 const float shift = shift_of(m);
 #pragma unroll
@@ -607,10 +621,11 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
                         float v[K];
                         unpack(raw[i], v, T());
 #pragma unroll
-                        for (int k = 0; k < K; ++k) s += exp_of(v[k] - shift, a.t);
+                        for (int k = 0; k < K; ++k) v[k] = exp_of(v[k] - shift, a.t);
+                        own += tree_sum(v);
                     }
             }
-            const double sum = fold_row<kBlock>(m, s, a.t, lds);
+            const double sum = fold_row<kBlock>(m, own, a.t, lds);
             logp = logp_of(to_f32(x[y]) - shift_of(m), sum, a.t);
             s = (float)sum;
         }

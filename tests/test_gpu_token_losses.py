@@ -739,3 +739,18 @@ def test_planes_of_few_classes_keep_a_tail(dev, layout, n, positions, c):
     if len(positions) == 1:      # one position a lane
         wide = x.to(dev)
         _check_long_tail(dev, torch.stack([wide, torch.zeros_like(wide)], -1)[..., 0], y, 1, logp, p)
+
+
+@pytest.mark.parametrize("layout, n, positions, c", [
+    ("last", 2, (9,), 7), ("last", 2, (40,), 31), ("last", 2, (40,), 150), ("last", 2, (20,), 255), ("last", 2, (20,), 447),
+    ("last", 2, (20,), 895), ("last", 2, (9,), 2000), ("last", 2, (9,), 8000), ("last", 2, (3,), 32000), ("last", 2, (3,), 50001),
+    ("last", 1, (2,), 131072), ("last", 1, (2,), 200003), ("planes", 2, (5,), 3001), ("planes", 2, (3,), 100001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_keep_a_long_tail(dev, layout, n, positions, c, dtype):
+    x, y, logp, p = _long_tail(layout, n, positions, c)
+    d = -1 if layout == "last" else 1
+    if dtype == torch.float32:
+        _check_long_tail(dev, x, y, d, logp, p)
+    else:
+        got = ops.token_logprobs(x.to(dtype).to(dev), y.to(dev), class_dim=d, ignore_index=-100)[0]
+        assert (got.double() - logp).abs().max().item() <= TAIL * U * abs(logp) + TREE * U
