@@ -79,12 +79,12 @@ __device__ __forceinline__ double log_of(float s) {
     return (double)e * 0.69314718055994530942 + (2.0 * exact + (double)(2.f * t * q * r));
 }
 
-// A label's log-probability from its distance to the maximum and the sum, in fp64: a sequence's log ratio is a small
-// difference of thousands of them, and rounding each to fp32 (2^-22 at 4 to 8) would show in it.
-__device__ __forceinline__ double logp_of(float d, double s, Temper t) {
+// A label's log-probability from its logit, the maximum and the sum, in fp64: a sequence's log ratio is a small difference of
+// thousands of them, and rounding each, or the logit's distance to the maximum, to fp32 (2^-22 at 4 to 8) would show in it.
+__device__ __forceinline__ double logp_of(float xl, float shift, double s, Temper t) {
     const float near = (float)s;
     const double rest = near > 0.f && near < INFINITY ? (s - (double)near) / s : 0.0;
-    return (double)d * t.exact_inv - (log_of(near) + rest);
+    return ((double)xl - (double)shift) * t.exact_inv - (log_of(near) + rest);
 }
 
 // What a position's label says.
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(kTokThreads) void tok_any_kernel(TokArgs a) {
                     own += (double)exp_of(v - shift_of(m), a.t);
                 }
                 const double sum = fold_max_sum<kTokThreads>(m, own, a.t, lds);
-                logp = logp_of(to_f32(x[y * a.x.sc]) - shift_of(m), sum, a.t);
+                logp = logp_of(to_f32(x[y * a.x.sc]), shift_of(m), sum, a.t);
                 s = (float)sum;
             } else if (kind == kBad) {
                 logp = NAN;
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(LANES < kTokThreads ? kTokThreads : LANES, NV <= 8 
                     own += tree_sum(v);
                 }
             const double sum = fold_row<LANES>(m, own, a.t, lds);
-            if (kGrad || lane == 0) logp = logp_of(xl - shift_of(m), sum, a.t);
+            if (kGrad || lane == 0) logp = logp_of(xl, shift_of(m), sum, a.t);
             s = (float)sum;
         }
     }
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(1024) void tok_long_row_kernel(TokArgs a) {
                     }
             }
             const double sum = fold_row<kBlock>(m, own, a.t, lds);
-            logp = logp_of(to_f32(x[y]) - shift_of(m), sum, a.t);
+            logp = logp_of(to_f32(x[y]), shift_of(m), sum, a.t);
             s = (float)sum;
         }
         if (threadIdx.x == 0) leave_logp(a, at, logp, m, s, ref);
@@ -888,7 +888,7 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
             const int64_t l = l0 + k;
             each[k] = 0.f;
             if (!kStats) {
-                const double logp = kind[k] == kCounted ? logp_of(xl[k] - shift_of(m[k]), sum[k], a.t) : kind[k] == kBad ? NAN : 0.0;
+                const double logp = kind[k] == kCounted ? logp_of(xl[k], shift_of(m[k]), sum[k], a.t) : kind[k] == kBad ? NAN : 0.0;
                 if (k >= dup) leave_logp(a, at + k, logp, m[k], s[k], 0.f);
                 if (MODE == kModePreference && kind[k] != kIgnored && k >= dup) {
                     sums[0] += logp - (double)a.ref[at + k];
@@ -1080,7 +1080,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
             double sum = 0.0;
             for (int g = 0; g < GROUPS; ++g) sum += part_sum[g][q] * (double)rescale(part_max[g][q], m, a.t);
             s = (float)sum;
-            const double exact = yq >= 0 ? logp_of(at_label[q] - shift_of(m), sum, a.t) : yq == -2 ? (double)NAN : 0.0;
+            const double exact = yq >= 0 ? logp_of(at_label[q], shift_of(m), sum, a.t) : yq == -2 ? (double)NAN : 0.0;
             if (q >= dup) leave_logp(a, at, exact, m, s, 0.f);
             if (MODE == kModePreference && yq != -1 && q >= dup) {
                 sums[0] += exact - (double)a.ref[at];

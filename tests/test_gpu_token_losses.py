@@ -754,3 +754,32 @@ def test_rows_keep_a_long_tail(dev, layout, n, positions, c, dtype):
     else:
         got = ops.token_logprobs(x.to(dtype).to(dev), y.to(dev), class_dim=d, ignore_index=-100)[0]
         assert (got.double() - logp).abs().max().item() <= TAIL * U * abs(logp) + TREE * U
+
+
+@pytest.mark.parametrize("layout, positions, c", [("last", (1000,), 2), ("last", (1000,), 300), ("last", (100,), 5000), ("last", (100,), 90000),
+                                                  ("planes", (1000,), 2), ("planes", (1000,), 40), ("planes", (200,), 300)])
+@pytest.mark.parametrize("t", [1.0])
+def test_log_ratios_of_many_positions_that_round_alike(dev, layout, positions, c, t):
+    """Every position's label lies 8 - 0.4 steps below the maximum, which a subtraction in fp32 rounds to 8, and all the same way:
+    a sequence's log ratio adds that up.  Two classes count (the rest are -inf): the
+    other one's exp(-8 / T) is off by 24 u at most (its distance, the product of up to 16.5, the instruction), its addition to
+    the maximum's 1 rounds by half a step at 1, which is u (all further ones add zeros), and a position's log ratio, where it
+    is kept in fp32, by u."""
+    n, low32 = 2, torch.tensor(0.4 * 2.0 ** -21)
+    x = torch.full((n, *positions, c), -math.inf)
+    x[..., 0], x[..., c - 1] = 8.0, low32
+    y = torch.full((n, *positions), c - 1)
+    y[1, ::3] = 0
+    if layout == "planes":
+        x = x.movedim(-1, 1).contiguous()
+    d = -1 if layout == "last" else 1
+    how = dict(class_dim=d, ignore_index=-100, temperature=t)
+    z = -(8.0 - low32.double().item()) / t
+    norm = math.log1p(math.exp(z))
+    logp = torch.where(y == 0, torch.tensor(-norm, dtype=torch.float64), torch.tensor(z - norm, dtype=torch.float64))
+    ref = logp.float()
+    per = (logp - ref.double())
+    want = per.sum(1)
+    _, rewards, _ = ops.preference_loss(x.to(dev), y.to(dev), ref.to(dev), beta=1.0, **how)
+    tol = positions[0] * (24 * U * math.exp(z) + U) + U * per.abs().sum(1) + U * want.abs()
+    assert ((rewards.cpu().double() - want).abs() <= tol).all(), (rewards, want, tol)
