@@ -589,7 +589,7 @@ typedef struct spice_preference_params {
  * logp - ref_logp, h_i = R_i - R_{n/2+i}, total = mean over pairs of the loss of h_i; rewards[n] = beta * R_n.
  * weight[n] = d total / d logp of every counted position of sequence n: spice_token_logprobs_grad(weight, 1, 0) on the
  * stats written here is the gradient.  ref_logp [n,l] fp32 (anything where ignored).
- * Log ratios and sums in fp64, in a fixed order.  ratio [n,l]: scratch. */
+ * Log ratios and sums in fp64, in a fixed order (in the workspace; `ratio` is not used and may be NULL). */
 int spice_preference_loss(const spice_logits *logits, const spice_labels *labels, const float *ref_logp,
                           const spice_preference_params *params, float *total, float *rewards, float *weight, float *ratio,
                           float *stats, void *workspace, size_t workspace_bytes, void *stream);

@@ -232,7 +232,7 @@ struct TokArgs {
     Labels y;
     Temper t;
     float *logp;            // [n, l], may be NULL
-    float *ratio;           // [n, l] logp - ref, may be NULL
+    double *ratio;          // [n, l] logp - ref, may be NULL
     float2 *stats;          // [n, l] (max, sum), may be NULL
     const float2 *stats_in;
     const float *weight;    // kModeGrad: factor of each position
@@ -253,7 +253,7 @@ struct TokArgs {
 // What a position leaves: its log-probability, or the preference loss's log ratio, and its statistics.
 __device__ __forceinline__ void leave_logp(const TokArgs &a, int64_t at, double logp, float m, float s, float ref) {
     if (a.logp) a.logp[at] = (float)logp;
-    if (a.ratio) a.ratio[at] = (float)(logp - (double)ref);   // (where ignored it is not read)
+    if (a.ratio) a.ratio[at] = logp - (double)ref;   // (where ignored it is not read)
     if (a.stats) a.stats[at] = make_float2(m, s);
 }
 
@@ -1152,7 +1152,7 @@ __global__ __launch_bounds__(kTokThreads, HOLD > 0 ? 4 : 3) void tok_split_kerne
 
 struct SumArgs {
     const float *logp;
-    const float *ratio;     // preference: logp - ref
+    const double *ratio;    // preference: logp - ref, in fp64: pairs of sequences are subtracted from each other
     Labels y;
     int64_t n, l, chunks;
     Policy policy;
@@ -1171,7 +1171,7 @@ __device__ __forceinline__ void sum_position(const SumArgs &a, int64_t n, int64_
     const int64_t at = n * a.l + l;
     if (a.y.y[n * a.y.sn + l * a.y.sl] == a.y.ignore) return;
     v[K - 1] += 1.0;
-    if (WHAT == kSumPreference) v[0] += (double)a.ratio[at];
+    if (WHAT == kSumPreference) v[0] += a.ratio[at];
     if (WHAT == kSumPolicy) {
         const PolicyTerm t = policy_term(a.policy, policy_in(a.policy, at, n, l), a.logp[at]);
         v[0] += t.surrogate;
@@ -1526,6 +1526,7 @@ int64_t items_of(const TokArgs &a) {
     return !a.x.l ? 1 : a.x.c > kPlanesClasses ? ceil_div(a.x.l, kSplitTile) : planes_tiles(a.x.l, planes_vec(a));
 }
 
+// The losses' workspace: the partial sums, 4 n + 8 of the sequences', the preference loss's log ratios [n, l].
 // Partial sums of a call at most: the workgroups' of the split planes kernel, or the waves' of the folding workgroup.
 int64_t part_doubles(int64_t n, int64_t l) {
     const int64_t items = l > kSplitTile ? ceil_div(l, kSplitTile) : 1, waves = kTokFold / kWave;
@@ -1560,7 +1561,7 @@ using namespace spice;
 
 extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
     if (n < 0 || l < 0) return 0;
-    return (size_t)(part_doubles(n, l) + 4 * n + 8) * sizeof(double);
+    return (size_t)(part_doubles(n, l) + 4 * n + 8 + n * l) * sizeof(double);
 }
 
 extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, float temperature, float *logp, float *stats,
@@ -1593,20 +1594,20 @@ extern "C" int spice_token_logprobs_grad(const spice_logits *x, const spice_labe
 }
 
 extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *y, const float *ref_logp,
-                                     const spice_preference_params *p, float *total, float *rewards, float *weight, float *ratio,
+                                     const spice_preference_params *p, float *total, float *rewards, float *weight, float *,
                                      float *stats, void *workspace, size_t workspace_bytes, void *stream) {
     if (!logits_ok(x) || !labels_ok(x, y) || !p || x->n < 2 || x->n % 2 || !total || !rewards || !weight || !workspace ||
-        !aligned8(workspace) || ((!ref_logp || !ratio) && x->l) || !aligned8(stats) || !(p->beta > 0.f) ||
+        !aligned8(workspace) || (!ref_logp && x->l) || !aligned8(stats) || !(p->beta > 0.f) ||
         !(p->smoothing >= 0.f && p->smoothing < 0.5f) || p->loss_type < 0 || p->loss_type > 1 ||
         (p->loss_type == SPICE_PREFERENCE_IPO && p->smoothing != 0.f) || !temperature_ok(p->temperature))
         return SPICE_ERR_ARG;
     if (workspace_bytes < spice_token_loss_workspace_bytes(x->n, x->l)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     TokArgs a = args_of(x, y, p->temperature);
-    if (route_of(a) != kByPlanes) a.ratio = ratio;      // (the planes kernels sum it themselves)
     a.stats = (float2 *)stats;
     a.ref = ref_logp;
     a.part = (double *)workspace;
+    if (route_of(a) != kByPlanes) a.ratio = a.part + part_doubles(x->n, x->l) + 4 * x->n + 8;   // (the planes kernels sum it themselves)
     int rc = launch_positions<kModePreference>(a, x->dtype, s);
     if (rc) return rc;
     SumArgs sums = sums_of(a, a.part);

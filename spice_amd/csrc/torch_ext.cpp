@@ -1057,13 +1057,12 @@ std::vector<Tensor> preference_loss(const Tensor &logits, const Tensor &labels, 
     const auto f32 = logits.options().dtype(at::kFloat);
     const int64_t positions = v.x.n * v.x.l, ws_bytes = (int64_t)spice_token_loss_workspace_bytes(v.x.n, v.x.l);
     Tensor total = at::empty({}, f32), rewards = at::empty({v.x.n}, f32), weight, stats;
-    // the workspace, logp and, where only the gradient below needs them, weight and statistics in one piece
-    Tensor scratch = at::empty({ws_bytes / 4 + positions + (want_grad ? 2 * positions + v.x.n : 0)}, f32);
-    float *logp = scratch.data_ptr<float>() + ws_bytes / 4, *stats_p, *weight_p;
+    // the workspace and, where only the gradient below needs them, weight and statistics in one piece
+    Tensor scratch = at::empty({ws_bytes / 4 + (want_grad ? 2 * positions + v.x.n : 0)}, f32);
+    float *stats_p, *weight_p;
     if (want_grad) {
         stats_p = scratch.data_ptr<float>() + ws_bytes / 4;
-        logp = stats_p + 2 * positions;
-        weight_p = logp + positions;
+        weight_p = stats_p + 2 * positions;
     } else {
         weight = at::empty({v.x.n}, f32);
         stats = stats_for(labels, f32);
@@ -1078,7 +1077,7 @@ std::vector<Tensor> preference_loss(const Tensor &logits, const Tensor &labels, 
     p.average = average ? 1 : 0;
     void *stream = current_stream(logits);
     check_rc(spice_preference_loss(&v.x, &v.y, ref_logprobs.data_ptr<float>(), &p, total.data_ptr<float>(),
-                                   rewards.data_ptr<float>(), weight_p, logp, stats_p, scratch.data_ptr(), (size_t)ws_bytes, stream),
+                                   rewards.data_ptr<float>(), weight_p, nullptr, stats_p, scratch.data_ptr(), (size_t)ws_bytes, stream),
              "spice_preference_loss");
     if (!want_grad) return {total, rewards, weight, stats};
     Tensor grad = at::empty(logits.sizes(), logits.options());

@@ -783,3 +783,24 @@ def test_log_ratios_of_many_positions_that_round_alike(dev, layout, positions, c
     _, rewards, _ = ops.preference_loss(x.to(dev), y.to(dev), ref.to(dev), beta=1.0, **how)
     tol = positions[0] * (24 * U * math.exp(z) + U) + U * per.abs().sum(1) + U * want.abs()
     assert ((rewards.cpu().double() - want).abs() <= tol).all(), (rewards, want, tol)
+
+
+@pytest.mark.parametrize("layout, c, l", [("last", 2, 1), ("last", 2, 5000), ("planes", 2, 1), ("planes", 2, 600), ("planes", 2000, 7),
+                                          ("last", 90000, 3)])
+def test_log_ratios_are_held_in_64_bits(dev, layout, c, l):
+    """ipo: h - 1 / (2 beta), h the difference of two sequences' log ratios.  Two equal classes (the others -inf): logp = -log 2 up
+    to 2^-50, every log ratio is exact up to that, the loss rounds to fp32 once."""
+    x = torch.full((2, l, c), -math.inf)
+    x[..., 0] = x[..., 1] = 0.0
+    d = -1 if layout == "last" else 1
+    x = (x if d == -1 else x.movedim(-1, 1).contiguous()).to(dev)
+    y = torch.zeros(2, l, dtype=torch.int64, device=dev)
+    ref = torch.full((2, l), -math.log(2.0))
+    ref[0] -= 4.0 + 1e-4
+    ref[1, ::2] += 1e-3
+    s = (-math.log(2.0) - ref.double()).mean(1)
+    off = (s[0] - s[1]).item() - 4.0
+    total, rewards, _ = ops.preference_loss(x, y, ref.to(dev), beta=0.125, loss_type="ipo", average=True, class_dim=d, ignore_index=-100)
+    # (h is off by 2^-47 at most, the square by twice that of its root)
+    assert abs(total.item() - off * off) <= U * off * off + 2 * 2.0 ** -47 * abs(off)
+    assert ((rewards.cpu().double() - 0.125 * s).abs() <= U * 0.125 * s.abs() + 2.0 ** -50).all()
