@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SPICE_ABI_VERSION 5
+#define SPICE_ABI_VERSION 6
 
 #define SPICE_OK 0
 #define SPICE_ERR_ARG 10001         /* null pointer, negative size, misaligned base */
@@ -564,14 +564,14 @@ typedef struct spice_labels {
 size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l);
 
 /* logp [n,l] fp32; stats [n,l,2] fp32 = {m, s} for spice_token_logprobs_grad, or NULL. */
-int spice_token_logprobs(const spice_logits *logits, const spice_labels *labels, float temperature, float *logp,
+int spice_token_logprobs(const spice_logits *logits, const spice_labels *labels, double temperature, float *logp,
                          float *stats, void *stream);
 
 /* grad = scale * d(sum_nl weight[n,l] * logp[n,l]) / d(logits), dense in the order [n][l][c] (class_last) or [n][c][l],
  * in the logits' type; weight[n*w_n_stride + l*w_l_stride] (a stride may be 0).  device_scale: a further factor in device
  * memory, or NULL; with unless_one nothing is read or written where that factor is 1 (a gradient taken with the loss
  * already stands in `grad`, and an upstream factor other than 1 asks for it anew, rounded once). */
-int spice_token_logprobs_grad(const spice_logits *logits, const spice_labels *labels, float temperature, const float *stats,
+int spice_token_logprobs_grad(const spice_logits *logits, const spice_labels *labels, double temperature, const float *stats,
                               const float *weight, int64_t w_n_stride, int64_t w_l_stride, float scale,
                               const float *device_scale, int32_t unless_one, int32_t class_last, void *grad, void *stream);
 
@@ -594,6 +594,16 @@ int spice_preference_loss(const spice_logits *logits, const spice_labels *labels
                           const spice_preference_params *params, float *total, float *rewards, float *weight, float *ratio,
                           float *stats, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The same with options that keep their precision: T = 0.7 rounded to fp32 moves every log-probability of a sequence the
+ * same way, and 1/(2 beta) is the other side of a difference. */
+typedef struct spice_preference_options {
+    double temperature, beta, smoothing;
+    int32_t loss_type, average;
+} spice_preference_options;
+int spice_preference_loss_opts(const spice_logits *logits, const spice_labels *labels, const float *ref_logp,
+                               const spice_preference_options *options, float *total, float *rewards, float *weight,
+                               float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
 #define SPICE_POLICY_TOKEN 0    /* mean over all counted positions */
 #define SPICE_POLICY_SEQUENCE 1 /* mean over the n sequences of the mean over each one's counted positions (none: 0) */
 typedef struct spice_policy_params {
@@ -615,6 +625,16 @@ int spice_policy_loss(const spice_logits *logits, const spice_labels *labels, co
                       const float *advantages, int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp,
                       const spice_policy_params *params, float *out4, float *logp, float *stats, float *weight,
                       int32_t class_last, void *grad, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same with options that keep their precision (ratio bounds, kl_weight and grad_scale round to fp32 once, where they are used). */
+typedef struct spice_policy_options {
+    double temperature, clip_low, clip_high, kl_weight, grad_scale;
+    int32_t reduction, pad_;
+} spice_policy_options;
+int spice_policy_loss_opts(const spice_logits *logits, const spice_labels *labels, const float *old_logp,
+                           const float *advantages, int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp,
+                           const spice_policy_options *options, float *out4, float *logp, float *stats, float *weight,
+                           int32_t class_last, void *grad, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------- *
  * (10) The update end of a fine-tuning step over many tensors: global gradient

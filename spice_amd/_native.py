@@ -17,7 +17,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libspice_amd.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "lib", "libspice_torch.so")
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 ERR_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_BLAS, ERR_STATIC_LIMIT = 10001, 10002, 10003, 10004, 10005
 IMP_L1, IMP_L2, IMP_TAYLOR = 0, 1, 2
 
@@ -83,6 +83,16 @@ class PreferenceParams(Structure):
 class PolicyParams(Structure):
     _fields_ = [("temperature", c_float), ("clip_low", c_float), ("clip_high", c_float), ("kl_weight", c_float),
                 ("grad_scale", c_float), ("reduction", c_int32)]
+
+
+class PreferenceOptions(Structure):
+    _fields_ = [("temperature", c_double), ("beta", c_double), ("smoothing", c_double), ("loss_type", c_int32),
+                ("average", c_int32)]
+
+
+class PolicyOptions(Structure):
+    _fields_ = [("temperature", c_double), ("clip_low", c_double), ("clip_high", c_double), ("kl_weight", c_double),
+                ("grad_scale", c_double), ("reduction", c_int32), ("pad_", c_int32)]
 
 
 class AdamParams(Structure):
@@ -163,14 +173,19 @@ SIGNATURES = {
     "spice_upsample_bilinear_into": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int32,
                                           c_int32, c_int32, c_int32, c_float, c_float, c_int64, c_int64, c_void_p]),
     "spice_token_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
-    "spice_token_logprobs": (c_int32, [POINTER(Logits), POINTER(Labels), c_float, c_void_p, c_void_p, c_void_p]),
-    "spice_token_logprobs_grad": (c_int32, [POINTER(Logits), POINTER(Labels), c_float, c_void_p, c_void_p, c_int64, c_int64,
+    "spice_token_logprobs": (c_int32, [POINTER(Logits), POINTER(Labels), c_double, c_void_p, c_void_p, c_void_p]),
+    "spice_token_logprobs_grad": (c_int32, [POINTER(Logits), POINTER(Labels), c_double, c_void_p, c_void_p, c_int64, c_int64,
                                             c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "spice_preference_loss": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, POINTER(PreferenceParams), c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "spice_policy_loss": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                                     POINTER(PolicyParams), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
                                     c_void_p, c_size_t, c_void_p]),
+    "spice_preference_loss_opts": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, POINTER(PreferenceOptions), c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "spice_policy_loss_opts": (c_int32, [POINTER(Logits), POINTER(Labels), c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                         POINTER(PolicyOptions), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
+                                         c_void_p, c_size_t, c_void_p]),
     "spice_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int32]),
     "spice_grad_norm": (c_int32, [POINTER(c_void_p), POINTER(c_int64), c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
                                   c_size_t, c_void_p]),

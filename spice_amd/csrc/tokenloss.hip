@@ -40,13 +40,13 @@ struct Temper {
     double exact_inv;
 };
 
-static Temper temper(float t) {
-    const double k = 1.4426950408889634074 / (double)t;
+static Temper temper(double t) {
+    const double k = 1.4426950408889634074 / t;
     Temper r;
     r.k = (float)k;
     if ((double)r.k >= k) r.k = nextafterf(r.k, 0.f);   // k_lo > 0: an excluded class's d = -inf stays -inf in both products
     r.k_lo = (float)(k - (double)r.k);
-    r.exact_inv = 1.0 / (double)t;
+    r.exact_inv = 1.0 / t;
     r.inv = (float)r.exact_inv;
     return r;
 }
@@ -1258,7 +1258,7 @@ __global__ __launch_bounds__(kTokFold) void tok_share_kernel(SumArgs a, int64_t 
 }
 
 struct PreferenceEnd {
-    float beta, smoothing;
+    double beta, smoothing;
     int ipo, average;
     float *total, *rewards, *weight;   // [1], [n], [n]: d total / d logp of every counted position of sequence n
     double *ratio;                     // [n, 2] scratch: a sequence's log ratio, and what its positions count
@@ -1287,7 +1287,7 @@ __global__ __launch_bounds__(kTokFold) void tok_preference_kernel(SumArgs a, int
     double v[1] = {0.0};
     for (int64_t i = threadIdx.x; i < half; i += kTokFold) {
         const double sa = e.ratio[2 * i], sb = e.ratio[2 * (half + i)];
-        const double h = sa - sb, b = (double)e.beta, eps = (double)e.smoothing;
+        const double h = sa - sb, b = e.beta, eps = e.smoothing;
         double dh;
         if (e.ipo) {
             const double off = h - 0.5 / b;
@@ -1307,8 +1307,8 @@ __global__ __launch_bounds__(kTokFold) void tok_preference_kernel(SumArgs a, int
 }
 
 // out4 = {total, surrogate, kl, share of the counted positions where the clipping holds}
-__device__ __forceinline__ void policy_end(double surrogate, double far, double over, double count, float kl, float *out4) {
-    out4[0] = (float)(kl != 0.f ? surrogate + (double)kl * far : surrogate);
+__device__ __forceinline__ void policy_end(double surrogate, double far, double over, double count, double kl, float *out4) {
+    out4[0] = (float)(kl != 0.0 ? surrogate + kl * far : surrogate);
     out4[1] = (float)surrogate;
     out4[2] = (float)far;
     out4[3] = (float)(over / fmax(count, 1.0));
@@ -1316,7 +1316,7 @@ __device__ __forceinline__ void policy_end(double surrogate, double far, double 
 
 // The end of the policy loss.  `each` [n, 4]: scratch.  One workgroup, latency: 6.0 us.  (By the last workgroup of the loss's
 // pass, told by a ticket: 100 us for [8,21,512x512], 79 at that time with launches of their own.)
-__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, int per_sequence, double *each, float kl,
+__global__ __launch_bounds__(kTokFold) void tok_policy_end_kernel(SumArgs a, int64_t ways, int per_sequence, double *each, double kl,
                                                                   float *out4) {
     __shared__ double lds[4 * kTokFold / kWave];
     if (ways) sums_here<kSumPolicy>(a, ways);
@@ -1366,9 +1366,9 @@ bool labels_ok(const spice_logits *x, const spice_labels *y) {
     return y && (y->data || x->n == 0 || x->l == 0) && (y->ignore_index < 0 || y->ignore_index >= x->c);
 }
 
-bool temperature_ok(float t) { return t > 0.f && t <= 3.0e38f && 1.f / t <= 3.0e38f; }
+bool temperature_ok(double t) { return t > 0.0 && t <= 3.0e38 && 1.0 / t <= 3.0e38; }
 
-TokArgs args_of(const spice_logits *x, const spice_labels *y, float t) {
+TokArgs args_of(const spice_logits *x, const spice_labels *y, double t) {
     TokArgs a = {};
     a.x = Logits{x->data, x->n, x->l, x->c, x->n_stride, x->l_stride, x->c_stride};
     a.y = Labels{y->data, y->n_stride, y->l_stride, y->ignore_index};
@@ -1564,7 +1564,7 @@ extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
     return (size_t)(part_doubles(n, l) + 4 * n + 8 + n * l) * sizeof(double);
 }
 
-extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, float temperature, float *logp, float *stats,
+extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, double temperature, float *logp, float *stats,
                                     void *stream) {
     if (!logits_ok(x) || !labels_ok(x, y) || !temperature_ok(temperature) || (!logp && x->n * x->l) || !aligned8(stats))
         return SPICE_ERR_ARG;
@@ -1574,7 +1574,7 @@ extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y
     return launch_positions<kModeLogp>(a, x->dtype, (hipStream_t)stream);
 }
 
-extern "C" int spice_token_logprobs_grad(const spice_logits *x, const spice_labels *y, float temperature, const float *stats,
+extern "C" int spice_token_logprobs_grad(const spice_logits *x, const spice_labels *y, double temperature, const float *stats,
                                          const float *weight, int64_t w_n_stride, int64_t w_l_stride, float scale,
                                          const float *device_scale, int32_t unless_one, int32_t class_last, void *grad,
                                          void *stream) {
@@ -1593,13 +1593,13 @@ extern "C" int spice_token_logprobs_grad(const spice_logits *x, const spice_labe
     return launch_positions<kModeGrad>(a, x->dtype, (hipStream_t)stream);
 }
 
-extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *y, const float *ref_logp,
-                                     const spice_preference_params *p, float *total, float *rewards, float *weight, float *,
-                                     float *stats, void *workspace, size_t workspace_bytes, void *stream) {
+extern "C" int spice_preference_loss_opts(const spice_logits *x, const spice_labels *y, const float *ref_logp,
+                                          const spice_preference_options *p, float *total, float *rewards, float *weight,
+                                          float *stats, void *workspace, size_t workspace_bytes, void *stream) {
     if (!logits_ok(x) || !labels_ok(x, y) || !p || x->n < 2 || x->n % 2 || !total || !rewards || !weight || !workspace ||
-        !aligned8(workspace) || (!ref_logp && x->l) || !aligned8(stats) || !(p->beta > 0.f) ||
-        !(p->smoothing >= 0.f && p->smoothing < 0.5f) || p->loss_type < 0 || p->loss_type > 1 ||
-        (p->loss_type == SPICE_PREFERENCE_IPO && p->smoothing != 0.f) || !temperature_ok(p->temperature))
+        !aligned8(workspace) || (!ref_logp && x->l) || !aligned8(stats) || !(p->beta > 0.0 && p->beta <= 3.0e38) ||
+        !(p->smoothing >= 0.0 && p->smoothing < 0.5) || p->loss_type < 0 || p->loss_type > 1 ||
+        (p->loss_type == SPICE_PREFERENCE_IPO && p->smoothing != 0.0) || !temperature_ok(p->temperature))
         return SPICE_ERR_ARG;
     if (workspace_bytes < spice_token_loss_workspace_bytes(x->n, x->l)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -1625,13 +1625,21 @@ extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *
     return SPICE_OK;
 }
 
-extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, const float *old_logp, const float *advantages,
-                                 int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp, const spice_policy_params *p,
-                                 float *out4, float *logp, float *stats, float *weight, int32_t class_last, void *grad,
-                                 void *workspace, size_t workspace_bytes, void *stream) {
+extern "C" int spice_preference_loss(const spice_logits *x, const spice_labels *y, const float *ref_logp,
+                                     const spice_preference_params *p, float *total, float *rewards, float *weight, float *,
+                                     float *stats, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!p) return SPICE_ERR_ARG;
+    const spice_preference_options o = {p->temperature, p->beta, p->smoothing, p->loss_type, p->average};
+    return spice_preference_loss_opts(x, y, ref_logp, &o, total, rewards, weight, stats, workspace, workspace_bytes, stream);
+}
+
+extern "C" int spice_policy_loss_opts(const spice_logits *x, const spice_labels *y, const float *old_logp, const float *advantages,
+                                      int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp,
+                                      const spice_policy_options *p, float *out4, float *logp, float *stats, float *weight,
+                                      int32_t class_last, void *grad, void *workspace, size_t workspace_bytes, void *stream) {
     if (!logits_ok(x) || !labels_ok(x, y) || !p || !out4 || !workspace || !aligned8(workspace) ||
-        ((!old_logp || !advantages || !logp) && x->n * x->l) || !(p->clip_low >= 0.f && p->clip_low <= 1.f) ||
-        !(p->clip_high >= 0.f) || !(p->kl_weight >= 0.f) || (p->kl_weight > 0.f && !ref_logp && x->n * x->l) ||
+        ((!old_logp || !advantages || !logp) && x->n * x->l) || !(p->clip_low >= 0.0 && p->clip_low <= 1.0) ||
+        !(p->clip_high >= 0.0) || !(p->kl_weight >= 0.0) || (p->kl_weight > 0.0 && !ref_logp && x->n * x->l) ||
         p->reduction < 0 || p->reduction > 1 || !aligned8(stats) || !temperature_ok(p->temperature))
         return SPICE_ERR_ARG;
     if (workspace_bytes < spice_token_loss_workspace_bytes(x->n, x->l)) return SPICE_ERR_WORKSPACE;
@@ -1640,9 +1648,9 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     a.logp = logp;
     a.stats = (float2 *)stats;
     a.weight_out = weight;
-    a.host_scale = p->grad_scale;
-    a.policy = Policy{old_logp, advantages, ref_logp, adv_n_stride, adv_l_stride, 1.f - p->clip_low, 1.f + p->clip_high,
-                      p->kl_weight};
+    a.host_scale = (float)p->grad_scale;
+    a.policy = Policy{old_logp, advantages, ref_logp, adv_n_stride, adv_l_stride, (float)(1.0 - p->clip_low),
+                      (float)(1.0 + p->clip_high), (float)p->kl_weight};
     if (grad) grad_layout(a, grad, class_last);
     a.part = (double *)workspace;
     SumArgs sums = sums_of(a, a.part);
@@ -1673,4 +1681,14 @@ extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, c
     tok_policy_end_kernel<<<1, kTokFold, 0, s>>>(sums, ways, a.per_sequence, scratch, p->kl_weight, out4);
     SPICE_LAUNCH_CHECK();
     return SPICE_OK;
+}
+
+extern "C" int spice_policy_loss(const spice_logits *x, const spice_labels *y, const float *old_logp, const float *advantages,
+                                 int64_t adv_n_stride, int64_t adv_l_stride, const float *ref_logp, const spice_policy_params *p,
+                                 float *out4, float *logp, float *stats, float *weight, int32_t class_last, void *grad,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
+    if (!p) return SPICE_ERR_ARG;
+    const spice_policy_options o = {p->temperature, p->clip_low, p->clip_high, p->kl_weight, p->grad_scale, p->reduction, 0};
+    return spice_policy_loss_opts(x, y, old_logp, advantages, adv_n_stride, adv_l_stride, ref_logp, &o, out4, logp, stats, weight,
+                                  class_last, grad, workspace, workspace_bytes, stream);
 }

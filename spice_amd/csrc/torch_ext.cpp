@@ -1001,7 +1001,7 @@ std::tuple<Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &la
     c10::DeviceGuard guard(logits.device());
     const auto f32 = logits.options().dtype(at::kFloat);
     Tensor logp = at::empty(labels.sizes(), f32), stats = stats_for(labels, f32);
-    check_rc(spice_token_logprobs(&v.x, &v.y, (float)temperature, logp.data_ptr<float>(), stats.data_ptr<float>(),
+    check_rc(spice_token_logprobs(&v.x, &v.y, temperature, logp.data_ptr<float>(), stats.data_ptr<float>(),
                                   current_stream(logits)),
              "spice_token_logprobs");
     return std::make_tuple(logp, stats);
@@ -1032,7 +1032,7 @@ Tensor token_logprobs_grad(const Tensor &logits, const Tensor &labels, const Ten
         check_apart(writes, reads, "token_logprobs_grad");
     }
     Tensor grad = out.has_value() ? *out : at::empty(logits.sizes(), logits.options());
-    check_rc(spice_token_logprobs_grad(&v.x, &v.y, (float)temperature, stats.data_ptr<float>(), weight.data_ptr<float>(),
+    check_rc(spice_token_logprobs_grad(&v.x, &v.y, temperature, stats.data_ptr<float>(), weight.data_ptr<float>(),
                                        per_sequence ? 1 : v.x.l, per_sequence ? 0 : 1, (float)scale,
                                        one_float(device_scale, "device_scale", logits), out.has_value() ? 1 : 0,
                                        v.last ? 1 : 0, grad.data_ptr(), current_stream(logits)),
@@ -1069,19 +1069,19 @@ std::vector<Tensor> preference_loss(const Tensor &logits, const Tensor &labels, 
         stats_p = stats.data_ptr<float>();
         weight_p = weight.data_ptr<float>();
     }
-    spice_preference_params p;
-    p.temperature = (float)temperature;
-    p.beta = (float)beta;
-    p.smoothing = (float)smoothing;
+    spice_preference_options p;
+    p.temperature = temperature;
+    p.beta = beta;
+    p.smoothing = smoothing;
     p.loss_type = (int32_t)loss_type;
     p.average = average ? 1 : 0;
     void *stream = current_stream(logits);
-    check_rc(spice_preference_loss(&v.x, &v.y, ref_logprobs.data_ptr<float>(), &p, total.data_ptr<float>(),
-                                   rewards.data_ptr<float>(), weight_p, nullptr, stats_p, scratch.data_ptr(), (size_t)ws_bytes, stream),
-             "spice_preference_loss");
+    check_rc(spice_preference_loss_opts(&v.x, &v.y, ref_logprobs.data_ptr<float>(), &p, total.data_ptr<float>(),
+                                        rewards.data_ptr<float>(), weight_p, stats_p, scratch.data_ptr(), (size_t)ws_bytes, stream),
+             "spice_preference_loss_opts");
     if (!want_grad) return {total, rewards, weight, stats};
     Tensor grad = at::empty(logits.sizes(), logits.options());
-    check_rc(spice_token_logprobs_grad(&v.x, &v.y, (float)temperature, stats_p, weight_p, 1, 0, (float)grad_scale, nullptr, 0,
+    check_rc(spice_token_logprobs_grad(&v.x, &v.y, temperature, stats_p, weight_p, 1, 0, (float)grad_scale, nullptr, 0,
                                        v.last ? 1 : 0, grad.data_ptr(), stream),
              "spice_token_logprobs_grad");
     return {total, rewards, grad};
@@ -1114,20 +1114,23 @@ std::vector<Tensor> policy_loss(const Tensor &logits, const Tensor &labels, cons
         stats = stats_for(labels, f32);
         weight = at::empty(labels.sizes(), f32);
     }
-    spice_policy_params p;
-    p.temperature = (float)temperature;
-    p.clip_low = (float)clip_low;
-    p.clip_high = (float)clip_high;
-    p.kl_weight = (float)kl_weight;
-    p.grad_scale = (float)grad_scale;
+    spice_policy_options p;
+    p.temperature = temperature;
+    p.clip_low = clip_low;
+    p.clip_high = clip_high;
+    p.kl_weight = kl_weight;
+    p.grad_scale = grad_scale;
     p.reduction = (int32_t)reduction;
-    check_rc(spice_policy_loss(&v.x, &v.y, old_logprobs.data_ptr<float>(), advantages.data_ptr<float>(),
-                               per_sequence ? 1 : v.x.l, per_sequence ? 0 : 1,
-                               ref_logprobs.has_value() ? ref_logprobs->data_ptr<float>() : nullptr, &p, out4.data_ptr<float>(),
-                               logp.data_ptr<float>(), want_weight ? stats.data_ptr<float>() : nullptr,
-                               want_weight ? weight.data_ptr<float>() : nullptr, v.last ? 1 : 0,
-                               want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), current_stream(logits)),
-             "spice_policy_loss");
+    p.pad_ = 0;
+    check_rc(spice_policy_loss_opts(&v.x, &v.y, old_logprobs.data_ptr<float>(), advantages.data_ptr<float>(),
+                                    per_sequence ? 1 : v.x.l, per_sequence ? 0 : 1,
+                                    ref_logprobs.has_value() ? ref_logprobs->data_ptr<float>() : nullptr, &p,
+                                    out4.data_ptr<float>(), logp.data_ptr<float>(),
+                                    want_weight ? stats.data_ptr<float>() : nullptr,
+                                    want_weight ? weight.data_ptr<float>() : nullptr, v.last ? 1 : 0,
+                                    want_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(),
+                                    current_stream(logits)),
+             "spice_policy_loss_opts");
     if (want_weight) return {out4, logp, grad, stats, weight};
     if (want_grad) return {out4, logp, grad};
     return {out4, logp};

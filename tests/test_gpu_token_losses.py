@@ -758,10 +758,10 @@ def test_rows_keep_a_long_tail(dev, layout, n, positions, c, dtype):
 
 @pytest.mark.parametrize("layout, positions, c", [("last", (1000,), 2), ("last", (1000,), 300), ("last", (100,), 5000), ("last", (100,), 90000),
                                                   ("planes", (1000,), 2), ("planes", (1000,), 40), ("planes", (200,), 300)])
-@pytest.mark.parametrize("t", [1.0])
+@pytest.mark.parametrize("t", [1.0, 0.7])
 def test_log_ratios_of_many_positions_that_round_alike(dev, layout, positions, c, t):
     """Every position's label lies 8 - 0.4 steps below the maximum, which a subtraction in fp32 rounds to 8, and all the same way:
-    a sequence's log ratio adds that up.  Two classes count (the rest are -inf): the
+    a sequence's log ratio adds that up.  Nor may T = 0.7 be its neighbour in fp32.  Two classes count (the rest are -inf): the
     other one's exp(-8 / T) is off by 24 u at most (its distance, the product of up to 16.5, the instruction), its addition to
     the maximum's 1 rounds by half a step at 1, which is u (all further ones add zeros), and a position's log ratio, where it
     is kept in fp32, by u."""
@@ -804,3 +804,19 @@ def test_log_ratios_are_held_in_64_bits(dev, layout, c, l):
     # (h is off by 2^-47 at most, the square by twice that of its root)
     assert abs(total.item() - off * off) <= U * off * off + 2 * 2.0 ** -47 * abs(off)
     assert ((rewards.cpu().double() - 0.125 * s).abs() <= U * 0.125 * s.abs() + 2.0 ** -50).all()
+
+
+def test_preference_options_keep_their_precision(dev):
+    """ipo: h - 1 / (2 beta) is a difference: beta = 0.1 may not be its neighbour in fp32.  Two equal classes: logp =
+    -log 2 up to 2^-50, h is exact, the loss rounds to fp32 once."""
+    x = torch.zeros(2, 2, 1, device=dev)
+    y = torch.zeros(2, 1, dtype=torch.int64, device=dev)
+    for beta, off in ((0.1, 1e-4), (0.3, -3e-5), (0.7, 1e-3)):
+        ref = torch.tensor([[-math.log(2.0) - 0.5 / beta - off], [-math.log(2.0)]]).float()
+        h = ref[1].double().item() - ref[0].double().item()
+        want = (h - 0.5 / beta) ** 2
+        total, rewards, grad = ops.preference_loss(x, y, ref.to(dev), beta=beta, loss_type="ipo", want_grad=True)
+        # (h is off by 2^-48 at most, the square by twice that of its root)
+        assert abs(total.item() - want) <= U * want + 2 * 2.0 ** -48 * math.sqrt(want)
+        slope = 2 * (h - 0.5 / beta)
+        assert abs(grad[0, 0, 0].item() - 0.5 * slope) <= 4 * U * abs(slope) + 2.0 ** -48

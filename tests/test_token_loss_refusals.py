@@ -257,3 +257,27 @@ def test_states_that_are_not_its_own_are_refused_as_a_whole():
         with pytest.raises(ValueError, match=text):
             opt.load_state_dict(state)
         assert opt.param_groups[0]["lr"] == 0.25 and not opt.state[q]
+
+
+def test_c_abi_checks_the_options_in_full_precision():
+    L = nat.lib()
+    assert ctypes.sizeof(nat.PreferenceOptions) == 32 and ctypes.sizeof(nat.PolicyOptions) == 48
+    need = L.spice_token_loss_workspace_bytes(2, 3)
+
+    def pref(*p, size=need):
+        return L.spice_preference_loss_opts(_logits(), _labels(), 16, nat.PreferenceOptions(*p), 16, 16, 16, 16, 16, size, None)
+
+    def pol(*p, ref=None, size=need):
+        return L.spice_policy_loss_opts(_logits(), _labels(), 16, 16, 1, 0, ref, nat.PolicyOptions(*p), 16, 16, None, None, 1, None, 16,
+                                        size, None)
+
+    nan, inf = float("nan"), float("inf")
+    for bad in ((0.0, 0.1, 0.0, 0, 0), (nan, 0.1, 0.0, 0, 0), (inf, 0.1, 0.0, 0, 0), (1e-39, 0.1, 0.0, 0, 0), (1.0, 0.0, 0.0, 0, 0),
+                (1.0, nan, 0.0, 0, 0), (1.0, inf, 0.0, 0, 0), (1.0, 0.1, 0.5, 0, 0), (1.0, 0.1, -0.1, 0, 0), (1.0, 0.1, 0.0, 2, 0),
+                (1.0, 0.1, 0.1, 1, 0)):
+        assert pref(*bad) == nat.ERR_ARG, bad
+    assert pref(1.0, 0.1, 0.0, 0, 0, size=need - 1) == nat.ERR_WORKSPACE
+    for bad in ((nan, 0.2, 0.2, 0.0, 1.0, 0), (1.0, -0.1, 0.2, 0.0, 1.0, 0), (1.0, 1.1, 0.2, 0.0, 1.0, 0), (1.0, 0.2, nan, 0.0, 1.0, 0),
+                (1.0, 0.2, 0.2, 0.1, 1.0, 0), (1.0, 0.2, 0.2, -1.0, 1.0, 0), (1.0, 0.2, 0.2, 0.0, 1.0, 2)):
+        assert pol(*bad) == nat.ERR_ARG, bad
+    assert pol(1.0, 0.2, 0.2, 0.0, 1.0, 0, size=need - 1) == nat.ERR_WORKSPACE
