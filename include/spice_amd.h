@@ -657,11 +657,11 @@ size_t spice_grad_norm_workspace_bytes(const int64_t *numel, int32_t count);
 /* record[0] = norm over all tensors (squares summed in fp64, fixed order), record[1] = min(1, max_norm / (norm + 1e-6)).
  * A NaN or infinite gradient makes the norm NaN or infinite and the factor NaN or 0. */
 int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
-                    float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
+                    double max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
 
 /* The same over tensors of several types: dtypes [count] on the host. */
 int spice_grad_norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *numel, int32_t count, int32_t norm_type,
-                             float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
+                             double max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream);
 
 /* out = record[1] * grads, rounded once to out_dtype (the gradients' own, or fp32).  out may be grads (then nothing is
  * moved where the factor is 1); other overlaps are not allowed. */
@@ -670,7 +670,7 @@ int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t
 
 /* Both in one call (and one launch where the tensors hold few elements). */
 int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
-                         int32_t count, int32_t norm_type, float max_norm, float *record, void *workspace,
+                         int32_t count, int32_t norm_type, double max_norm, float *record, void *workspace,
                          size_t workspace_bytes, void *stream);
 
 typedef struct spice_adam_params {
@@ -687,6 +687,16 @@ typedef struct spice_adam_params {
 int spice_adam_step(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
                     const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_params *p, const float *norm,
                     int64_t *step, float *record, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same with a max_norm that keeps its precision, as the norms above take it. */
+typedef struct spice_adam_options {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    int64_t step;
+    int32_t decoupled, pad_;
+} spice_adam_options;
+int spice_adam_step_opts(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
+                         const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_options *options,
+                         const float *norm, int64_t *step, float *record, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -100,6 +100,11 @@ class AdamParams(Structure):
                 ("step", c_int64), ("max_norm", c_float), ("decoupled", c_int32)]
 
 
+class AdamOptions(Structure):
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+                ("max_norm", c_double), ("step", c_int64), ("decoupled", c_int32), ("pad_", c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/spice_amd.h declares
 SIGNATURES = {
     "spice_abi_version": (c_int32, []),
@@ -187,17 +192,20 @@ SIGNATURES = {
                                          POINTER(PolicyOptions), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
                                          c_void_p, c_size_t, c_void_p]),
     "spice_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int32]),
-    "spice_grad_norm": (c_int32, [POINTER(c_void_p), POINTER(c_int64), c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
+    "spice_grad_norm": (c_int32, [POINTER(c_void_p), POINTER(c_int64), c_int32, c_int32, c_int32, c_double, c_void_p, c_void_p,
                                   c_size_t, c_void_p]),
-    "spice_grad_norm_of_types": (c_int32, [POINTER(c_void_p), POINTER(c_int32), POINTER(c_int64), c_int32, c_int32, c_float,
+    "spice_grad_norm_of_types": (c_int32, [POINTER(c_void_p), POINTER(c_int32), POINTER(c_int64), c_int32, c_int32, c_double,
                                            c_void_p, c_void_p, c_size_t, c_void_p]),
     "spice_grad_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_void_p,
                                   c_void_p]),
     "spice_grad_norm_clip": (c_int32, [POINTER(c_void_p), c_int32, POINTER(c_void_p), c_int32, POINTER(c_int64), c_int32, c_int32,
-                                       c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                       c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
     "spice_adam_step": (c_int32, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64),
                                   c_int32, c_int32, POINTER(AdamParams), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                   c_void_p]),
+    "spice_adam_step_opts": (c_int32, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p),
+                                       POINTER(c_int64), c_int32, c_int32, POINTER(AdamOptions), c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

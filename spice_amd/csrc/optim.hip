@@ -532,17 +532,17 @@ int norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *nume
     }
     return record_of(a, part - item_count(numel, count, each), numel, count, s);
 }
-bool norm_ok(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type, float max_norm,
+bool norm_ok(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type, double max_norm,
              const float *record, const void *workspace) {
     return dtype >= 0 && dtype <= 2 && counts_ok(numel, count) && pointers_ok(grads, numel, count, type_bytes(dtype)) && record &&
-           workspace && aligned8(workspace) && norm_type >= 0 && norm_type <= 1 && max_norm >= 0.f;
+           workspace && aligned8(workspace) && norm_type >= 0 && norm_type <= 1 && max_norm >= 0.0;
 }
 
-RecordArgs norm_record(int32_t norm_type, float max_norm, float *record) {
+RecordArgs norm_record(int32_t norm_type, double max_norm, float *record) {
     RecordArgs a = {};
     a.inf = norm_type == SPICE_NORM_INF;
     a.clip = 1;
-    a.max_norm = (double)max_norm;
+    a.max_norm = max_norm;
     a.record = record;
     return a;
 }
@@ -551,7 +551,7 @@ RecordArgs norm_record(int32_t norm_type, float max_norm, float *record) {
 }  // namespace spice
 
 extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type,
-                               float max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream) {
+                               double max_norm, float *record, void *workspace, size_t workspace_bytes, void *stream) {
     if (!norm_ok(grads, numel, count, dtype, norm_type, max_norm, record, workspace)) return SPICE_ERR_ARG;
     if (workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
     RecordArgs a = norm_record(norm_type, max_norm, record);
@@ -559,7 +559,7 @@ extern "C" int spice_grad_norm(void *const *grads, const int64_t *numel, int32_t
 }
 
 extern "C" int spice_grad_norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *numel, int32_t count,
-                                        int32_t norm_type, float max_norm, float *record, void *workspace, size_t workspace_bytes,
+                                        int32_t norm_type, double max_norm, float *record, void *workspace, size_t workspace_bytes,
                                         void *stream) {
     if (!norm_ok(grads, numel, count, 1, norm_type, max_norm, record, workspace) || (count && !dtypes)) return SPICE_ERR_ARG;
     for (int32_t i = 0; i < count; ++i)
@@ -570,7 +570,7 @@ extern "C" int spice_grad_norm_of_types(void *const *grads, const int32_t *dtype
 }
 
 extern "C" int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
-                                    int32_t count, int32_t norm_type, float max_norm, float *record, void *workspace,
+                                    int32_t count, int32_t norm_type, double max_norm, float *record, void *workspace,
                                     size_t workspace_bytes, void *stream) {
     if (!norm_ok(grads, numel, count, dtype, norm_type, max_norm, record, workspace) || !(out_dtype == dtype || out_dtype == 0) ||
         !pointers_ok(out, numel, count, type_bytes(out_dtype)))
@@ -604,17 +604,17 @@ extern "C" int spice_grad_clip(void *const *grads, int32_t dtype, void *const *o
                           : launch_clip<__bf16, __bf16>(grads, out, numel, count, record, s);
 }
 
-extern "C" int spice_adam_step(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
-                               const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_params *p,
-                               const float *norm, int64_t *step, float *record, void *workspace, size_t workspace_bytes,
-                               void *stream) {
+extern "C" int spice_adam_step_opts(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
+                                    const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_options *p,
+                                    const float *norm, int64_t *step, float *record, void *workspace, size_t workspace_bytes,
+                                    void *stream) {
     if (dtype < 0 || dtype > 2 || !p || !counts_ok(numel, count) || !pointers_ok(params, numel, count, type_bytes(dtype)) ||
         !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(exp_avg, numel, count, 4) ||
         !pointers_ok(exp_avg_sq, numel, count, 4) || !record || !(p->lr >= 0.0 && p->lr <= 1e30) ||
         !(p->beta1 >= 0.0 && p->beta1 < 1.0) || !(p->beta2 >= 0.0 && p->beta2 < 1.0) || !(p->eps >= 0.0) ||
         !(p->weight_decay >= 0.0) || (!step && p->step < 1) || p->max_norm != p->max_norm)
         return SPICE_ERR_ARG;
-    const bool clip = p->max_norm >= 0.f, take = clip && !norm;
+    const bool clip = p->max_norm >= 0.0, take = clip && !norm;
     if (take && (!workspace || !aligned8(workspace))) return SPICE_ERR_ARG;
     if (take && workspace_bytes < spice_grad_norm_workspace_bytes(numel, count)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -622,7 +622,7 @@ extern "C" int spice_adam_step(void *const *params, void *const *grads, void *co
     r.norm_in = clip ? norm : nullptr;
     r.clip = clip;
     r.adam = 1;
-    r.max_norm = (double)p->max_norm;
+    r.max_norm = p->max_norm;
     r.lr = p->lr;
     r.beta1 = p->beta1;
     r.beta2 = p->beta2;
@@ -649,4 +649,14 @@ extern "C" int spice_adam_step(void *const *params, void *const *grads, void *co
     return dtype == 0   ? launch_adam<float>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
            : dtype == 1 ? launch_adam<_Float16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s)
                         : launch_adam<__bf16>(params, grads, exp_avg, exp_avg_sq, numel, count, a, record, s);
+}
+
+extern "C" int spice_adam_step(void *const *params, void *const *grads, void *const *exp_avg, void *const *exp_avg_sq,
+                               const int64_t *numel, int32_t count, int32_t dtype, const spice_adam_params *p,
+                               const float *norm, int64_t *step, float *record, void *workspace, size_t workspace_bytes,
+                               void *stream) {
+    if (!p) return SPICE_ERR_ARG;
+    const spice_adam_options o = {p->lr, p->beta1, p->beta2, p->eps, p->weight_decay, p->max_norm, p->step, p->decoupled, 0};
+    return spice_adam_step_opts(params, grads, exp_avg, exp_avg_sq, numel, count, dtype, &o, norm, step, record, workspace,
+                                workspace_bytes, stream);
 }

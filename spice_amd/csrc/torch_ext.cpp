@@ -1209,11 +1209,11 @@ Tensor grad_norm(const TensorList &grads, double max_norm, bool inf, bool any_ty
     Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws = norm_workspace(g.n, like);
     const int32_t norm = inf ? SPICE_NORM_INF : SPICE_NORM_L2;
     if (any_type && std::any_of(g.types.begin(), g.types.end(), [&](int32_t t) { return t != g.types[0]; }))
-        check_rc(spice_grad_norm_of_types(g.p.data(), g.types.data(), g.n.data(), (int32_t)g.n.size(), norm, (float)max_norm,
+        check_rc(spice_grad_norm_of_types(g.p.data(), g.types.data(), g.n.data(), (int32_t)g.n.size(), norm, max_norm,
                                           record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
                  "spice_grad_norm_of_types");
     else
-        check_rc(spice_grad_norm(g.p.data(), g.n.data(), (int32_t)g.n.size(), type_code(type), norm, (float)max_norm,
+        check_rc(spice_grad_norm(g.p.data(), g.n.data(), (int32_t)g.n.size(), type_code(type), norm, max_norm,
                                  record.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), current_stream(like)),
                  "spice_grad_norm");
     return record;
@@ -1252,7 +1252,7 @@ Tensor grad_clip(const TensorList &grads, const TensorList &out, double max_norm
         record = at::empty({4}, like.options().dtype(at::kFloat));
         Tensor ws = norm_workspace(g.n, like);
         check_rc(spice_grad_norm_clip(g.p.data(), type_code(type), o.p.data(), type_code(out_type), g.n.data(), (int32_t)g.n.size(),
-                                      inf ? SPICE_NORM_INF : SPICE_NORM_L2, (float)max_norm, record.data_ptr<float>(), ws.data_ptr(),
+                                      inf ? SPICE_NORM_INF : SPICE_NORM_L2, max_norm, record.data_ptr<float>(), ws.data_ptr(),
                                       (size_t)ws.numel(), current_stream(like)),
                  "spice_grad_norm_clip");
     }
@@ -1295,19 +1295,20 @@ Tensor adam_step(const TensorList &params, const TensorList &grads, const Tensor
     Tensor record = at::empty({4}, like.options().dtype(at::kFloat)), ws;
     const bool take = max_norm >= 0.0 && !norm.has_value();
     if (take) ws = norm_workspace(p.n, like);
-    spice_adam_params a;
+    spice_adam_options a;
     a.lr = lr;
     a.beta1 = beta1;
     a.beta2 = beta2;
     a.eps = eps;
     a.weight_decay = weight_decay;
     a.step = host_step;
-    a.max_norm = (float)max_norm;
+    a.max_norm = max_norm;
     a.decoupled = decoupled ? 1 : 0;
-    check_rc(spice_adam_step(p.p.data(), g.p.data(), m.p.data(), v.p.data(), p.n.data(), (int32_t)p.n.size(), type_code(type), &a,
-                             one_float(norm, "norm", like), device_step, record.data_ptr<float>(), take ? ws.data_ptr() : nullptr,
-                             take ? (size_t)ws.numel() : 0, current_stream(like)),
-             "spice_adam_step");
+    a.pad_ = 0;
+    check_rc(spice_adam_step_opts(p.p.data(), g.p.data(), m.p.data(), v.p.data(), p.n.data(), (int32_t)p.n.size(), type_code(type),
+                                  &a, one_float(norm, "norm", like), device_step, record.data_ptr<float>(),
+                                  take ? ws.data_ptr() : nullptr, take ? (size_t)ws.numel() : 0, current_stream(like)),
+             "spice_adam_step_opts");
     written(params);
     written(exp_avg);
     written(exp_avg_sq);

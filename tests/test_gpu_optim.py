@@ -346,3 +346,24 @@ def test_steps_after_loading_are_the_uninterrupted_ones(dev, dtype):
     take(second, again, grads[1:])
     # (the norm's squares are added up in memory order: fp64, the same fp32 norm and factor)
     assert all(torch.equal(a, b) for a, b in zip(whole, second))
+
+
+def test_max_norm_keeps_its_precision(dev):
+    """The factor is max_norm / (norm + 1e-6) in fp64, rounded to fp32 once: with limits that fp32 does not hold, bit for bit.
+    The limits are those of 1000 whose factor would be another fp32 value had they been rounded themselves."""
+    f32 = lambda v: torch.tensor(v, dtype=torch.float64).float()  # noqa: E731
+    limits = [k / 700.0 for k in range(1, 1000) if f32(k / 700.0 / (3.0 + 1e-6)) != f32(f32(k / 700.0).double().item() / (3.0 + 1e-6))]
+    assert len(limits) > 50
+    for limit in limits[::10]:
+        want = f32(limit / (3.0 + 1e-6)) * torch.tensor(3.0)
+        for size in (1, 40000):      # one launch, and several
+            out = [torch.empty(size, device=dev)]
+            g = [torch.zeros(size, device=dev)]
+            g[0][0] = 3.0
+            ops.clip_grad_norm(g, limit, out=out)
+            assert out[0][0].item() == want.item()
+            m, v = [torch.zeros(size, device=dev)], [torch.zeros(size, device=dev)]
+            ops.adam_step([torch.zeros(size, device=dev)], g, m, v, 1, lr=1e-3, betas=(0.0, 0.0), max_norm=limit)
+            assert m[0][0].item() == want.item()
+            ops.clip_grad_norm(g, limit, error_if_nonfinite=True)
+            assert g[0][0].item() == want.item()

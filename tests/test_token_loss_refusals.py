@@ -281,3 +281,19 @@ def test_c_abi_checks_the_options_in_full_precision():
                 (1.0, 0.2, 0.2, 0.1, 1.0, 0), (1.0, 0.2, 0.2, -1.0, 1.0, 0), (1.0, 0.2, 0.2, 0.0, 1.0, 2)):
         assert pol(*bad) == nat.ERR_ARG, bad
     assert pol(1.0, 0.2, 0.2, 0.0, 1.0, 0, size=need - 1) == nat.ERR_WORKSPACE
+
+
+def test_c_abi_checks_the_adam_options():
+    L = nat.lib()
+    assert ctypes.sizeof(nat.AdamOptions) == 64
+    n, t = _counts(8, 8), _table(16, 64)
+    need = L.spice_grad_norm_workspace_bytes(n, 2)
+
+    def adam(lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.0, limit=1.0, step=1, ws=16, size=need):
+        return L.spice_adam_step_opts(t, t, t, t, n, 2, 0, nat.AdamOptions(lr, b1, b2, eps, wd, limit, step, 0), None, None, 16, ws, size,
+                                      None)
+
+    for bad in (dict(lr=-1.0), dict(b1=1.0), dict(b2=float("nan")), dict(eps=-1.0), dict(wd=-1.0), dict(limit=float("nan")), dict(step=0),
+                dict(ws=None), dict(ws=12)):
+        assert adam(**bad) == nat.ERR_ARG, bad
+    assert adam(size=need - 1) == nat.ERR_WORKSPACE
