@@ -544,7 +544,8 @@ int spice_conv3x3_bn_act_f16(const void *x, const void *weight9, void *y, int64_
  *   logp = (x_label - m) / T - log s          (0 where the label is ignore_index)
  * A label that is neither ignore_index nor in [0, c) gives NaN: logp, the loss and
  * that position's gradient.  Nothing that belongs to a position with ignore_index is
- * used; its gradient is zero.  ignore_index must not be a class.
+ * used; its gradient is zero.  ignore_index must not be a class.  Pointers are aligned to their element (statistics and
+ * workspace to 8 bytes), or SPICE_ERR_ARG comes back.
  * ------------------------------------------------------------------------- */
 typedef struct spice_logits {
     const void *data;

@@ -397,6 +397,8 @@ bool pointers_ok(void *const *p, const int64_t *numel, int32_t count, int64_t by
     return true;
 }
 
+bool on4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
 int64_t type_bytes(int32_t dtype) { return dtype == 0 ? 4 : 2; }
 
 template <typename T>
@@ -534,7 +536,7 @@ int norm_of_types(void *const *grads, const int32_t *dtypes, const int64_t *nume
 }
 bool norm_ok(void *const *grads, const int64_t *numel, int32_t count, int32_t dtype, int32_t norm_type, double max_norm,
              const float *record, const void *workspace) {
-    return dtype >= 0 && dtype <= 2 && counts_ok(numel, count) && pointers_ok(grads, numel, count, type_bytes(dtype)) && record &&
+    return dtype >= 0 && dtype <= 2 && counts_ok(numel, count) && pointers_ok(grads, numel, count, type_bytes(dtype)) && record && on4(record) &&
            workspace && aligned8(workspace) && norm_type >= 0 && norm_type <= 1 && max_norm >= 0.0;
 }
 
@@ -593,7 +595,8 @@ extern "C" int spice_grad_norm_clip(void *const *grads, int32_t dtype, void *con
 extern "C" int spice_grad_clip(void *const *grads, int32_t dtype, void *const *out, int32_t out_dtype, const int64_t *numel,
                                int32_t count, const float *record, void *stream) {
     if (dtype < 0 || dtype > 2 || !(out_dtype == dtype || out_dtype == 0) || !counts_ok(numel, count) ||
-        !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(out, numel, count, type_bytes(out_dtype)) || !record)
+        !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(out, numel, count, type_bytes(out_dtype)) || !record ||
+        !on4(record))
         return SPICE_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == 0) return launch_clip<float, float>(grads, out, numel, count, record, s);
@@ -612,7 +615,8 @@ extern "C" int spice_adam_step_opts(void *const *params, void *const *grads, voi
         !pointers_ok(grads, numel, count, type_bytes(dtype)) || !pointers_ok(exp_avg, numel, count, 4) ||
         !pointers_ok(exp_avg_sq, numel, count, 4) || !record || !(p->lr >= 0.0 && p->lr <= 1e30) ||
         !(p->beta1 >= 0.0 && p->beta1 < 1.0) || !(p->beta2 >= 0.0 && p->beta2 < 1.0) || !(p->eps >= 0.0) ||
-        !(p->weight_decay >= 0.0) || (!step && p->step < 1) || p->max_norm != p->max_norm)
+        !(p->weight_decay >= 0.0) || (!step && p->step < 1) || p->max_norm != p->max_norm || !on4(record) ||
+        !on4(norm) || !aligned8(step))
         return SPICE_ERR_ARG;
     const bool clip = p->max_norm >= 0.0, take = clip && !norm;
     if (take && (!workspace || !aligned8(workspace))) return SPICE_ERR_ARG;

@@ -1356,14 +1356,19 @@ unsigned grid_of(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks
 
 constexpr int64_t kThreadsMost = (int64_t)1 << 31;   // threads of a launch: a grid's are counted in 32 bits
 
+// Every pointer on its element's bytes (a power of two); NULL passes.
+bool on_bytes(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+template <typename... P>
+bool on_floats(P... p) { return (on_bytes(p, 4) && ...); }
+
 bool logits_ok(const spice_logits *x) {
     return x && x->n >= 0 && x->l >= 0 && x->c >= 1 && x->c <= 0x7fffffff - 65536 && x->dtype >= 0 && x->dtype <= 2 &&
-           (x->data || x->n == 0 || x->l == 0) &&
+           (x->data || x->n == 0 || x->l == 0) && on_bytes(x->data, x->dtype == 0 ? 4 : 2) &&
            (x->n == 0 || x->l <= ((int64_t)1 << 39) / x->n);
 }
 
 bool labels_ok(const spice_logits *x, const spice_labels *y) {
-    return y && (y->data || x->n == 0 || x->l == 0) && (y->ignore_index < 0 || y->ignore_index >= x->c);
+    return y && (y->data || x->n == 0 || x->l == 0) && aligned8(y->data) && (y->ignore_index < 0 || y->ignore_index >= x->c);
 }
 
 bool temperature_ok(double t) { return t > 0.0 && t <= 3.0e38 && 1.0 / t <= 3.0e38; }
@@ -1566,7 +1571,8 @@ extern "C" size_t spice_token_loss_workspace_bytes(int64_t n, int64_t l) {
 
 extern "C" int spice_token_logprobs(const spice_logits *x, const spice_labels *y, double temperature, float *logp, float *stats,
                                     void *stream) {
-    if (!logits_ok(x) || !labels_ok(x, y) || !temperature_ok(temperature) || (!logp && x->n * x->l) || !aligned8(stats))
+    if (!logits_ok(x) || !labels_ok(x, y) || !temperature_ok(temperature) || (!logp && x->n * x->l) || !aligned8(stats) ||
+        !on_floats(logp))
         return SPICE_ERR_ARG;
     TokArgs a = args_of(x, y, temperature);
     a.logp = logp;
@@ -1579,7 +1585,7 @@ extern "C" int spice_token_logprobs_grad(const spice_logits *x, const spice_labe
                                          const float *device_scale, int32_t unless_one, int32_t class_last, void *grad,
                                          void *stream) {
     if (!logits_ok(x) || !labels_ok(x, y) || !temperature_ok(temperature) || !aligned8(stats) || (unless_one && !device_scale) ||
-        ((!stats || !weight || !grad) && x->n * x->l))
+        ((!stats || !weight || !grad) && x->n * x->l) || !on_floats(weight, device_scale) || !on_bytes(grad, x->dtype == 0 ? 4 : 2))
         return SPICE_ERR_ARG;
     TokArgs a = args_of(x, y, temperature);
     a.stats_in = (const float2 *)stats;
@@ -1599,7 +1605,8 @@ extern "C" int spice_preference_loss_opts(const spice_logits *x, const spice_lab
     if (!logits_ok(x) || !labels_ok(x, y) || !p || x->n < 2 || x->n % 2 || !total || !rewards || !weight || !workspace ||
         !aligned8(workspace) || (!ref_logp && x->l) || !aligned8(stats) || !(p->beta > 0.0 && p->beta <= 3.0e38) ||
         !(p->smoothing >= 0.0 && p->smoothing < 0.5) || p->loss_type < 0 || p->loss_type > 1 ||
-        (p->loss_type == SPICE_PREFERENCE_IPO && p->smoothing != 0.0) || !temperature_ok(p->temperature))
+        (p->loss_type == SPICE_PREFERENCE_IPO && p->smoothing != 0.0) || !temperature_ok(p->temperature) ||
+        !on_floats(ref_logp, total, rewards, weight))
         return SPICE_ERR_ARG;
     if (workspace_bytes < spice_token_loss_workspace_bytes(x->n, x->l)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -1640,7 +1647,8 @@ extern "C" int spice_policy_loss_opts(const spice_logits *x, const spice_labels 
     if (!logits_ok(x) || !labels_ok(x, y) || !p || !out4 || !workspace || !aligned8(workspace) ||
         ((!old_logp || !advantages || !logp) && x->n * x->l) || !(p->clip_low >= 0.0 && p->clip_low <= 1.0) ||
         !(p->clip_high >= 0.0) || !(p->kl_weight >= 0.0) || (p->kl_weight > 0.0 && !ref_logp && x->n * x->l) ||
-        p->reduction < 0 || p->reduction > 1 || !aligned8(stats) || !temperature_ok(p->temperature))
+        p->reduction < 0 || p->reduction > 1 || !aligned8(stats) || !temperature_ok(p->temperature) ||
+        !on_floats(old_logp, advantages, ref_logp, out4, logp, weight) || !on_bytes(grad, x->dtype == 0 ? 4 : 2))
         return SPICE_ERR_ARG;
     if (workspace_bytes < spice_token_loss_workspace_bytes(x->n, x->l)) return SPICE_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;

@@ -297,3 +297,38 @@ def test_c_abi_checks_the_adam_options():
                 dict(ws=None), dict(ws=12)):
         assert adam(**bad) == nat.ERR_ARG, bad
     assert adam(size=need - 1) == nat.ERR_WORKSPACE
+
+
+def test_c_abi_checks_every_pointers_alignment():
+    """Before anything is queued: an address between two elements would fault on the device, or read half of each."""
+    L = nat.lib()
+    need, odd = L.spice_token_loss_workspace_bytes(2, 3), 18
+    pref_opts, pol_opts = nat.PreferenceOptions(1.0, 0.1, 0.0, 0, 0), nat.PolicyOptions(1.0, 0.2, 0.2, 0.1, 1.0, 0)
+
+    def logp(x=_logits(), y=_labels(), out=16, stats=16):
+        return L.spice_token_logprobs(x, y, 1.0, out, stats, None)
+
+    def grad(x=_logits(), y=_labels(), stats=16, weight=16, scale=16, out=16):
+        return L.spice_token_logprobs_grad(x, y, 1.0, stats, weight, 3, 1, 1.0, scale, 0, 1, out, None)
+
+    def pref(x=_logits(), y=_labels(), ref=16, total=16, rewards=16, weight=16, stats=16, ws=16):
+        return L.spice_preference_loss_opts(x, y, ref, pref_opts, total, rewards, weight, stats, ws, need, None)
+
+    def pol(x=_logits(), y=_labels(), old=16, adv=16, ref=16, out=16, logp=16, stats=16, weight=16, g=16, ws=16):
+        return L.spice_policy_loss_opts(x, y, old, adv, 1, 0, ref, pol_opts, out, logp, stats, weight, 1, g, ws, need, None)
+
+    for call, names in ((logp, ("out", "stats")), (grad, ("stats", "weight", "scale", "out")),
+                        (pref, ("ref", "total", "rewards", "weight", "stats", "ws")),
+                        (pol, ("old", "adv", "ref", "out", "logp", "stats", "weight", "g", "ws"))):
+        for name in names:
+            assert call(**{name: odd}) == nat.ERR_ARG, (call.__name__, name)
+        assert call(x=_logits(data=18)) == call(x=_logits(data=17, dtype=1)) == call(y=_labels(data=20)) == nat.ERR_ARG, call.__name__
+    assert grad(x=_logits(dtype=2), out=17) == pol(x=_logits(dtype=2), g=17) == nat.ERR_ARG
+    n, t = _counts(8, 8), _table(16, 64)
+    size = L.spice_grad_norm_workspace_bytes(n, 2)
+    a = nat.AdamOptions(1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, 1, 0)
+    assert L.spice_grad_norm(t, n, 2, 0, 0, 1.0, odd, 16, size, None) == nat.ERR_ARG
+    assert L.spice_grad_clip(t, 0, t, 0, n, 2, odd, None) == nat.ERR_ARG
+    assert L.spice_grad_norm_clip(t, 0, t, 0, n, 2, 0, 1.0, odd, 16, size, None) == nat.ERR_ARG
+    for norm, step, record in ((odd, None, 16), (None, 20, 16), (None, None, odd)):
+        assert L.spice_adam_step_opts(t, t, t, t, n, 2, 0, a, norm, step, record, 16, size, None) == nat.ERR_ARG
