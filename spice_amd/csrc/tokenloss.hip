@@ -424,7 +424,8 @@ __device__ __forceinline__ void grad_of(float (&v)[K], float m, float each, floa
     for (int k = 0; k < K; ++k) v[k] = each * exp_of(v[k] - m, t);
     if ((uint32_t)(y - c0) < (uint32_t)K) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += y - c0 == k ? w : 0.f;
+        for (int k = 0; k < K; ++k) v[k] = y - c0 == k ? v[k] + w : v[k];   // (+ 0 elsewhere would make -0 of a softmax of 0 a +0,
+                                                                            // and a class that two lanes store is one value)
     }
 }
 

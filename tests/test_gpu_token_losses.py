@@ -820,3 +820,27 @@ def test_preference_options_keep_their_precision(dev):
         assert abs(total.item() - want) <= U * want + 2 * 2.0 ** -48 * math.sqrt(want)
         slope = 2 * (h - 0.5 / beta)
         assert abs(grad[0, 0, 0].item() - 0.5 * slope) <= 4 * U * abs(slope) + 2.0 ** -48
+
+
+@pytest.mark.parametrize("layout, l, c", [("last", 3, 13), ("last", 3, 29), ("last", 5, 150), ("last", 2, 1001), ("last", 2, 5003),
+                                          ("last", 2, 50001), ("last", 1, 200003), ("planes", 9, 13), ("planes", 70, 45), ("planes", 2, 700)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_zeros_carry_one_sign(dev, layout, l, c, dtype):
+    """An excluded class's gradient is -w p with p = 0: minus zero for a positive weight, plus zero for a negative one, wherever
+    the label lies and whichever lane stores it (a row's last classes belong to two vectors)."""
+    d = -1 if layout == "last" else 1
+    for label in (0, c // 2, c - 9 if c > 9 else 1, c - 1):
+        x = torch.randn(2, l, c, generator=torch.Generator().manual_seed(label))
+        x[..., torch.arange(c) % 3 == (label + 1) % 3] = -math.inf
+        y = torch.full((2, l), label)
+        x = (x if d == -1 else x.movedim(-1, 1).contiguous()).to(dtype).to(dev)
+        y, weight = y.to(dev), torch.tensor([1.0, -2.0], device=dev)
+        how = dict(class_dim=d, ignore_index=-100)
+        logp, stats = ops.token_logprobs(x, y, **how)
+        grads = [ops.token_logprobs_grad(x, y, stats, weight, **how), ops.policy_loss(x, y, logp, -weight, want_grad=True, **how)[2]]
+        zero = torch.isinf(_last(x, d))
+        for k, g in enumerate(grads):      # (the surrogate -r A at A = -weight and r = 1: d / d logp = weight)
+            g = _last(g, d)
+            assert (g[zero] == 0).all()
+            right = torch.signbit(g) == (weight > 0).view(2, 1, 1)
+            assert right[zero].all(), (k, label)
