@@ -1316,12 +1316,25 @@ Tensor adam_step(const TensorList &params, const TensorList &grads, const Tensor
     return record;
 }
 
+// What the current stream of `like`'s device is being captured into: a number of its own for each capture, 0 for none, -1 where
+// it cannot be asked now (the default stream while another one captures).
+int64_t capture_id(const Tensor &like) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)current_stream(like), &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return -1;
+    }
+    return status == hipStreamCaptureStatusNone ? 0 : (int64_t)(id + 1);
+}
+
 int64_t abi_version() { return spice_abi_version(); }
 
 }  // namespace
 
 TORCH_LIBRARY(spice, m) {
     m.def("abi_version() -> int", &abi_version);
+    m.def("capture_id(Tensor like) -> int", &capture_id);
     m.def("importance_run(Tensor[] weights, Tensor[] grads, Tensor(a!) scores, Tensor items, int n_items, int mode, "
           "bool accumulate) -> ()", &importance_run);
     m.def("importance_cols_run(Tensor[] weights, Tensor(a!) scores, Tensor(b!) partial, Tensor items, int n_items, "

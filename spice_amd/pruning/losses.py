@@ -206,7 +206,9 @@ class _Preference(torch.autograd.Function):
 
 class _Policy(torch.autograd.Function):
     """The gradient for an upstream factor of 1 is written by the forward pass over the logits; backward takes it anew
-    from the logits where the factor is another one (decided on the device), so that it is rounded once either way."""
+    from the logits where the factor is another one (decided on the device), so that it is rounded once either way.
+    It is handed on only where forward and backward run once each: both eagerly, or both in one capture.  A backward pass
+    that is replayed by itself would find what the last replay, or the caller, left there."""
 
     @staticmethod
     def forward(ctx, logits, labels, old, advantages, ref, how, opts, want):
@@ -214,7 +216,7 @@ class _Policy(torch.autograd.Function):
             logits.detach(), labels, old, advantages, ref, how["class_dim"], how["temperature"], how["ignore_index"], *opts,
             want, 1.0, want)
         if want:
-            ctx.how, ctx.grad = how, saved[0]
+            ctx.how, ctx.grad, ctx.capture = how, saved[0], ops.spice_ops().capture_id(logits)
             ctx.save_for_backward(logits, labels, *saved[1:])
         parts = out4.unbind()
         total, rest = parts[0].clone(), [p.clone() for p in parts[1:]]
@@ -226,6 +228,8 @@ class _Policy(torch.autograd.Function):
     def backward(ctx, g_total, *_):
         logits, labels, stats, weight = ctx.saved_tensors
         out, ctx.grad = ctx.grad, None   # (handed on: a second backward through the same graph takes a new one)
+        if ctx.capture < 0 or ctx.capture != ops.spice_ops().capture_id(logits):
+            out = None
         return (ops.token_logprobs_grad(logits.detach(), labels, stats, weight, device_scale=g_total.float().contiguous(),
                                         out=out, **ctx.how), *([None] * 7))
 

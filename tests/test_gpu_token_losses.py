@@ -844,3 +844,51 @@ def test_zeros_carry_one_sign(dev, layout, l, c, dtype):
             assert (g[zero] == 0).all()
             right = torch.signbit(g) == (weight > 0).view(2, 1, 1)
             assert right[zero].all(), (k, label)
+
+
+def test_policy_gradients_of_captured_passes(dev):
+    """The forward pass leaves a gradient for a factor of 1.  Captured with its backward pass, apart from it, or a captured
+    backward pass of an eager forward: every replay, at another factor and with its last result overwritten, is the eager one."""
+    x, y, d, ignore = _inputs("last", 3, (20,), 1000, torch.bfloat16, seed=61)
+    y, adv = y.to(dev), torch.randn(3, generator=torch.Generator().manual_seed(1)).to(dev)
+    old = ops.token_logprobs(x.to(dev), y, class_dim=d, ignore_index=ignore)[0] - 0.05
+    loss = ClippedPolicyLoss(kl_weight=0.1, class_dim=d, ignore_index=ignore)
+    want = [ops.policy_loss(x.to(dev), y, old, adv, ref_logprobs=old, kl_weight=0.1, clip_low=0.2, clip_high=0.2, class_dim=d,
+                            ignore_index=ignore, want_grad=True, grad_scale=s)[2] for s in (1.0, 2.0)]
+    side = torch.cuda.Stream()
+
+    for how in ("one capture", "two captures", "eager forward"):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            factor, base = torch.ones((), device=dev), x.to(dev).requires_grad_(True)
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+
+        def ahead():
+            logits = base * 1      # (no leaf's accumulator takes part)
+            return logits, loss(logits, y, old, adv, ref_logprobs=old)["total"]
+
+        if how == "one capture":
+            with torch.cuda.graph(graphs[1], stream=side):
+                logits, total = ahead()
+                got, = torch.autograd.grad(total, logits, factor)
+            graphs = graphs[1:]
+        else:
+            if how == "two captures":
+                with torch.cuda.graph(graphs[0], stream=side):
+                    logits, total = ahead()
+            else:
+                with torch.cuda.stream(side):
+                    logits, total = ahead()
+                graphs = graphs[1:]
+            side.synchronize()
+            with torch.cuda.graph(graphs[-1], stream=side):
+                got, = torch.autograd.grad(total, logits, factor)
+        for g in graphs[:-1]:
+            g.replay()
+        for turn, k in enumerate((0, 1, 0, 0, 1)):
+            factor.fill_(1.0 + k)
+            got.zero_()
+            graphs[-1].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want[k]), (how, turn)
+        del got, total, logits
