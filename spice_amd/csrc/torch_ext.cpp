@@ -908,6 +908,11 @@ bool one_axis(const Tensor &t, int64_t from, int64_t to, int64_t &size, int64_t 
     size = 1;
     stride = 1;
     bool any = false;
+    for (int64_t d = from; d < to; ++d)
+        if (t.size(d) == 0) {      // no elements: at any stride
+            size = 0;
+            return true;
+        }
     for (int64_t d = to - 1; d >= from; --d) {
         if (t.size(d) == 1) continue;
         if (any && t.stride(d) != stride * size) return false;

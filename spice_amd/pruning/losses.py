@@ -236,6 +236,8 @@ class _Policy(torch.autograd.Function):
 
 def _one_stride(t: torch.Tensor, first: int, last: int) -> bool:
     """Whether the axes first .. last - 1 of t lie at one stride in memory."""
+    if 0 in t.shape[first:last]:
+        return True
     size = step = None
     for d in range(last - 1, first - 1, -1):
         if t.shape[d] == 1:

@@ -892,3 +892,21 @@ def test_policy_gradients_of_captured_passes(dev):
             torch.cuda.synchronize()
             assert torch.equal(got, want[k]), (how, turn)
         del got, total, logits
+
+
+@pytest.mark.parametrize("d, shape", [(-1, (2, 3, 0, 5)), (-1, (2, 0, 4, 5)), (1, (2, 5, 3, 0)), (1, (2, 5, 0, 3)), (-1, (0, 3, 4, 5)), (1, (2, 300, 0, 3))])
+def test_no_positions_on_several_axes(dev, d, shape):
+    x = torch.zeros(shape, device=dev, dtype=torch.bfloat16)
+    lab = _last(x, d).shape[:-1]
+    y, f = torch.zeros(lab, dtype=torch.int64, device=dev), torch.zeros(lab, device=dev)
+    how = dict(class_dim=d, ignore_index=-100)
+    logp, stats = ops.token_logprobs(x, y, **how)
+    assert logp.shape == lab and ops.token_logprobs_grad(x, y, stats, f, **how).shape == shape
+    out, _, grad = ops.policy_loss(x, y, f, f, want_grad=True, **how)
+    assert (out == 0).all() and grad.shape == shape
+    leaf = x.clone().requires_grad_(True)
+    (token_logprobs(leaf, y, **how).sum() + ClippedPolicyLoss(**how)(leaf, y, f, f)["total"]).backward()
+    assert leaf.grad.shape == shape
+    if shape[0]:
+        total, rewards, grad = ops.preference_loss(x, y, f, want_grad=True, **how)
+        assert abs(total.item() - math.log(2)) <= 2 * U and (rewards == 0).all() and grad.shape == shape
