@@ -194,8 +194,8 @@ __device__ __forceinline__ void far_of(float q, float &far, float &e1) {
 __device__ __forceinline__ PolicyTerm policy_term(const Policy &p, const PolicyIn &in, float logp) {
     PolicyTerm r;
     const float a = in.adv;
-    const float ratio = expf(logp - in.old_logp);
-    const float free = ratio * a;
+    const float moved = logp - in.old_logp, ratio = expf(moved);
+    const float free = a == 0.f && moved < INFINITY ? 0.f : ratio * a;   // (a ratio past fp32's range is finite all the same)
     const float held = fminf(fmaxf(ratio, p.low), p.high) * a;
     r.over = free > held;
     r.surrogate = r.over ? -held : -free;

@@ -910,3 +910,27 @@ def test_no_positions_on_several_axes(dev, d, shape):
     if shape[0]:
         total, rewards, grad = ops.preference_loss(x, y, f, want_grad=True, **how)
         assert abs(total.item() - math.log(2)) <= 2 * U and (rewards == 0).all() and grad.shape == shape
+
+
+@pytest.mark.parametrize("layout, positions, c", [("last", (6,), 1000), ("last", (40,), 9), ("last", (3,), 90001), ("planes", (8, 12), 21),
+                                                  ("planes", (5, 7), 70), ("planes", (6,), 3001)])
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_positions_without_an_advantage_add_nothing(dev, layout, positions, c, reduction):
+    """r A = 0 for A = 0, however far the policy has moved: r = exp(200) is no fp32 value, and yet finite; a place holder of -1e9
+    as the old log-probability alike."""
+    x, y, d, ignore = _inputs(layout, 2, positions, c, torch.float32, seed=71)
+    how = dict(class_dim=d, ignore_index=ignore, reduction=reduction)
+    xd, yd = x.to(dev), y.to(dev)
+    old = ops.token_logprobs(xd, yd, class_dim=d, ignore_index=ignore)[0] - 0.05
+    adv = torch.randn(y.shape, generator=torch.Generator().manual_seed(72)).to(dev)
+    adv.view(-1)[::3] = 0.0
+    want = ops.policy_loss(xd, yd, old, adv, want_grad=True, **how)
+    far = old.clone()
+    far.view(-1)[::3] = -200.0
+    far.view(-1)[::6] = -1e9
+    got = ops.policy_loss(xd, yd, far, adv, want_grad=True, **how)
+    for a, b in zip(want, got):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    far.view(-1)[3] = -math.inf        # an excluded label's: its ratio is infinite, the product undefined
+    if y.view(-1)[3] != ignore:
+        assert torch.isnan(ops.policy_loss(xd, yd, far, adv, **how)[0][0])
