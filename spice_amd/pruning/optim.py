@@ -32,6 +32,9 @@ class ClippedAdam(torch.optim.Optimizer):
         self.last_grad_norm: Optional[torch.Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled))
 
+    def __getstate__(self) -> dict:      # (the base class keeps its own three attributes alone)
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "last_grad_norm": self.last_grad_norm}
+
     def _state_of(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if not state:

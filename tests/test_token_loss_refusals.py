@@ -1,5 +1,7 @@
 """What the loss and update entry points refuse, and what runs without a device."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -332,3 +334,12 @@ def test_c_abi_checks_every_pointers_alignment():
     assert L.spice_grad_norm_clip(t, 0, t, 0, n, 2, 0, 1.0, odd, 16, size, None) == nat.ERR_ARG
     for norm, step, record in ((odd, None, 16), (None, 20, 16), (None, None, odd)):
         assert L.spice_adam_step_opts(t, t, t, t, n, 2, 0, a, norm, step, record, 16, size, None) == nat.ERR_ARG
+
+
+def test_copies_of_the_optimizer_keep_its_limit():
+    p = torch.nn.Parameter(torch.ones(5))
+    opt = _with_state([p], lr=0.5, max_grad_norm=0.25)
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert again.max_grad_norm == 0.25 and again.last_grad_norm is None and again.param_groups[0]["lr"] == 0.5
+        q, = again.param_groups[0]["params"]
+        assert again.state[q]["step"] == 3 and torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"])
