@@ -934,3 +934,54 @@ def test_positions_without_an_advantage_add_nothing(dev, layout, positions, c, r
     far.view(-1)[3] = -math.inf        # an excluded label's: its ratio is infinite, the product undefined
     if y.view(-1)[3] != ignore:
         assert torch.isnan(ops.policy_loss(xd, yd, far, adv, **how)[0][0])
+
+
+@pytest.mark.parametrize("t", [0.7, 1.3])
+@pytest.mark.parametrize("shape", [("last", 4, (37,), 1031, torch.bfloat16), ("last", 6, (3000,), 7, torch.float32), ("last", 2, (9,), 50001, torch.float16),
+                                   ("planes", 4, (24, 20), 21, torch.float32), ("planes", 2, (30, 22), 150, torch.float32)],
+                         ids=lambda s: "%s-%d" % (s[0], s[3]))
+@pytest.mark.parametrize("average", [False, True])
+def test_preference_loss_at_a_temperature(dev, shape, t, average):
+    """The bounds of test_preference_loss, at T != 1."""
+    x, y, d, ignore = _inputs(*shape, seed=81)
+    beta, n = 0.3, x.shape[0]
+    how = dict(class_dim=d, ignore_index=ignore, temperature=t)
+    lp, keep = ot.token_logprobs(x.double(), y, **how)
+    ref = (lp + 0.3 * torch.randn(y.shape, generator=torch.Generator().manual_seed(82), dtype=torch.float64)).float()
+    v = x.double().requires_grad_(True)
+    total, rewards = ot.preference(v, y, ref, beta=beta, average=average, **how)
+    g64, = torch.autograd.grad(total, v)
+    got, rew, grad = ops.preference_loss(x.to(dev), y.to(dev), ref.to(dev), beta=beta, average=average, want_grad=True, **how)
+    tr = _ratio_tol(x, lp, keep, d, t, average)
+    _close(rew, rewards.detach(), beta * tr + 2 * U * rewards.detach().abs(), "rewards")
+    th = tr[: n // 2] + tr[n // 2:]
+    _close(got, total.detach(), (beta * th).mean() + 2 * U * total.detach().abs(), "total")
+    r = rewards.detach() / beta
+    dh = -beta * torch.sigmoid(-beta * (r[: n // 2] - r[n // 2:]))
+    ddh = beta * beta / 4 * th + 4 * U * dh.abs()
+    counts = keep.reshape(n, -1).sum(1).clamp(min=1).double() if average else torch.ones(n, dtype=torch.float64)
+    wide = lambda s: (torch.cat([s, s]).abs() / (n // 2) / counts).view(-1, *([1] * (y.dim() - 1))).expand(y.shape)  # noqa: E731
+    _close(grad, g64, _grad_tol(x, g64, wide(dh), d, t) + (wide(ddh) / t).unsqueeze(d if d == 1 else -1), "grad")
+
+
+@pytest.mark.parametrize("shape", [("last", 3, (41,), 1025, torch.bfloat16), ("last", 2, (7,), 50001, torch.float16), ("last", 4, (40,), 6, torch.float32),
+                                   ("last", 2, (3,), 140001, torch.bfloat16), ("planes", 3, (24, 20), 21, torch.float32),
+                                   ("planes", 2, (30, 22), 150, torch.float32), ("planes", 2, (6,), 3001, torch.float32)],
+                         ids=lambda s: "%s-%d" % (s[0], s[3]))
+def test_policy_module_gradients_under_a_factor(dev, shape):
+    """Upstream factors of 1, 4 and 1/8, value by value: old = logp, so r = 1 up to logp's error and d / d logp = -A share."""
+    x, y, d, ignore = _inputs(*shape, seed=91)
+    how = dict(class_dim=d, ignore_index=ignore)
+    lp, keep = ot.token_logprobs(x.double(), y, **how)
+    adv = torch.randn(x.shape[0], generator=torch.Generator().manual_seed(92))
+    wide = torch.where(keep, adv.double().view(-1, *([1] * (y.dim() - 1))).expand(y.shape), 0.0)
+    tl = _bounds(x, d, 1.0)[1] + 3 * U * lp.abs()
+    for factor in (1.0, 4.0, 0.125):
+        v = x.double().requires_grad_(True)
+        w = -factor * wide / keep.sum()
+        g64, = torch.autograd.grad((ot.token_logprobs(v, y, **how)[0] * w).sum(), v)
+        leaf = x.to(dev).requires_grad_(True)
+        (factor * ClippedPolicyLoss(**how)(leaf, y.to(dev), lp.float().to(dev), adv.to(dev))["total"]).backward()
+        # the weight: the ratio is off by logp's error and old's rounding, the exponential 3 u, the products and the share 4 u
+        extra = (w.abs() * (2 * tl + 8 * U)).unsqueeze(d if d == 1 else -1)
+        _close(leaf.grad, g64, _grad_tol(x, g64, w.abs(), d, 1.0) + extra, factor)
