@@ -81,7 +81,8 @@ class ClippedAdam(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
-        if torch.cuda.is_current_stream_capturing():
+        on_device = any(p.is_cuda for group in self.param_groups for p in group["params"])
+        if on_device and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("ClippedAdam counts its steps on the host: capture ops.adam_step with a device step count")
         loss = None
         if closure is not None:

@@ -343,3 +343,14 @@ def test_copies_of_the_optimizer_keep_its_limit():
         assert again.max_grad_norm == 0.25 and again.last_grad_norm is None and again.param_groups[0]["lr"] == 0.5
         q, = again.param_groups[0]["params"]
         assert again.state[q]["step"] == 3 and torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"])
+
+
+@pytest.mark.parametrize("types", [(torch.float32,), (torch.float32, torch.bfloat16)])
+def test_the_optimizer_refuses_host_parameters(types):
+    params = [torch.nn.Parameter(torch.ones(5, dtype=t)) for t in types]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = ClippedAdam(params, lr=0.5, max_grad_norm=1.0)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        opt.step()
+    assert all((p == 1).all() for p in params)
