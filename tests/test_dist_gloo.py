@@ -190,3 +190,64 @@ def test_gradient_buckets_average_over_ranks(tmp_path):
     assert sorted(list(two[0]["val_ids"]) + list(two[1]["val_ids"])) == list(range(10))
     assert not set(two[0]["val_ids"]) & set(two[1]["val_ids"])
     np.testing.assert_array_equal(two[0]["cal_first"], two[1]["cal_first"])  # same calibration order on all ranks
+
+
+def _clip_worker(rank, world, port, out_dir):
+    sys.path.insert(0, ROOT)
+    sys.path.insert(0, os.path.join(ROOT, "tests"))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    torch.set_num_threads(2)
+    if world > 1:
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+    from oracle import tokenloss as ot
+    from spice_amd import dist as sdist
+    from spice_amd import ops
+    from spice_amd.pruning.config import PruningConfig
+    from spice_amd.pruning.trainer import PruningTrainer
+    from toy_models import ToyNet
+
+    norms = []
+
+    def adam_step(params, grads, m, v, step, *, lr, betas, eps, weight_decay, decoupled, max_norm, norm):
+        total = ot.grad_norm(grads)
+        norms.append(total.item())
+        for p, g, a, b in zip(params, grads, m, v):
+            new = ot.adam(p, g, a, b, step, ot.clip_factor(total, max_norm), lr, betas, eps, weight_decay, decoupled)
+            for t, value in zip((p, a, b), new):
+                t.copy_(value)
+        return total.float()
+
+    ops.adam_step = adam_step           # the arithmetic by the oracle; the trainer, its buckets and its optimiser are the product's
+    trainer = PruningTrainer.__new__(PruningTrainer)
+    trainer.config = PruningConfig(model_name="UNET_resnet", num_classes=4, max_grad_norm=0.01, fine_tune_lr=1e-2, weight_decay=1e-2,
+                                   output_dir=out_dir, device="cpu", use_wandb=False)
+    torch.manual_seed(5)
+    net = ToyNet().eval()
+    opt = trainer._setup_optimizer(net)
+    trainer._grad_buckets = sdist.FlatGradBuckets(net.parameters(), bucket_bytes=256)
+    data = torch.Generator().manual_seed(77)
+    xs, ys = torch.randn(4, 3, 12, 12, generator=data), torch.randint(0, 4, (4, 12, 12), generator=data)
+    lo, hi = rank * 4 // world, (rank + 1) * 4 // world
+    for _ in range(3):
+        trainer._zero_grad(opt)
+        torch.nn.functional.cross_entropy(net(xs[lo:hi]), ys[lo:hi]).backward()
+        trainer._step(opt)
+    np.savez(os.path.join(out_dir, f"clip_rank{rank}_of{world}.npz"), norms=np.array(norms),
+             **{k: v.detach().numpy() for k, v in net.named_parameters()})
+    trainer._grad_buckets.close()
+    if world > 1:
+        dist.destroy_process_group()
+
+
+def test_two_ranks_clip_the_averaged_gradient(tmp_path):
+    """max_grad_norm under two ranks: the norm is that of the exchanged gradients, so both ranks clip and step alike, and like one
+    rank over the whole batch."""
+    for world in (1, 2):
+        mp.spawn(_clip_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
+    one, a, b = (np.load(os.path.join(tmp_path, f"clip_rank{r}_of{w}.npz")) for r, w in ((0, 1), (0, 2), (1, 2)))
+    assert len(one["norms"]) == 3 and (one["norms"] > 0.02).all()      # (the limit binds)
+    np.testing.assert_allclose(a["norms"], one["norms"], rtol=1e-4)
+    for k in one.files:
+        np.testing.assert_array_equal(a[k], b[k])
+        if k != "norms":      # (Adam's first steps are lr times a gradient's sign nearly: where one is around 0 they may differ)
+            assert (np.abs(a[k] - one[k]) > 1e-4).mean() < 0.02
