@@ -66,7 +66,7 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
 // bn_tail of bn_math.h for two neighbouring pixels of one channel at once, value for value the same: the fp32 steps
-// as packed operations, every rounding to fp16 a conversion of its own (never folded into the multiply-add before
+// as pairs of operations, every rounding to fp16 a conversion of its own (never folded into the multiply-add before
 // it), the clamp on the rounded halves (rounding is monotonic and keeps 0 and NaN, so max-then-round and
 // round-then-max agree).
 template <bool HAS_RES, bool RES_BN>

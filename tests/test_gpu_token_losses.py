@@ -985,3 +985,28 @@ def test_policy_module_gradients_under_a_factor(dev, shape):
         # the weight: the ratio is off by logp's error and old's rounding, the exponential 3 u, the products and the share 4 u
         extra = (w.abs() * (2 * tl + 8 * U)).unsqueeze(d if d == 1 else -1)
         _close(leaf.grad, g64, _grad_tol(x, g64, w.abs(), d, 1.0) + extra, factor)
+
+
+@pytest.mark.parametrize("shape", SHAPES + [("planes", 2, (300,), 5001, torch.float32), ("channels last", 1, (700,), 2000, torch.bfloat16)],
+                         ids=IDS + ["planes-2-300-5001-float32", "channels last-1-700-2000-bfloat16"])
+@pytest.mark.parametrize("t", [1.0, 0.7])
+def test_long_sums_stay_within_short_chains(dev, shape, t):
+    """The bound of sums in short trees joined in fp64: no chain grows with the classes.  An exponential is off by 2 u D + 2 u, its
+    tree by 4 u; a running maximum's rescalings by 2 u each, 12 of them at most here (256 threads over 3001 classes at random,
+    six steps of the long rows), the last one's distance part of D: R = u (2 D + 32).  logp = d / T - log s, d / T and the
+    logarithm in fp64: R and its own rounding.  A gradient w (1[label] - p) / T: p off by R and the exponential's 2 u D + 6 u
+    again, 4 u of w, half a step."""
+    x, y, d, ignore = _inputs(*shape, seed=101)
+    how = dict(class_dim=d, temperature=t, ignore_index=ignore)
+    v = x.double().requires_grad_(True)
+    want, keep = ot.token_logprobs(v, y, **how)
+    weight = torch.randn(y.shape, generator=torch.Generator().manual_seed(102))
+    g64, = torch.autograd.grad((want * weight.double()).sum(), v)
+    z = _last(x.double(), d) / t
+    r = U * (2 * (z.amax(-1) - z.amin(-1)) + 32)
+    logp, stats = ops.token_logprobs(x.to(dev), y.to(dev), **how)
+    _close(logp, want.detach(), torch.where(keep, r + U * want.detach().abs(), 0.0), "logp")
+    grad = ops.token_logprobs_grad(x.to(dev), y.to(dev), stats, weight.to(dev), **how)
+    p, w = torch.softmax(z, -1), (weight.double().abs() / t).unsqueeze(-1)
+    tol = (w * (p * 2 * r.unsqueeze(-1) + 4 * U)).movedim(-1, d if d == 1 else -1)
+    _close(grad, g64, tol + HALF_STEP[x.dtype] * (g64.abs() + tol) + LEAST[x.dtype] / 2, "grad")
