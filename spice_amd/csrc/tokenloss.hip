@@ -4,8 +4,11 @@
 // Positions (n, l) of N sequences (or pictures) of L labels each carry C logits x_c.  With z = x / T, m = max x and
 // s = sum_c exp((x_c - m) / T):
 //   logp = (x_label - m) / T - log s,      d logp / d x_c = ([c == label] - exp((x_c - m) / T) / s) / T.
-// Everything is held in fp32 (sums over positions in fp64); logits are rounded nowhere, gradients once, when they are
-// stored in the logits' type.
+// Logits are rounded nowhere; an exponential is fp32, a sum of them short fp32 trees or chains (four roundings at most)
+// joined in fp64, a label's log-probability, a log ratio and what is summed over positions fp64; what leaves (logp, the
+// statistics, the factor of a position's gradient) rounds to fp32, and gradients once, when they are stored in the logits'
+// type.  (One fp32 chain a lane loses what lies 2^-25 below its sum; the trees cost 0 to 3 % of a forward pass over it, every
+// exponential added in fp64 by itself 5 to 16 %.)
 #include "common.h"
 
 #include <math.h>
@@ -958,8 +961,9 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
 // kTokThreads / RUN-th class, eight planes in flight a lane.  The groups' maxima and sums meet in LDS, where one wave
 // finishes the positions.  HOLD > 0: at most HOLD classes a group, kept for the gradient; HOLD = 0: any number, read again.
 // (One lane walking all classes: [1,150,1024] fp32 26 / 24 / 56 us forward / gradient / policy, so 6.4 / 6.0 / 13.)  Bound by
-// the bytes on large calls, 64 positions being 256 bytes a plane and load: fp32 [8,150,128x128] forward 18.8 us (4.2 TB/s),
-// gradient 28.6 (5.5), policy loss 45.7 with its count and end; [1,1000,512x512] 223 (4.7), 439 (4.8), 545.
+// the bytes on large calls, 64 positions being 256 bytes a plane and load: fp32 [8,150,128x128] forward 17.5 us (4.5 TB/s),
+// gradient 26.4 (6.0), policy loss 44.9 with its count and end; [1,1000,512x512] 191 (5.5), 424 (4.9), 529.  (Four chains a position, not a tree of the HOLD values: fp32 HOLD = 16 spilled 65 registers,
+// policy loss 60 us.)
 constexpr int kSplitTile = 64;
 
 template <typename T, int VEC, int HOLD, int MODE>
