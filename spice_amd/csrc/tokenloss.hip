@@ -962,8 +962,8 @@ __global__ __launch_bounds__(kTokThreads, VEC == 1 || CREG <= 8 ? 4 : CREG <= 24
 // finishes the positions.  HOLD > 0: at most HOLD classes a group, kept for the gradient; HOLD = 0: any number, read again.
 // (One lane walking all classes: [1,150,1024] fp32 26 / 24 / 56 us forward / gradient / policy, so 6.4 / 6.0 / 13.)  Bound by
 // the bytes on large calls, 64 positions being 256 bytes a plane and load: fp32 [8,150,128x128] forward 17.5 us (4.5 TB/s),
-// gradient 26.4 (6.0), policy loss 44.9 with its count and end; [1,1000,512x512] 191 (5.5), 424 (4.9), 529.  (Four chains a position, not a tree of the HOLD values: fp32 HOLD = 16 spilled 65 registers,
-// policy loss 60 us.)
+// gradient 26.4 (6.0), policy loss 44.9 with its count and end; [1,1000,512x512] 191 (5.5), 424 (4.9), 529.  (Four
+// chains a position, not a tree of the HOLD values: with it fp32 HOLD = 16 spilled 65 registers, policy loss 60 us.)
 constexpr int kSplitTile = 64;
 
 template <typename T, int VEC, int HOLD, int MODE>
